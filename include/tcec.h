@@ -246,6 +246,75 @@ int tcec_cgemm(int layout_a, int layout_b, int layout_c, int m, int n, int k, co
 int tcec_split(const float* in, float* hi, float* lo, size_t count, int policy, void* stream);
 
 /*
+ * Operands held in few bits.  The reference has no counterpart; these stand beside tcec_pack_* and tcec_sgemm_packed for the layers of
+ * large models, whose weights (when it answers) or kept inputs (when it trains) are too large in 32 or 16 bits.
+ *
+ * Dense matrices are FP32, f16 or bf16 (TCEC_TYPE_*), in either layout, of any alignment that their type allows.  Codes are whole
+ * numbers, which the tensor cores multiply with the dense operand exactly (FP32 in three bf16 parts); the sum over the codes that share a
+ * scale is an FP32 sum of the tensor core, and is multiplied by the scale and added to the others in FP32, rounded to nearest.  The
+ * result is rounded to its type once.  The order of all sums follows from the sizes alone, so equal calls give equal bits.
+ *
+ * Packed buffers and workspaces are the caller's, in device memory and aligned to 16 bytes; the calls allocate nothing, so each captured
+ * graph may have a workspace of its own.  A workspace may be used again as soon as the stream has passed the call.  Results must not overlap
+ * operands or workspace (TCEC_ERR_INVALID_ARGUMENT), and nothing outside a result's rows and columns is written.  Sizes may be zero; a sum over
+ * nothing, or alpha == 0, gives beta * C; beta == 0 never reads C.  The "path", tile and other options of the FP32 products have no
+ * effect here, "reserve_sms" included.  A bounded wait that ran out is reported by tcec_device_status.
+ */
+#define TCEC_TYPE_F32 0
+#define TCEC_TYPE_F16 1
+#define TCEC_TYPE_BF16 2
+
+/*
+ * Weights W (n x k) in 4 bits: W[j][i] is s (q - z) with a code q in 0..15, and a scale s (f16 or bf16) and a zero point z in 0..15 for
+ * every `group` (32, 64 or 128) consecutive k of a row; the last group may be short.
+ *
+ * tcec_pack_q4 makes the codes: with lo = min(0, smallest) and hi = max(0, largest) of the group,
+ *   s = RN16(RN32(RN32(hi - lo) / 15)), z = min(rint(-lo / s), 15), q = clamp(rint(w / s) + z, 0, 15)
+ * where rint is of the exact quotient, ties to even.  s = 0 gives a group of zeros.  A group with a value that is not finite, or whose scale
+ * does not fit type_scale, is NaN throughout.
+ * tcec_pack_q4_codes takes codes that the caller has: `codes` holds n rows of ceil(k / 2) bytes, ld_codes bytes apart, the code of an even k in
+ * the low half of its byte; `scales` n x ceil(k / group) in type_scale; `zeros` the same in bytes (their low four bits count), or NULL
+ * for z = 8.  A scale that is not finite makes its group NaN.
+ * `packed` takes tcec_q4_bytes(n, k, group) bytes (0 on bad arguments).  tcec_unpack_q4 writes the values back as a dense matrix.
+ */
+size_t tcec_q4_bytes(int n, int k, int group);
+int tcec_pack_q4(int layout_w, int n, int k, const void* w, long long ldw, int type_w, int group, int type_scale, void* packed,
+                 void* stream);
+int tcec_pack_q4_codes(int n, int k, const unsigned char* codes, long long ld_codes, const void* scales, int type_scale,
+                       const unsigned char* zeros, int group, void* packed, void* stream);
+int tcec_unpack_q4(int layout_w, int n, int k, const void* packed, int group, void* w, long long ldw, int type_w, void* stream);
+
+/*
+ * C (m x n) = alpha * X (m x k) * W^T + beta * C for weights packed as above: the product of a linear layer, from one token (a
+ * matrix-vector product, bound by the 4-bit weights) to a whole prompt.  type_c is type_x or FP32.  `workspace` takes
+ * tcec_gemm_q4_workspace_bytes(m, n, k, type_x) bytes, which is 0 for few tokens (it may then be NULL).
+ */
+size_t tcec_gemm_q4_workspace_bytes(int m, int n, int k, int type_x);
+int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, const void* x, long long ldx, int type_x,
+                 const void* packed, int group, float beta, void* c, long long ldc, int type_c, void* workspace,
+                 size_t workspace_bytes, void* stream);
+
+/*
+ * Activations X (m x k) kept in 8 bits for the backward pass: X[i][l] is s q with a code q in -127..127 and an FP32 scale s for every 128
+ * consecutive tokens (rows) of a feature (column), so that a feature of large values does not coarsen the others:
+ *   s = max(RN32(largest magnitude / 127), 2^-120), q = rint(x / s) of the exact quotient, ties to even.
+ * 128 tokens of a feature with a value that is not finite are NaN.  `packed` takes tcec_q8_bytes(m, k) bytes.
+ */
+size_t tcec_q8_bytes(int m, int k);
+int tcec_pack_q8(int layout_x, int m, int k, const void* x, long long ldx, int type_x, void* packed, void* stream);
+int tcec_unpack_q8(int layout_x, int m, int k, const void* packed, void* x, long long ldx, int type_x, void* stream);
+
+/*
+ * C (n x k) = alpha * dY^T (n x m) * X (m x k) + beta * C for activations kept as above: the gradient of a layer's weights from the
+ * gradient dY (m x n) of its outputs; beta = 1 adds up over several batches.  type_c is type_dy or FP32.
+ * `workspace` takes tcec_wgrad_q8_workspace_bytes(m, n, k, type_dy) bytes.
+ */
+size_t tcec_wgrad_q8_workspace_bytes(int m, int n, int k, int type_dy);
+int tcec_wgrad_q8(int layout_dy, int layout_c, int m, int n, int k, float alpha, const void* dy, long long lddy, int type_dy,
+                  const void* packed, float beta, void* c, long long ldc, int type_c, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
+/*
  * Options (process-wide):
  *   "promote_k"  K extent accumulated inside the tensor-core accumulator before
  *                it is added to the FP32 running sum with a round-to-nearest add.

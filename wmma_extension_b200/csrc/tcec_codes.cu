@@ -1,0 +1,458 @@
+// Host side of the entry points for operands held in few bits (include/tcec.h): argument checks, kernel selection and launches.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <initializer_list>
+#include <mutex>
+
+#include "tcec_codes.cuh"
+#include "tcec_gemm_codes.cuh"
+#include "tcec_gemv_q4.cuh"
+#include "tcec_internal.h"
+#include "tcec_launch.h"
+
+using namespace tcec_sm100;
+
+namespace tcec_host {
+namespace {
+
+static_assert(TCEC_TYPE_F32 == kTypeF32 && TCEC_TYPE_F16 == kTypeF16 && TCEC_TYPE_BF16 == kTypeBf16, "types of tcec.h");
+
+constexpr long long kMostBlocks = 0x7fffffffll;  // CTAs of a grid
+
+bool bad_type(int t) { return t < 0 || t > 2; }
+bool bad_group(int g) { return g != 32 && g != 64 && g != 128; }
+int type_bytes(int t) { return t == TCEC_TYPE_F32 ? 4 : 2; }
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+// A dense matrix of the caller.
+struct Dense {
+  int layout, rows, cols;
+  const void* p;
+  long long ld;
+  int type;
+  long long row_step() const { return layout == TCEC_ROW_MAJOR ? ld : 1; }
+  long long col_step() const { return layout == TCEC_ROW_MAJOR ? 1 : ld; }
+  bool bad() const { return bad_layout(layout) || bad_type(type) || rows < 0 || cols < 0; }
+  bool empty() const { return rows == 0 || cols == 0; }
+  // Only of one that holds elements.
+  bool bad_memory() const { return !p || !aligned(p, type_bytes(type)) || ld < (layout == TCEC_ROW_MAJOR ? cols : rows); }
+  size_t extent() const {
+    if (empty()) return 0;
+    const long long outer = layout == TCEC_ROW_MAJOR ? rows : cols, inner = layout == TCEC_ROW_MAJOR ? cols : rows;
+    return static_cast<size_t>((outer - 1) * ld + inner) * type_bytes(type);
+  }
+  // Whether its elements may be read or written `bytes` at a time from every multiple of that along a line.
+  bool wide(size_t bytes) const { return aligned(p, bytes) && (ld * type_bytes(type)) % static_cast<long long>(bytes) == 0; }
+};
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na && nb && x < y + nb && y < x + na;
+}
+
+size_t q4_bytes(int n, int k, int group) {
+  return static_cast<size_t>(ceil_div(n, kCodeRows)) * ceil_div(k, kCodeSpan) * q4_block_bytes(group);
+}
+size_t q8_bytes(int m, int k) { return static_cast<size_t>(ceil_div(k, kCodeRows)) * ceil_div(m, kCodeSpan) * kQ8BlockBytes; }
+// Panels of a dense operand: `cols` columns, `sum` along the sum.
+size_t panel_bytes(int cols, int sum, int type) {
+  return static_cast<size_t>(ceil_div(cols, kCodeRows)) * ceil_div(sum, kCodeSpan) * (type == TCEC_TYPE_F32 ? 3 : 1) * kSpanBytes;
+}
+
+template <int BN, bool F, bool Q8>
+cudaError_t set_codes_attr() {
+  const cudaError_t e = cudaFuncSetAttribute(tcec_gemm_codes_kernel<BN, F, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             GemmCodesCfg<BN, Q8>::SMEM_BYTES);
+  if (e != cudaSuccess || !GemmCodesCfg<BN, Q8>::REBALANCE) return e;
+  cudaFuncAttributes a{};  // the split of the registers among the warps is made for a launch with 128 a thread
+  const cudaError_t got = cudaFuncGetAttributes(&a, tcec_gemm_codes_kernel<BN, F, Q8>);
+  return got != cudaSuccess ? got : a.numRegs == 128 ? cudaSuccess : cudaErrorInvalidConfiguration;
+}
+template <bool F, bool Q8>
+cudaError_t set_codes_attrs() {
+  cudaError_t e = set_codes_attr<64, F, Q8>();
+  if (e == cudaSuccess) e = set_codes_attr<128, F, Q8>();
+  if (e == cudaSuccess) e = set_codes_attr<256, F, Q8>();
+  return e;
+}
+
+// What a launch needs to know of the current device.
+struct Here {
+  int* status;
+  int sm_count;
+};
+int get_here(Here* out) {
+  std::lock_guard<std::mutex> lock(state_mutex());
+  DeviceState* st = nullptr;
+  const int rc = get_device_state(&st);
+  if (rc != TCEC_OK) return rc;
+  if (!st->codes_attrs_done) {
+    TCEC_CUDA((set_codes_attrs<false, false>()));
+    TCEC_CUDA((set_codes_attrs<false, true>()));
+    TCEC_CUDA((set_codes_attrs<true, false>()));
+    TCEC_CUDA((set_codes_attrs<true, true>()));
+    st->codes_attrs_done = true;
+  }
+  *out = {st->status, st->sm_count};
+  return TCEC_OK;
+}
+
+// No exception leaves the library.
+template <class Body>
+int guarded(Body body) {
+  try {
+    return body();
+  } catch (...) {
+    return TCEC_ERR_ALLOC;
+  }
+}
+int launched() { return cudaGetLastError() == cudaSuccess ? TCEC_OK : TCEC_ERR_CUDA; }
+
+template <template <int> class Launch, class... Args>
+void by_type(int type, const Args&... args) {
+  if (type == TCEC_TYPE_F32) Launch<kTypeF32>::go(args...);
+  else if (type == TCEC_TYPE_F16) Launch<kTypeF16>::go(args...);
+  else Launch<kTypeBf16>::go(args...);
+}
+
+template <int T>
+struct PackQ4 {
+  static void go(int group, int grid, cudaStream_t stream, const PackQ4Params& p) {
+    if (group == 32) launch_early(pack_q4_kernel<T, 32>, grid, 256, 0, stream, p);
+    else if (group == 64) launch_early(pack_q4_kernel<T, 64>, grid, 256, 0, stream, p);
+    else launch_early(pack_q4_kernel<T, 128>, grid, 256, 0, stream, p);
+  }
+};
+template <int T>
+struct UnpackQ4 {
+  static void go(int group, int grid, cudaStream_t stream, const UnpackParams& p) {
+    if (group == 32) launch_early(unpack_q4_kernel<T, 32>, grid, 256, 0, stream, p);
+    else if (group == 64) launch_early(unpack_q4_kernel<T, 64>, grid, 256, 0, stream, p);
+    else launch_early(unpack_q4_kernel<T, 128>, grid, 256, 0, stream, p);
+  }
+};
+template <int T>
+struct PackQ8 {
+  static void go(int grid, cudaStream_t stream, const PackQ8Params& p) { launch_early(pack_q8_kernel<T>, grid, 256, 0, stream, p); }
+};
+template <int T>
+struct UnpackQ8 {
+  static void go(int grid, cudaStream_t stream, const UnpackParams& p) { launch_early(unpack_q8_kernel<T>, grid, 256, 0, stream, p); }
+};
+template <int T>
+struct StagePanels {
+  static void go(int grid, cudaStream_t stream, const StagePanelsParams& p) { launch_early(stage_panels_kernel<T>, grid, 256, 0, stream, p); }
+};
+template <int T>
+struct GemvQ4 {
+  template <int G>
+  static void of_group(int columns, cudaStream_t stream, const GemvQ4Params& p) {
+    if (columns <= 8) launch_early(gemv_q4_kernel<T, G, 1, 1>, static_cast<int>(ceil_div(p.n, 16)), 256, 0, stream, p);
+    else if (columns <= 16) launch_early(gemv_q4_kernel<T, G, 2, 2>, static_cast<int>(ceil_div(p.n, 32)), 256, 0, stream, p);
+    else launch_early(gemv_q4_kernel<T, G, 4, 2>, static_cast<int>(ceil_div(p.n, 32)), 256, 0, stream, p);
+  }
+  static void go(int group, int columns, cudaStream_t stream, const GemvQ4Params& p) {
+    if (group == 32) of_group<32>(columns, stream, p);
+    else if (group == 64) of_group<64>(columns, stream, p);
+    else of_group<128>(columns, stream, p);
+  }
+};
+
+template <int BN, bool F, bool Q8>
+void launch_codes_as(const GemmCodesParams& gp, int shares, cudaStream_t stream) {
+  launch_clusters(tcec_gemm_codes_kernel<BN, F, Q8>, shares, gp.row_tiles * gp.col_tiles * shares, 512, GemmCodesCfg<BN, Q8>::SMEM_BYTES,
+                  stream, gp);
+}
+template <bool F, bool Q8>
+void launch_codes(int bn, const GemmCodesParams& gp, int shares, cudaStream_t stream) {
+  if (bn == 64) launch_codes_as<64, F, Q8>(gp, shares, stream);
+  else if (bn == 128) launch_codes_as<128, F, Q8>(gp, shares, stream);
+  else launch_codes_as<256, F, Q8>(gp, shares, stream);
+}
+
+// D[row][col] of tcec_gemm_codes.cuh for an operand of codes and a dense one whose columns and sum lie at the given steps.
+int gemm_codes(bool q8, const void* codes, int spans, int rows, int cols, int sum, const void* dense, long long col_step, long long sum_step,
+               int type, bool vec, float alpha, float beta, void* c, long long c_row, long long c_col, int c_type, void* workspace,
+               const Here& here, cudaStream_t stream) {
+  const int parts = type == TCEC_TYPE_F32 ? 3 : 1, blocks = static_cast<int>(ceil_div(sum, kCodeSpan));
+  if (blocks) {
+    StagePanelsParams sp{};
+    sp.src = dense;
+    sp.col_step = col_step;
+    sp.sum_step = sum_step;
+    sp.cols = cols;
+    sp.sum = sum;
+    sp.blocks = blocks;
+    sp.panels = static_cast<uint8_t*>(workspace);
+    sp.vec = vec;
+    by_type<StagePanels>(type, static_cast<int>(ceil_div(cols, kCodeRows) * blocks), stream, sp);
+  }
+  GemmCodesParams gp{};
+  gp.codes = static_cast<const uint8_t*>(codes);
+  gp.panels = static_cast<const uint8_t*>(workspace);
+  gp.rows = rows;
+  gp.cols = cols;
+  gp.blocks = blocks;
+  gp.parts = parts;
+  gp.spans = spans;
+  gp.row_tiles = static_cast<int>(ceil_div(rows, 128));
+  gp.alpha = alpha;
+  gp.beta = beta;
+  gp.c = c;
+  gp.c_row = c_row;
+  gp.c_col = c_col;
+  gp.c_type = c_type;
+  gp.status = here.status;
+  int bn = cols <= 64 ? 64 : 128;
+  if (cols > 128 && gp.row_tiles * ceil_div(cols, 256) >= 100) bn = 256;
+  gp.col_tiles = static_cast<int>(ceil_div(cols, bn));
+  const long long tiles = static_cast<long long>(gp.row_tiles) * gp.col_tiles;
+  int shares = 1;
+  while (bn < 256 && shares < 8 && tiles * shares * 2 <= 148 && blocks >= 4 * shares) shares *= 2;
+  if (tiles * shares > kMostBlocks) return TCEC_ERR_UNSUPPORTED;
+  if (type == TCEC_TYPE_F16) {
+    if (q8) launch_codes<true, true>(bn, gp, shares, stream);
+    else launch_codes<true, false>(bn, gp, shares, stream);
+  } else {
+    if (q8) launch_codes<false, true>(bn, gp, shares, stream);
+    else launch_codes<false, false>(bn, gp, shares, stream);
+  }
+  return launched();
+}
+
+// Columns of the tensor-core operand that this many tokens take, and whether they are so few that the weights are streamed through
+// registers (tcec_gemv_q4.cuh).
+long long columns_of(int m, int type) { return static_cast<long long>(m) * (type == TCEC_TYPE_F32 ? 3 : 1); }
+bool streamed(int m, int type) { return columns_of(m, type) <= 32; }
+
+}  // namespace
+}  // namespace tcec_host
+
+using namespace tcec_host;
+
+extern "C" {
+
+size_t tcec_q4_bytes(int n, int k, int group) { return n < 0 || k < 0 || bad_group(group) ? 0 : q4_bytes(n, k, group); }
+
+int tcec_pack_q4(int layout_w, int n, int k, const void* w, long long ldw, int type_w, int group, int type_scale, void* packed, void* stream) {
+  return guarded([&]() -> int {
+    const Dense d{layout_w, n, k, w, ldw, type_w};
+    if (d.bad() || bad_group(group) || (type_scale != TCEC_TYPE_F16 && type_scale != TCEC_TYPE_BF16)) return TCEC_ERR_INVALID_ARGUMENT;
+    if (d.empty()) return TCEC_OK;
+    if (d.bad_memory() || !packed || !aligned(packed, 16) || overlap(w, d.extent(), packed, q4_bytes(n, k, group))) return TCEC_ERR_INVALID_ARGUMENT;
+    const long long tiles = ceil_div(n, kCodeRows), blocks = ceil_div(k, kCodeSpan);
+    if (tiles * blocks > kMostBlocks) return TCEC_ERR_UNSUPPORTED;
+    Here here;
+    const int rc = get_here(&here);
+    if (rc != TCEC_OK) return rc;
+    PackQ4Params p{};
+    p.w = w;
+    p.row_step = d.row_step();
+    p.k_step = d.col_step();
+    p.n = n;
+    p.k = k;
+    p.scale_bf16 = type_scale == TCEC_TYPE_BF16;
+    p.packed = static_cast<uint8_t*>(packed);
+    p.blocks = static_cast<int>(blocks);
+    p.vec = layout_w == TCEC_ROW_MAJOR && d.wide(4 * type_bytes(type_w));
+    by_type<PackQ4>(type_w, group, static_cast<int>(tiles * blocks), static_cast<cudaStream_t>(stream), p);
+    return launched();
+  });
+}
+
+int tcec_pack_q4_codes(int n, int k, const unsigned char* codes, long long ld_codes, const void* scales, int type_scale,
+                       const unsigned char* zeros, int group, void* packed, void* stream) {
+  return guarded([&]() -> int {
+    if (n < 0 || k < 0 || bad_group(group) || (type_scale != TCEC_TYPE_F16 && type_scale != TCEC_TYPE_BF16)) return TCEC_ERR_INVALID_ARGUMENT;
+    if (n == 0 || k == 0) return TCEC_OK;
+    if (!codes || !scales || !aligned(scales, 2) || ld_codes < ceil_div(k, 2) || !packed || !aligned(packed, 16)) return TCEC_ERR_INVALID_ARGUMENT;
+    const long long tiles = ceil_div(n, kCodeRows), blocks = ceil_div(k, kCodeSpan), groups = ceil_div(k, group);
+    const size_t out = q4_bytes(n, k, group);
+    if (overlap(codes, static_cast<size_t>((n - 1) * ld_codes + ceil_div(k, 2)), packed, out) ||
+        overlap(scales, static_cast<size_t>(n) * groups * 2, packed, out) ||
+        (zeros && overlap(zeros, static_cast<size_t>(n) * groups, packed, out)))
+      return TCEC_ERR_INVALID_ARGUMENT;
+    if (tiles * blocks > kMostBlocks) return TCEC_ERR_UNSUPPORTED;
+    Here here;
+    const int rc = get_here(&here);
+    if (rc != TCEC_OK) return rc;
+    PackQ4Params p{};
+    p.n = n;
+    p.k = k;
+    p.scale_bf16 = type_scale == TCEC_TYPE_BF16;
+    p.packed = static_cast<uint8_t*>(packed);
+    p.blocks = static_cast<int>(blocks);
+    p.codes = codes;
+    p.codes_ld = ld_codes;
+    p.scales = scales;
+    p.zeros = zeros;
+    p.groups = static_cast<int>(groups);
+    const int grid = static_cast<int>(tiles * blocks);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (group == 32) launch_early(pack_q4_codes_kernel<32>, grid, 256, 0, s, p);
+    else if (group == 64) launch_early(pack_q4_codes_kernel<64>, grid, 256, 0, s, p);
+    else launch_early(pack_q4_codes_kernel<128>, grid, 256, 0, s, p);
+    return launched();
+  });
+}
+
+int tcec_unpack_q4(int layout_w, int n, int k, const void* packed, int group, void* w, long long ldw, int type_w, void* stream) {
+  return guarded([&]() -> int {
+    const Dense d{layout_w, n, k, w, ldw, type_w};
+    if (d.bad() || bad_group(group)) return TCEC_ERR_INVALID_ARGUMENT;
+    if (d.empty()) return TCEC_OK;
+    if (d.bad_memory() || !packed || !aligned(packed, 16) || overlap(w, d.extent(), packed, q4_bytes(n, k, group))) return TCEC_ERR_INVALID_ARGUMENT;
+    const long long tiles = ceil_div(n, kCodeRows), blocks = ceil_div(k, kCodeSpan);
+    if (tiles * blocks > kMostBlocks) return TCEC_ERR_UNSUPPORTED;
+    Here here;
+    const int rc = get_here(&here);
+    if (rc != TCEC_OK) return rc;
+    UnpackParams p{};
+    p.packed = static_cast<const uint8_t*>(packed);
+    p.out = w;
+    p.row_step = d.row_step();
+    p.sum_step = d.col_step();
+    p.rows = n;
+    p.sum = k;
+    p.blocks = static_cast<int>(blocks);
+    p.vec = layout_w == TCEC_ROW_MAJOR && d.wide(4 * type_bytes(type_w));
+    by_type<UnpackQ4>(type_w, group, static_cast<int>(tiles * blocks), static_cast<cudaStream_t>(stream), p);
+    return launched();
+  });
+}
+
+size_t tcec_gemm_q4_workspace_bytes(int m, int n, int k, int type_x) {
+  return m < 0 || n < 0 || k < 0 || bad_type(type_x) || streamed(m, type_x) ? 0 : panel_bytes(m, k, type_x);
+}
+
+int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, const void* x, long long ldx, int type_x, const void* packed,
+                 int group, float beta, void* c, long long ldc, int type_c, void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&]() -> int {
+    const Dense dx{layout_x, m, k, x, ldx, type_x}, dc{layout_c, m, n, c, ldc, type_c};
+    if (dx.bad() || dc.bad() || bad_group(group) || (type_c != type_x && type_c != TCEC_TYPE_F32)) return TCEC_ERR_INVALID_ARGUMENT;
+    if (dc.empty()) return TCEC_OK;
+    if (dc.bad_memory()) return TCEC_ERR_INVALID_ARGUMENT;
+    const int sum = alpha == 0.f ? 0 : k;  // as without a product, X and W are then not read
+    const size_t scratch = sum ? tcec_gemm_q4_workspace_bytes(m, n, sum, type_x) : 0;
+    if (sum) {
+      if (dx.bad_memory() || !packed || !aligned(packed, 16) || workspace_bytes < scratch || (scratch && (!workspace || !aligned(workspace, 16))))
+        return TCEC_ERR_INVALID_ARGUMENT;
+      if (overlap(c, dc.extent(), x, dx.extent()) || overlap(c, dc.extent(), packed, q4_bytes(n, k, group)) ||
+          overlap(workspace, scratch, x, dx.extent()) || overlap(workspace, scratch, c, dc.extent()) ||
+          overlap(workspace, scratch, packed, q4_bytes(n, k, group)))
+        return TCEC_ERR_INVALID_ARGUMENT;
+    }
+    if (ceil_div(m, kCodeRows) * ceil_div(k, kCodeSpan) > kMostBlocks) return TCEC_ERR_UNSUPPORTED;
+    Here here;
+    const int rc = get_here(&here);
+    if (rc != TCEC_OK) return rc;
+    const bool vec = layout_x == TCEC_ROW_MAJOR && dx.wide(16);
+    if (!streamed(m, type_x))
+      return gemm_codes(false, packed, kCodeSpan / group, n, m, sum, x, dx.row_step(), dx.col_step(), type_x, vec, alpha, beta, c, dc.col_step(),
+                        dc.row_step(), type_c, workspace, here, static_cast<cudaStream_t>(stream));
+    GemvQ4Params p{};
+    p.codes = static_cast<const uint8_t*>(packed);
+    p.x = x;
+    p.x_token = dx.row_step();
+    p.x_k = dx.col_step();
+    p.n = n;
+    p.k = sum;
+    p.tokens = m;
+    p.blocks = static_cast<int>(ceil_div(sum, kCodeSpan));
+    p.vec = vec;
+    p.alpha = alpha;
+    p.beta = beta;
+    p.c = c;
+    p.c_token = dc.row_step();
+    p.c_row = dc.col_step();
+    p.c_type = type_c;
+    by_type<GemvQ4>(type_x, group, static_cast<int>(columns_of(m, type_x)), static_cast<cudaStream_t>(stream), p);
+    return launched();
+  });
+}
+
+size_t tcec_q8_bytes(int m, int k) { return m < 0 || k < 0 ? 0 : q8_bytes(m, k); }
+
+int tcec_pack_q8(int layout_x, int m, int k, const void* x, long long ldx, int type_x, void* packed, void* stream) {
+  return guarded([&]() -> int {
+    const Dense d{layout_x, m, k, x, ldx, type_x};
+    if (d.bad()) return TCEC_ERR_INVALID_ARGUMENT;
+    if (d.empty()) return TCEC_OK;
+    if (d.bad_memory() || !packed || !aligned(packed, 16) || overlap(x, d.extent(), packed, q8_bytes(m, k))) return TCEC_ERR_INVALID_ARGUMENT;
+    const long long tiles = ceil_div(k, kCodeRows), blocks = ceil_div(m, kCodeSpan);
+    if (tiles * blocks > kMostBlocks) return TCEC_ERR_UNSUPPORTED;
+    Here here;
+    const int rc = get_here(&here);
+    if (rc != TCEC_OK) return rc;
+    PackQ8Params p{};
+    p.x = x;
+    p.token_step = d.row_step();
+    p.feature_step = d.col_step();
+    p.tokens = m;
+    p.features = k;
+    p.token_blocks = static_cast<int>(blocks);
+    p.packed = static_cast<uint8_t*>(packed);
+    p.vec = layout_x == TCEC_ROW_MAJOR && d.wide(4 * type_bytes(type_x));
+    by_type<PackQ8>(type_x, static_cast<int>(tiles * blocks), static_cast<cudaStream_t>(stream), p);
+    return launched();
+  });
+}
+
+int tcec_unpack_q8(int layout_x, int m, int k, const void* packed, void* x, long long ldx, int type_x, void* stream) {
+  return guarded([&]() -> int {
+    const Dense d{layout_x, m, k, x, ldx, type_x};
+    if (d.bad()) return TCEC_ERR_INVALID_ARGUMENT;
+    if (d.empty()) return TCEC_OK;
+    if (d.bad_memory() || !packed || !aligned(packed, 16) || overlap(x, d.extent(), packed, q8_bytes(m, k))) return TCEC_ERR_INVALID_ARGUMENT;
+    const long long tiles = ceil_div(k, kCodeRows), blocks = ceil_div(m, kCodeSpan);
+    if (tiles * blocks > kMostBlocks) return TCEC_ERR_UNSUPPORTED;
+    Here here;
+    const int rc = get_here(&here);
+    if (rc != TCEC_OK) return rc;
+    UnpackParams p{};
+    p.packed = static_cast<const uint8_t*>(packed);
+    p.out = x;
+    p.row_step = d.col_step();  // rows of the codes are features
+    p.sum_step = d.row_step();
+    p.rows = k;
+    p.sum = m;
+    p.blocks = static_cast<int>(blocks);
+    p.vec = layout_x == TCEC_ROW_MAJOR && d.wide(4 * type_bytes(type_x));
+    by_type<UnpackQ8>(type_x, static_cast<int>(tiles * blocks), static_cast<cudaStream_t>(stream), p);
+    return launched();
+  });
+}
+
+size_t tcec_wgrad_q8_workspace_bytes(int m, int n, int k, int type_dy) {
+  return m < 0 || n < 0 || k < 0 || bad_type(type_dy) ? 0 : panel_bytes(n, m, type_dy);
+}
+
+int tcec_wgrad_q8(int layout_dy, int layout_c, int m, int n, int k, float alpha, const void* dy, long long lddy, int type_dy, const void* packed,
+                  float beta, void* c, long long ldc, int type_c, void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&]() -> int {
+    const Dense dd{layout_dy, m, n, dy, lddy, type_dy}, dc{layout_c, n, k, c, ldc, type_c};
+    if (dd.bad() || dc.bad() || (type_c != type_dy && type_c != TCEC_TYPE_F32)) return TCEC_ERR_INVALID_ARGUMENT;
+    if (dc.empty()) return TCEC_OK;
+    if (dc.bad_memory()) return TCEC_ERR_INVALID_ARGUMENT;
+    const int sum = alpha == 0.f ? 0 : m;
+    const size_t scratch = sum ? tcec_wgrad_q8_workspace_bytes(sum, n, k, type_dy) : 0;
+    if (sum) {
+      if (dd.bad_memory() || !packed || !aligned(packed, 16) || workspace_bytes < scratch || !workspace || !aligned(workspace, 16))
+        return TCEC_ERR_INVALID_ARGUMENT;
+      if (overlap(c, dc.extent(), dy, dd.extent()) || overlap(c, dc.extent(), packed, q8_bytes(m, k)) ||
+          overlap(workspace, scratch, dy, dd.extent()) || overlap(workspace, scratch, c, dc.extent()) ||
+          overlap(workspace, scratch, packed, q8_bytes(m, k)))
+        return TCEC_ERR_INVALID_ARGUMENT;
+    }
+    if (ceil_div(n, kCodeRows) * ceil_div(m, kCodeSpan) > kMostBlocks) return TCEC_ERR_UNSUPPORTED;
+    Here here;
+    const int rc = get_here(&here);
+    if (rc != TCEC_OK) return rc;
+    // columns: the outputs of the layer; the sum: tokens
+    return gemm_codes(true, packed, 1, k, n, sum, dy, dd.col_step(), dd.row_step(), type_dy, layout_dy == TCEC_COL_MAJOR && dd.wide(16), alpha,
+                      beta, c, dc.col_step(), dc.row_step(), type_c, workspace, here, static_cast<cudaStream_t>(stream));
+  });
+}
+
+}  // extern "C"

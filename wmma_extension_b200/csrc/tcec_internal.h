@@ -62,6 +62,7 @@ struct DeviceState {
   int sm_count = 0;
   int cluster_slots[3] = {};  // clusters of 2, 4, 8 CTAs that run at a time (count_cluster_slots); only whether any do counts
   bool attrs_done = false;
+  bool codes_attrs_done = false;                // likewise of the kernels of tcec_codes.cu
   std::map<cudaStream_t, Workspace> ws;
   std::map<cudaStream_t, unsigned int*> sched;  // per stream: the panel GEMM's two tile-scheduler counters
   uint8_t* pair_lines = nullptr;                // kPairLines lines in the allocation of `status`

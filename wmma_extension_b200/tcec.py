@@ -25,6 +25,7 @@ ROW_MAJOR, COL_MAJOR = 0, 1
 POLICIES = {"fp16_ec": 0, "tf32_ec": 1, "fp16_no_ec": 2, "tf32_no_ec": 3}
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_CUDA, ERR_TIMEOUT, ERR_ALLOC, ERR_TOO_LARGE, ERR_COMM = range(8)
 COMM_ID_BYTES = 128
+TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # of the dense operands of products on operands held in few bits
 
 EXPORTED_SYMBOLS = (
     "tcec_sgemm",
@@ -35,6 +36,17 @@ EXPORTED_SYMBOLS = (
     "tcec_pack_a",
     "tcec_pack_b",
     "tcec_sgemm_packed",
+    "tcec_q4_bytes",
+    "tcec_pack_q4",
+    "tcec_pack_q4_codes",
+    "tcec_unpack_q4",
+    "tcec_gemm_q4_workspace_bytes",
+    "tcec_gemm_q4",
+    "tcec_q8_bytes",
+    "tcec_pack_q8",
+    "tcec_unpack_q8",
+    "tcec_wgrad_q8_workspace_bytes",
+    "tcec_wgrad_q8",
     "tcec_split",
     "tcec_cgemm",
     "tcec_sgemm_cublas",
@@ -140,6 +152,28 @@ def load() -> ctypes.CDLL:
     lib.tcec_sgemm_column_shard_host.restype = i
     lib.tcec_cgemm.argtypes = [i, i, i, i, i, i, fp, p, ll, p, ll, fp, p, ll, i, p]
     lib.tcec_cgemm.restype = i
+    lib.tcec_q4_bytes.argtypes = [i, i, i]
+    lib.tcec_q4_bytes.restype = sz
+    lib.tcec_pack_q4.argtypes = [i, i, i, p, ll, i, i, i, p, p]
+    lib.tcec_pack_q4.restype = i
+    lib.tcec_pack_q4_codes.argtypes = [i, i, p, ll, p, i, p, i, p, p]
+    lib.tcec_pack_q4_codes.restype = i
+    lib.tcec_unpack_q4.argtypes = [i, i, i, p, i, p, ll, i, p]
+    lib.tcec_unpack_q4.restype = i
+    lib.tcec_gemm_q4_workspace_bytes.argtypes = [i, i, i, i]
+    lib.tcec_gemm_q4_workspace_bytes.restype = sz
+    lib.tcec_gemm_q4.argtypes = [i, i, i, i, i, f, p, ll, i, p, i, f, p, ll, i, p, sz, p]
+    lib.tcec_gemm_q4.restype = i
+    lib.tcec_q8_bytes.argtypes = [i, i]
+    lib.tcec_q8_bytes.restype = sz
+    lib.tcec_pack_q8.argtypes = [i, i, i, p, ll, i, p, p]
+    lib.tcec_pack_q8.restype = i
+    lib.tcec_unpack_q8.argtypes = [i, i, i, p, p, ll, i, p]
+    lib.tcec_unpack_q8.restype = i
+    lib.tcec_wgrad_q8_workspace_bytes.argtypes = [i, i, i, i]
+    lib.tcec_wgrad_q8_workspace_bytes.restype = sz
+    lib.tcec_wgrad_q8.argtypes = [i, i, i, i, i, f, p, ll, i, p, f, p, ll, i, p, sz, p]
+    lib.tcec_wgrad_q8.restype = i
     lib.tcec_split.argtypes = [p, p, p, sz, i, p]
     lib.tcec_split.restype = i
     lib.tcec_set_option.argtypes = [ctypes.c_char_p, i]
@@ -463,6 +497,213 @@ def sgemm_packed(a_packed: torch.Tensor, b_packed: torch.Tensor, m: int, n: int,
         st = load().tcec_sgemm_packed(lc, m, n, k, alpha, a_packed.data_ptr(), b_packed.data_ptr(), beta,
                                       c.data_ptr(), ldc, _policy(policy), _stream_ptr())
     _check(st, "tcec_sgemm_packed")
+    return c
+
+
+# ---------------------------------------------------------------- operands held in few bits
+def _dense_type(t: torch.Tensor, what: str) -> int:
+    """The type of a dense operand: a matrix in float32, float16 or bfloat16 on a GPU."""
+    if not t.is_cuda or t.dtype not in TYPES or t.dim() != 2:
+        raise ValueError(f"{what} must be a float32, float16 or bfloat16 CUDA matrix")
+    return TYPES[t.dtype]
+
+
+def _result_type(dtype: torch.dtype, operand: torch.Tensor) -> int:
+    if dtype != operand.dtype and dtype != torch.float32:
+        raise ValueError(f"the result is float32 or of the operand's type {operand.dtype}, not {dtype}")
+    return TYPES[dtype]
+
+
+def _exact_result(c: Optional[torch.Tensor], shape, dtype: Optional[torch.dtype], operand: torch.Tensor, beta: float) -> torch.Tensor:
+    """`c` as given, or a new one of `dtype` (the operand's type by default)."""
+    if c is None:
+        if beta != 0.0:
+            raise ValueError("beta needs a c")
+        return operand.new_empty(shape, dtype=dtype or operand.dtype)
+    if dtype is not None and c.dtype != dtype:
+        raise ValueError(f"c is {c.dtype}, not {dtype}")
+    if not c.is_cuda or tuple(c.shape) != tuple(shape):
+        raise ValueError(f"c must be a CUDA matrix of {tuple(shape)}")
+    _require_one_device(c, operand)
+    return c
+
+
+def _require_bytes(t: torch.Tensor, need: int, what: str) -> None:
+    if not t.is_cuda or not t.is_contiguous() or t.numel() * t.element_size() < need:
+        raise ValueError(f"{what} takes {need} consecutive bytes on a GPU")
+
+
+def _scratch(need: int, device) -> Optional[torch.Tensor]:
+    """From torch's allocator, so that a captured graph has its own."""
+    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def q4_bytes(n: int, k: int, group: int = 128) -> int:
+    """Bytes of weights (n x k) packed by pack_q4 or pack_q4_codes."""
+    if group not in (32, 64, 128):
+        raise ValueError("group must be 32, 64 or 128")
+    return int(load().tcec_q4_bytes(n, k, group))
+
+
+def pack_q4(w: torch.Tensor, group: int = 128, scale: torch.dtype = torch.float16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Weights w (n x k, outputs first) in 4 bits, with a scale (float16 or bfloat16) and a zero point for every `group` of k.
+
+    Returns the uint8 buffer that gemm_q4 takes.  Every value is brought to the nearest of its group's 16 steps
+    (``tcec_pack_q4``); unpack_q4 gives the values that the codes stand for.
+    """
+    kind = _dense_type(w, "w")
+    if scale not in (torch.float16, torch.bfloat16):
+        raise ValueError("scale must be float16 or bfloat16")
+    n, k = w.shape
+    need = q4_bytes(n, k, group)
+    lw, ldw = _layout_ld(w)
+    if out is None:
+        out = torch.empty(need, dtype=torch.uint8, device=w.device)
+    _require_bytes(out, need, "packed weights of this size")
+    _require_one_device(w, out)
+    with _on(w.device):
+        st = load().tcec_pack_q4(lw, n, k, w.data_ptr(), ldw, kind, group, TYPES[scale], out.data_ptr(), _stream_ptr())
+    _check(st, "tcec_pack_q4")
+    return out
+
+
+def pack_q4_codes(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *, k: int, group: int = 128,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Lays out 4-bit codes that exist already: w[j, i] = scales[j, i // group] * (code - zeros[j, i // group]).
+
+    ``codes``: uint8 [n, ceil(k / 2)], the code of an even i in the low half of its byte; ``scales``: float16 or bfloat16
+    [n, ceil(k / group)]; ``zeros``: uint8 of the same shape, or None for 8.
+    """
+    if not codes.is_cuda or codes.dtype != torch.uint8 or codes.dim() != 2 or k < 0 or codes.shape[1] != (k + 1) // 2:
+        raise ValueError("codes must be a uint8 CUDA matrix of ceil(k / 2) columns")
+    n = codes.shape[0]
+    need = q4_bytes(n, k, group)
+    shape = (n, -(-k // group))
+    if not scales.is_cuda or scales.dtype not in (torch.float16, torch.bfloat16) or tuple(scales.shape) != shape:
+        raise ValueError(f"scales must be a float16 or bfloat16 CUDA matrix of {shape}")
+    if zeros is not None and (not zeros.is_cuda or zeros.dtype != torch.uint8 or tuple(zeros.shape) != shape):
+        raise ValueError(f"zeros must be a uint8 CUDA matrix of {shape}")
+    if codes.stride(1) != 1 or (n > 1 and codes.stride(0) < codes.shape[1]):
+        codes = codes.contiguous()
+    scales = scales.contiguous()
+    zeros = None if zeros is None else zeros.contiguous()
+    if out is None:
+        out = torch.empty(need, dtype=torch.uint8, device=codes.device)
+    _require_bytes(out, need, "packed weights of this size")
+    _require_one_device(codes, scales, out, *(() if zeros is None else (zeros,)))
+    with _on(codes.device):
+        st = load().tcec_pack_q4_codes(n, k, codes.data_ptr(), max(codes.stride(0), codes.shape[1]), scales.data_ptr(),
+                                       TYPES[scales.dtype], _ptr(zeros), group, out.data_ptr(), _stream_ptr())
+    _check(st, "tcec_pack_q4_codes")
+    return out
+
+
+def unpack_q4(packed: torch.Tensor, n: int, k: int, group: int = 128, dtype: torch.dtype = torch.float32,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The weights (n x k) that a packed buffer stands for, rounded to the result's type."""
+    need = q4_bytes(n, k, group)
+    _require_bytes(packed, need, "packed weights of this size")
+    if out is None:
+        out = torch.empty((n, k), dtype=dtype, device=packed.device)
+    kind = _dense_type(out, "the result")
+    if tuple(out.shape) != (n, k):
+        raise ValueError(f"the result must be {(n, k)}")
+    _require_one_device(packed, out)
+    lw, ldw = _layout_ld(out)
+    with _on(packed.device):
+        st = load().tcec_unpack_q4(lw, n, k, packed.data_ptr(), group, out.data_ptr(), ldw, kind, _stream_ptr())
+    _check(st, "tcec_unpack_q4")
+    return out
+
+
+def gemm_q4(x: torch.Tensor, packed: torch.Tensor, n: int, c: Optional[torch.Tensor] = None, *, group: int = 128, alpha: float = 1.0,
+            beta: float = 0.0, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """C = alpha * X @ W^T + beta * C for X (m x k, float32, float16 or bfloat16) and weights W (n x k) packed by pack_q4.
+
+    From one token to a whole prompt.  The result is of X's type, or of ``dtype`` (X's or float32).
+    """
+    kind = _dense_type(x, "x")
+    m, k = x.shape
+    need = q4_bytes(n, k, group)
+    _require_bytes(packed, need, "packed weights of this size")
+    c = _exact_result(c, (m, n), dtype, x, beta)
+    kind_c = _result_type(c.dtype, x)
+    _require_one_device(x, packed)
+    lx, ldx = _layout_ld(x)
+    lc, ldc = _layout_ld(c)
+    lib = load()
+    with _on(x.device):
+        need = int(lib.tcec_gemm_q4_workspace_bytes(m, n, k, kind))
+        scratch = _scratch(need, x.device)
+        st = lib.tcec_gemm_q4(lx, lc, m, n, k, alpha, x.data_ptr(), ldx, kind, packed.data_ptr(), group, beta, c.data_ptr(), ldc, kind_c,
+                              _ptr(scratch), need, _stream_ptr())
+    _check(st, "tcec_gemm_q4")
+    return c
+
+
+def q8_bytes(m: int, k: int) -> int:
+    """Bytes of activations (m x k) packed by pack_q8."""
+    return int(load().tcec_q8_bytes(m, k))
+
+
+def pack_q8(x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Activations x (m tokens x k features) in 8 bits, with a scale for every 128 tokens of a feature, to be kept for wgrad_q8."""
+    kind = _dense_type(x, "x")
+    m, k = x.shape
+    need = q8_bytes(m, k)
+    lx, ldx = _layout_ld(x)
+    if out is None:
+        out = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _require_bytes(out, need, "packed activations of this size")
+    _require_one_device(x, out)
+    with _on(x.device):
+        st = load().tcec_pack_q8(lx, m, k, x.data_ptr(), ldx, kind, out.data_ptr(), _stream_ptr())
+    _check(st, "tcec_pack_q8")
+    return out
+
+
+def unpack_q8(packed: torch.Tensor, m: int, k: int, dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The activations (m x k) that a packed buffer stands for, rounded to the result's type."""
+    _require_bytes(packed, q8_bytes(m, k), "packed activations of this size")
+    if out is None:
+        out = torch.empty((m, k), dtype=dtype, device=packed.device)
+    kind = _dense_type(out, "the result")
+    if tuple(out.shape) != (m, k):
+        raise ValueError(f"the result must be {(m, k)}")
+    _require_one_device(packed, out)
+    lx, ldx = _layout_ld(out)
+    with _on(packed.device):
+        st = load().tcec_unpack_q8(lx, m, k, packed.data_ptr(), out.data_ptr(), ldx, kind, _stream_ptr())
+    _check(st, "tcec_unpack_q8")
+    return out
+
+
+def wgrad_q8(dy: torch.Tensor, packed: torch.Tensor, k: int, c: Optional[torch.Tensor] = None, *, alpha: float = 1.0, beta: float = 0.0,
+             dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """C = alpha * dY^T @ X + beta * C: the gradient (n x k) of a layer's weights from the gradient dY (m x n, float32, float16 or
+    bfloat16) of its outputs and its input X (m x k), kept by pack_q8.  beta = 1 adds up over batches.
+
+    The result is of dY's type, or of ``dtype`` (dY's or float32).
+    """
+    kind = _dense_type(dy, "dy")
+    m, n = dy.shape
+    _require_bytes(packed, q8_bytes(m, k), "packed activations of this size")
+    c = _exact_result(c, (n, k), dtype, dy, beta)
+    kind_c = _result_type(c.dtype, dy)
+    _require_one_device(dy, packed)
+    ly, ldy = _layout_ld(dy)
+    lc, ldc = _layout_ld(c)
+    lib = load()
+    with _on(dy.device):
+        need = int(lib.tcec_wgrad_q8_workspace_bytes(m, n, k, kind))
+        scratch = _scratch(need, dy.device)
+        st = lib.tcec_wgrad_q8(ly, lc, m, n, k, alpha, dy.data_ptr(), ldy, kind, packed.data_ptr(), beta, c.data_ptr(), ldc, kind_c,
+                               _ptr(scratch), need, _stream_ptr())
+    _check(st, "tcec_wgrad_q8")
     return c
 
 
