@@ -60,20 +60,28 @@ size_t panel_bytes(int cols, int sum, int type) {
   return static_cast<size_t>(ceil_div(cols, kCodeRows)) * ceil_div(sum, kCodeSpan) * (type == TCEC_TYPE_F32 ? 3 : 1) * kSpanBytes;
 }
 
-template <int BN, bool F, bool Q8>
+template <int BN, bool F, int S>
 cudaError_t set_codes_attr() {
-  const cudaError_t e = cudaFuncSetAttribute(tcec_gemm_codes_kernel<BN, F, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             GemmCodesCfg<BN, Q8>::SMEM_BYTES);
-  if (e != cudaSuccess || !GemmCodesCfg<BN, Q8>::REBALANCE) return e;
+  const cudaError_t e = cudaFuncSetAttribute(tcec_gemm_codes_kernel<BN, F, S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             GemmCodesCfg<BN, S>::SMEM_BYTES);
+  if (e != cudaSuccess || !GemmCodesCfg<BN, S>::REBALANCE) return e;
   cudaFuncAttributes a{};  // the split of the registers among the warps is made for a launch with 128 a thread
-  const cudaError_t got = cudaFuncGetAttributes(&a, tcec_gemm_codes_kernel<BN, F, Q8>);
+  const cudaError_t got = cudaFuncGetAttributes(&a, tcec_gemm_codes_kernel<BN, F, S>);
   return got != cudaSuccess ? got : a.numRegs == 128 ? cudaSuccess : cudaErrorInvalidConfiguration;
 }
-template <bool F, bool Q8>
+template <bool F, int S>
 cudaError_t set_codes_attrs() {
-  cudaError_t e = set_codes_attr<64, F, Q8>();
-  if (e == cudaSuccess) e = set_codes_attr<128, F, Q8>();
-  if (e == cudaSuccess) e = set_codes_attr<256, F, Q8>();
+  cudaError_t e = set_codes_attr<64, F, S>();
+  if (e == cudaSuccess) e = set_codes_attr<128, F, S>();
+  if (e == cudaSuccess) e = set_codes_attr<256, F, S>();
+  return e;
+}
+template <bool F>
+cudaError_t set_all_codes_attrs() {
+  cudaError_t e = set_codes_attrs<F, 0>();
+  if (e == cudaSuccess) e = set_codes_attrs<F, 1>();
+  if (e == cudaSuccess) e = set_codes_attrs<F, 2>();
+  if (e == cudaSuccess) e = set_codes_attrs<F, 4>();
   return e;
 }
 
@@ -88,10 +96,8 @@ int get_here(Here* out) {
   const int rc = get_device_state(&st);
   if (rc != TCEC_OK) return rc;
   if (!st->codes_attrs_done) {
-    TCEC_CUDA((set_codes_attrs<false, false>()));
-    TCEC_CUDA((set_codes_attrs<false, true>()));
-    TCEC_CUDA((set_codes_attrs<true, false>()));
-    TCEC_CUDA((set_codes_attrs<true, true>()));
+    TCEC_CUDA(set_all_codes_attrs<false>());
+    TCEC_CUDA(set_all_codes_attrs<true>());
     st->codes_attrs_done = true;
   }
   *out = {st->status, st->sm_count};
@@ -159,20 +165,27 @@ struct GemvQ4 {
   }
 };
 
-template <int BN, bool F, bool Q8>
+template <int BN, bool F, int S>
 void launch_codes_as(const GemmCodesParams& gp, int shares, cudaStream_t stream) {
-  launch_clusters(tcec_gemm_codes_kernel<BN, F, Q8>, shares, gp.row_tiles * gp.col_tiles * shares, 512, GemmCodesCfg<BN, Q8>::SMEM_BYTES,
+  launch_clusters(tcec_gemm_codes_kernel<BN, F, S>, shares, gp.row_tiles * gp.col_tiles * shares, 512, GemmCodesCfg<BN, S>::SMEM_BYTES,
                   stream, gp);
 }
-template <bool F, bool Q8>
-void launch_codes(int bn, const GemmCodesParams& gp, int shares, cudaStream_t stream) {
-  if (bn == 64) launch_codes_as<64, F, Q8>(gp, shares, stream);
-  else if (bn == 128) launch_codes_as<128, F, Q8>(gp, shares, stream);
-  else launch_codes_as<256, F, Q8>(gp, shares, stream);
+template <bool F, int S>
+void launch_codes_of(int bn, const GemmCodesParams& gp, int shares, cudaStream_t stream) {
+  if (bn == 64) launch_codes_as<64, F, S>(gp, shares, stream);
+  else if (bn == 128) launch_codes_as<128, F, S>(gp, shares, stream);
+  else launch_codes_as<256, F, S>(gp, shares, stream);
+}
+template <bool F>
+void launch_codes(int spans, int bn, const GemmCodesParams& gp, int shares, cudaStream_t stream) {
+  if (spans == 0) launch_codes_of<F, 0>(bn, gp, shares, stream);
+  else if (spans == 1) launch_codes_of<F, 1>(bn, gp, shares, stream);
+  else if (spans == 2) launch_codes_of<F, 2>(bn, gp, shares, stream);
+  else launch_codes_of<F, 4>(bn, gp, shares, stream);
 }
 
-// D[row][col] of tcec_gemm_codes.cuh for an operand of codes and a dense one whose columns and sum lie at the given steps.
-int gemm_codes(bool q8, const void* codes, int spans, int rows, int cols, int sum, const void* dense, long long col_step, long long sum_step,
+// D[row][col] of tcec_gemm_codes.cuh for an operand of codes (spans: groups of 4-bit codes in a block, 0: 8-bit codes) and a dense one whose columns and sum lie at the given steps.
+int gemm_codes(const void* codes, int spans, int rows, int cols, int sum, const void* dense, long long col_step, long long sum_step,
                int type, bool vec, float alpha, float beta, void* c, long long c_row, long long c_col, int c_type, void* workspace,
                const Here& here, cudaStream_t stream) {
   const int parts = type == TCEC_TYPE_F32 ? 3 : 1, blocks = static_cast<int>(ceil_div(sum, kCodeSpan));
@@ -195,7 +208,6 @@ int gemm_codes(bool q8, const void* codes, int spans, int rows, int cols, int su
   gp.cols = cols;
   gp.blocks = blocks;
   gp.parts = parts;
-  gp.spans = spans;
   gp.row_tiles = static_cast<int>(ceil_div(rows, 128));
   gp.alpha = alpha;
   gp.beta = beta;
@@ -211,13 +223,8 @@ int gemm_codes(bool q8, const void* codes, int spans, int rows, int cols, int su
   int shares = 1;
   while (bn < 256 && shares < 8 && tiles * shares * 2 <= 148 && blocks >= 4 * shares) shares *= 2;
   if (tiles * shares > kMostBlocks) return TCEC_ERR_UNSUPPORTED;
-  if (type == TCEC_TYPE_F16) {
-    if (q8) launch_codes<true, true>(bn, gp, shares, stream);
-    else launch_codes<true, false>(bn, gp, shares, stream);
-  } else {
-    if (q8) launch_codes<false, true>(bn, gp, shares, stream);
-    else launch_codes<false, false>(bn, gp, shares, stream);
-  }
+  if (type == TCEC_TYPE_F16) launch_codes<true>(spans, bn, gp, shares, stream);
+  else launch_codes<false>(spans, bn, gp, shares, stream);
   return launched();
 }
 
@@ -349,7 +356,7 @@ int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, c
     if (rc != TCEC_OK) return rc;
     const bool vec = layout_x == TCEC_ROW_MAJOR && dx.wide(16);
     if (!streamed(m, type_x))
-      return gemm_codes(false, packed, kCodeSpan / group, n, m, sum, x, dx.row_step(), dx.col_step(), type_x, vec, alpha, beta, c, dc.col_step(),
+      return gemm_codes(packed, kCodeSpan / group, n, m, sum, x, dx.row_step(), dx.col_step(), type_x, vec, alpha, beta, c, dc.col_step(),
                         dc.row_step(), type_c, workspace, here, static_cast<cudaStream_t>(stream));
     GemvQ4Params p{};
     p.codes = static_cast<const uint8_t*>(packed);
@@ -450,7 +457,7 @@ int tcec_wgrad_q8(int layout_dy, int layout_c, int m, int n, int k, float alpha,
     const int rc = get_here(&here);
     if (rc != TCEC_OK) return rc;
     // columns: the outputs of the layer; the sum: tokens
-    return gemm_codes(true, packed, 1, k, n, sum, dy, dd.col_step(), dd.row_step(), type_dy, layout_dy == TCEC_COL_MAJOR && dd.wide(16), alpha,
+    return gemm_codes(packed, 0, k, n, sum, dy, dd.col_step(), dd.row_step(), type_dy, layout_dy == TCEC_COL_MAJOR && dd.wide(16), alpha,
                       beta, c, dc.col_step(), dc.row_step(), type_c, workspace, here, static_cast<cudaStream_t>(stream));
   });
 }

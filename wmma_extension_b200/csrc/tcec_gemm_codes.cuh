@@ -144,7 +144,6 @@ struct GemmCodesParams {
   const uint8_t* panels;      // [128 columns][block][part]
   int rows, cols, blocks;     // blocks along the sum
   int parts;                  // of the dense operand: 1, or 3 (FP32)
-  int spans;                  // groups in a block: 1, 2 or 4
   int row_tiles, col_tiles;
   float alpha, beta;
   void* c;
@@ -153,23 +152,29 @@ struct GemmCodesParams {
   int* status;
 };
 
-template <int BN, bool kQ8>
+// kSpans: groups of 4-bit codes in a block (1, 2 or 4); 0: 8-bit codes, one group a block.
+template <int BN, int kSpans>
 struct GemmCodesCfg {
+  static constexpr bool Q8 = kSpans == 0;
+  static constexpr int GROUPS = Q8 ? 1 : kSpans;
   static constexpr int THREADS = 512;
-  static constexpr int CODE_BYTES = kQ8 ? kQ8CodeBytes : kQ4CodeBytes;
-  static constexpr int CODE_STAGES = 2;
-  static constexpr int A_STAGES = 2;                          // expanded codes, 32 KB each
+  static constexpr int CODE_BYTES = Q8 ? kQ8CodeBytes : kQ4CodeBytes;
+  static constexpr int BLOCK_BYTES = CODE_BYTES + kEntryBytes * GROUPS;
+  // Expanded codes: a chunk of 8 along the sum is 128 rows x 16 bytes, in core matrices of 8 rows; the chunks lie 32 bytes off a
+  // multiple of 128, so that lanes with rows g, g + 1 of four chunks write to all banks at once.
+  static constexpr int CHUNK_BYTES = 128 * 16 + 32;
+  static constexpr int A_BYTES = 16 * CHUNK_BYTES;
+  static constexpr int A_STAGES = 2;
   static constexpr int B_BYTES = BN * 128;                    // 64 of the sum, one part
   static constexpr int B_STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-  static constexpr int A_OFFSET = 0;
-  static constexpr int B_OFFSET = A_STAGES * kSpanBytes;
-  static constexpr int CODE_OFFSET = B_OFFSET + B_STAGES * B_BYTES;
-  static constexpr int SMEM_BYTES = CODE_OFFSET + CODE_STAGES * CODE_BYTES + 1024;
+  static constexpr int B_OFFSET = 0;
+  static constexpr int A_OFFSET = B_STAGES * B_BYTES;
+  static constexpr int SMEM_BYTES = A_OFFSET + A_STAGES * A_BYTES + 1024;
   static_assert(SMEM_BYTES <= 232448 - 512, "dynamic + static shared memory exceed an SM");
   static_assert(B_STAGES * B_BYTES >= 128 * BN * 4, "partial results go where the dense operand was");
   static constexpr int TMEM_COLS = 2 * BN;
   static constexpr int NC = BN / 2;                           // columns of an epilogue thread
-  // 512 threads x 128 registers at launch: 2 x 128 x 56 + 2 x 128 x 200 = 65536
+  // 512 threads x 128 registers at launch: 128 x (40 + 72) + 2 x 128 x 200 = 65536
   static constexpr bool REBALANCE = BN == 256;
 };
 
@@ -180,15 +185,92 @@ __device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float
       : "+f"(x), "+f"(y)
       : "f"(a), "f"(b), "f"(s));
 }
+// Loads that are issued where they stand, ahead of the waits that follow.
+__device__ __forceinline__ uint32_t ld_ahead32(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ld_ahead64(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_ahead128(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// What a converter thread holds of one block: the codes of 16 chunks, one block ahead of the one it expands.
+template <bool kF16, int kSpans>
+struct Converter {  // 4 bits: two strips of 16 rows, lane 4 g + t has rows g and g + 8 of both
+  uint4 w[2][2];
+  uint32_t entry[kSpans][2][2];
+  int code_at, entry_at, out_at;
+  __device__ __forceinline__ Converter(int warp, int lane) {
+    code_at = warp * 2048 + lane * 16;
+    entry_at = kQ4CodeBytes + (warp * 32 + (lane >> 2)) * 4;
+    out_at = (lane & 3) * GemmCodesCfg<128, kSpans>::CHUNK_BYTES + warp * 512 + (lane >> 2) * 16;
+  }
+  __device__ __forceinline__ void load_strip(const uint8_t* block, int s) {
+    w[s][0] = ld_ahead128(block + code_at + s * 1024);
+    w[s][1] = ld_ahead128(block + code_at + s * 1024 + 512);
+#pragma unroll
+    for (int q = 0; q < kSpans; ++q) {
+      entry[q][s][0] = ld_ahead32(block + entry_at + q * kEntryBytes + s * 64);
+      entry[q][s][1] = ld_ahead32(block + entry_at + q * kEntryBytes + s * 64 + 32);
+    }
+  }
+  __device__ __forceinline__ void load(const uint8_t* block) {
+    load_strip(block, 0);
+    load_strip(block, 1);
+  }
+  // Expands what it holds to `out` and loads from `next` in its place.
+  __device__ __forceinline__ void expand(uint8_t* out, const uint8_t* next) {
+    constexpr int kChunk = GemmCodesCfg<128, kSpans>::CHUNK_BYTES;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int panel = 0; panel < 4; ++panel) {
+        const uint4 pair = w[s][panel >> 1];
+        uint8_t* to = out + out_at + panel * 4 * kChunk + s * 256;
+        const int q = panel * kSpans / 4;
+        *reinterpret_cast<uint4*>(to) = q4_expand<kF16>(panel & 1 ? pair.z : pair.x, q4_zero<kF16>(entry[q][s][0] & 15u));
+        *reinterpret_cast<uint4*>(to + 128) = q4_expand<kF16>(panel & 1 ? pair.w : pair.y, q4_zero<kF16>(entry[q][s][1] & 15u));
+      }
+      if (next) load_strip(next, s);
+    }
+  }
+};
+template <bool kF16>
+struct Converter<kF16, 0> {  // 8 bits: one row
+  uint2 w[16];
+  int code_at, out_at;
+  __device__ __forceinline__ Converter(int warp, int lane) {
+    code_at = (warp * 32 + lane) * 8;
+    out_at = (warp * 32 + lane) * 16;
+  }
+  __device__ __forceinline__ void load(const uint8_t* block) {
+#pragma unroll
+    for (int c = 0; c < 16; ++c) w[c] = ld_ahead64(block + code_at + c * 1024);
+  }
+  __device__ __forceinline__ void expand(uint8_t* out, const uint8_t* next) {
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      *reinterpret_cast<uint4*>(out + out_at + c * GemmCodesCfg<128, 0>::CHUNK_BYTES) = q8_expand<kF16>(w[c]);
+      if (next) w[c] = ld_ahead64(next + code_at + c * 1024);
+    }
+  }
+};
 
 // Launched with clusters of 1, 2, 4 or 8 CTAs (256 columns: 1): one tile of 128 rows x BN columns a cluster, whose CTAs divide the sum and add up through
 // shared memory, in the order of the sum.
-template <int BN, bool kF16, bool kQ8>
+template <int BN, bool kF16, int kSpans>
 __global__ void __launch_bounds__(512, 1) tcec_gemm_codes_kernel(const GemmCodesParams p) {
-  using Cfg = GemmCodesCfg<BN, kQ8>;
-  constexpr int kBlockCodes = kQ8 ? kQ8CodeBytes : kQ4CodeBytes;
+  using Cfg = GemmCodesCfg<BN, kSpans>;
+  constexpr int kGroups = Cfg::GROUPS;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bar_code_full[Cfg::CODE_STAGES], bar_code_empty[Cfg::CODE_STAGES];
   __shared__ uint64_t bar_a_full[Cfg::A_STAGES], bar_a_empty[Cfg::A_STAGES];
   __shared__ uint64_t bar_b_full[Cfg::B_STAGES], bar_b_empty[Cfg::B_STAGES];
   __shared__ uint64_t bar_acc_full[2], bar_acc_free[2], bar_drain[1];
@@ -203,17 +285,10 @@ __global__ void __launch_bounds__(512, 1) tcec_gemm_codes_kernel(const GemmCodes
   const int rt = tile % p.row_tiles, ct = tile / p.row_tiles;
   const int kb_first = static_cast<int>(static_cast<long long>(p.blocks) * share / shares);
   const int kb_end = static_cast<int>(static_cast<long long>(p.blocks) * (share + 1) / shares);
-  const int block_bytes = kBlockCodes + kEntryBytes * p.spans;
-  const uint8_t* codes = p.codes + static_cast<size_t>(rt) * p.blocks * block_bytes;
+  const uint8_t* codes = p.codes + static_cast<size_t>(rt) * p.blocks * Cfg::BLOCK_BYTES;
   const int cols = min(BN, p.cols - ct * BN), cols16 = (cols + 15) & ~15;
-  // accumulators handed over for each block: one where its codes share a scale, else one for each group and part
-  const int folds = p.spans == 1 ? 1 : p.spans * p.parts;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < Cfg::CODE_STAGES; ++s) {
-      mbar_init(smem_u32(&bar_code_full[s]), 1);
-      mbar_init(smem_u32(&bar_code_empty[s]), 4);
-    }
     for (int s = 0; s < Cfg::A_STAGES; ++s) {
       mbar_init(smem_u32(&bar_a_full[s]), 4);
       mbar_init(smem_u32(&bar_a_empty[s]), 1);
@@ -245,65 +320,48 @@ __global__ void __launch_bounds__(512, 1) tcec_gemm_codes_kernel(const GemmCodes
   float acc[Cfg::NC];
 
   if (warp < 4) {
-    if constexpr (Cfg::REBALANCE) setmaxnreg_dec<56>();
+    if constexpr (Cfg::REBALANCE) setmaxnreg_dec<40>();
     if (warp == 0) {
-      // ---------------------------------------------------------- copies
+      // ---------------------------------------------------------- copies of the dense operand
       if (elect_one()) {
-        uint32_t cs = 0, cph = 0, bs = 0, bph = 0;
-        uint32_t c_armed = 0, c_parity = 0, b_armed = 0, b_parity = 0;
+        uint32_t bs = 0, bph = 0, armed = 0, armed_parity = 0;
         bool ok = true;
-        const int halves = BN > 128 ? BN / 128 : 1;
-        for (int kb = kb_first; kb < kb_end && ok; ++kb) {
-          if (!mbar_wait(smem_u32(&bar_code_empty[cs]), cph ^ 1, abortp)) {
+        const uint8_t* src0 = p.panels + (static_cast<size_t>(ct * BN >> 7) * p.blocks + kb_first) * p.parts * kSpanBytes + (ct * BN & 127) * 64;
+        const uint8_t* src1 = src0 + static_cast<size_t>(p.blocks) * p.parts * kSpanBytes;  // the second 128 columns of 256
+        const uint32_t rows0 = min(128, cols16) * 64, rows1 = cols16 > 128 ? (cols16 - 128) * 64 : 0;
+        for (int left = (kb_end - kb_first) * p.parts * 2; left > 0; --left) {  // a half of a block and part
+          if (!mbar_wait(smem_u32(&bar_b_empty[bs]), bph ^ 1, abortp)) {
             ok = false;
             break;
           }
-          const uint32_t cfull = smem_u32(&bar_code_full[cs]);
-          mbar_arrive_expect_tx(cfull, kBlockCodes);
-          c_armed |= 1u << cs;
-          c_parity = (c_parity & ~(1u << cs)) | (cph << cs);
-          bulk_load(smem_base + Cfg::CODE_OFFSET + cs * Cfg::CODE_BYTES, codes + static_cast<size_t>(kb) * block_bytes, kBlockCodes, cfull);
-          if (++cs == Cfg::CODE_STAGES) cs = 0, cph ^= 1;
-          for (int h2 = 0; h2 < 2 * p.parts && ok; ++h2) {  // part, half of the block
-            if (!mbar_wait(smem_u32(&bar_b_empty[bs]), bph ^ 1, abortp)) {
-              ok = false;
-              break;
-            }
-            const uint32_t bfull = smem_u32(&bar_b_full[bs]);
-            mbar_arrive_expect_tx(bfull, 2 * cols16 * 64);
-            b_armed |= 1u << bs;
-            b_parity = (b_parity & ~(1u << bs)) | (bph << bs);
-            const uint32_t dst = smem_base + Cfg::B_OFFSET + bs * Cfg::B_BYTES;
-            for (int cb = 0; cb < halves; ++cb) {
-              const int here = min(128, cols16 - cb * 128);
-              if (here <= 0) break;
-              const int col = ct * BN + cb * 128;
-              const uint8_t* src = p.panels + (static_cast<size_t>(col >> 7) * p.blocks + kb) * p.parts * kSpanBytes +
-                                   static_cast<size_t>(h2) * 2 * kPanelBytes + (col & 127) * 64;
-              for (int q = 0; q < 2; ++q)
-                bulk_load(dst + q * (BN * 64) + cb * kPanelBytes, src + q * kPanelBytes, here * 64, bfull);
-            }
-            if (++bs == Cfg::B_STAGES) bs = 0, bph ^= 1;
+          const uint32_t bfull = smem_u32(&bar_b_full[bs]);
+          mbar_arrive_expect_tx(bfull, 2 * (rows0 + rows1));
+          armed |= 1u << bs;
+          armed_parity = (armed_parity & ~(1u << bs)) | (bph << bs);
+          const uint32_t dst = smem_base + Cfg::B_OFFSET + bs * Cfg::B_BYTES;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            bulk_load(dst + q * (BN * 64), src0 + q * kPanelBytes, rows0, bfull);
+            if (BN > 128 && rows1) bulk_load(dst + q * (BN * 64) + kPanelBytes, src1 + q * kPanelBytes, rows1, bfull);
           }
+          src0 += 2 * kPanelBytes;
+          src1 += 2 * kPanelBytes;
+          if (++bs == Cfg::B_STAGES) bs = 0, bph ^= 1;
         }
         if (!ok) {
           abort_flag = 1;
           atomicCAS(p.status, 0, kErrProducerWait);
           // this thread's own copies land before the CTA gives up its shared memory
-          for (uint32_t q = 0; q < Cfg::CODE_STAGES; ++q)
-            if (c_armed & (1u << q)) mbar_wait_plain(smem_u32(&bar_code_full[q]), (c_parity >> q) & 1);
           for (uint32_t q = 0; q < Cfg::B_STAGES; ++q)
-            if (b_armed & (1u << q)) mbar_wait_plain(smem_u32(&bar_b_full[q]), (b_parity >> q) & 1);
+            if (armed & (1u << q)) mbar_wait_plain(smem_u32(&bar_b_full[q]), (armed_parity >> q) & 1);
         }
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------- MMAs
       if (elect_one()) {
-        const uint64_t dconst = umma_desc_kmajor_noswizzle(0, 128, 512);
-        const uint32_t fmt = kF16 ? 0u : 1u;
-        const uint32_t idesc = umma_idesc(fmt, 128, cols16);
+        const uint64_t a_const = umma_desc_kmajor_noswizzle(0, Cfg::CHUNK_BYTES, 128), b_const = umma_desc_kmajor_noswizzle(0, 128, 512);
+        const uint32_t idesc = umma_idesc(kF16 ? 0u : 1u, 128, cols16);
         const uint32_t a16 = ((smem_base + Cfg::A_OFFSET) & 0x3ffff) >> 4, b16 = ((smem_base + Cfg::B_OFFSET) & 0x3ffff) >> 4;
-        const int steps_of_group = 8 / p.spans;  // MMAs of 16
         uint32_t as = 0, aph = 0, bs = 0, bph = 0, fold = 0;
         bool ok = true;
         for (int kb = kb_first; kb < kb_end && ok; ++kb) {
@@ -311,34 +369,40 @@ __global__ void __launch_bounds__(512, 1) tcec_gemm_codes_kernel(const GemmCodes
             ok = false;
             break;
           }
-          for (int h2 = 0; h2 < 2 * p.parts && ok; ++h2) {
-            if (!mbar_wait(smem_u32(&bar_b_full[bs]), bph, abortp, 0)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            for (int j = 0; j < 4; ++j) {
-              const int step = (h2 & 1) * 4 + j;
-              const bool first = p.spans == 1 ? h2 == 0 && j == 0 : step % steps_of_group == 0;
-              const bool last = p.spans == 1 ? h2 == 2 * p.parts - 1 && j == 3 : step % steps_of_group == steps_of_group - 1;
-              if (first) {
-                if (!mbar_wait(smem_u32(&bar_acc_free[fold & 1]), ((fold >> 1) & 1) ^ 1, abortp, 0)) {
-                  ok = false;
-                  break;
+          const uint32_t a_here = a16 + as * (Cfg::A_BYTES >> 4);
+          for (int part = 0; part < p.parts && ok; ++part) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (!mbar_wait(smem_u32(&bar_b_full[bs]), bph, abortp, 0)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const uint32_t b_here = b16 + bs * (Cfg::B_BYTES >> 4);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int step = h * 4 + j;  // of 16 along the sum
+                // an accumulator holds one group; where a block is one, all parts of it
+                const bool first = step % (8 / kGroups) == 0 && (kGroups > 1 || part == 0);
+                const bool last = step % (8 / kGroups) == 8 / kGroups - 1 && (kGroups > 1 || part == p.parts - 1);
+                if (first) {
+                  if (!mbar_wait(smem_u32(&bar_acc_free[fold & 1]), ((fold >> 1) & 1) ^ 1, abortp, 0)) {
+                    ok = false;
+                    break;
+                  }
+                  tc_fence_after();
                 }
-                tc_fence_after();
+                umma_ss<false>(tmem + (fold & 1) * BN, a_const | (a_here + step * (2 * Cfg::CHUNK_BYTES >> 4)),
+                               b_const | (b_here + (j >> 1) * (BN * 64 >> 4) + (j & 1) * 16), idesc, first ? 0u : 1u);
+                if (last) {
+                  umma_commit(smem_u32(&bar_acc_full[fold & 1]));
+                  ++fold;
+                }
               }
-              const uint64_t a_desc = dconst | (a16 + as * (kSpanBytes >> 4) + (step >> 1) * (kPanelBytes >> 4) + (step & 1) * 16);
-              const uint64_t b_desc = dconst | (b16 + bs * (Cfg::B_BYTES >> 4) + (j >> 1) * (BN * 64 >> 4) + (j & 1) * 16);
-              umma_ss<false>(tmem + (fold & 1) * BN, a_desc, b_desc, idesc, first ? 0u : 1u);
-              if (last) {
-                umma_commit(smem_u32(&bar_acc_full[fold & 1]));
-                ++fold;
-              }
+              if (!ok) break;
+              umma_commit(smem_u32(&bar_b_empty[bs]));
+              if (++bs == Cfg::B_STAGES) bs = 0, bph ^= 1;
             }
-            if (!ok) break;
-            umma_commit(smem_u32(&bar_b_empty[bs]));
-            if (++bs == Cfg::B_STAGES) bs = 0, bph ^= 1;
           }
           if (!ok) break;
           umma_commit(smem_u32(&bar_a_empty[as]));
@@ -349,42 +413,20 @@ __global__ void __launch_bounds__(512, 1) tcec_gemm_codes_kernel(const GemmCodes
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------ codes to operands
-    if constexpr (Cfg::REBALANCE) setmaxnreg_dec<56>();
-    const int t = threadIdx.x - 128;
-    uint32_t cs = 0, cph = 0, as = 0, aph = 0;
+    if constexpr (Cfg::REBALANCE) setmaxnreg_dec<72>();
+    Converter<kF16, kSpans> held(warp - 4, lane);
+    uint32_t as = 0, aph = 0;
     bool ok = true;
+    if (kb_first < kb_end) held.load(codes + static_cast<size_t>(kb_first) * Cfg::BLOCK_BYTES);
     for (int kb = kb_first; kb < kb_end; ++kb) {
-      [[maybe_unused]] uint32_t zeros[4];
-      if constexpr (!kQ8) {  // of this thread's row, for each 32 of the sum
-        const uint8_t* entries = codes + static_cast<size_t>(kb) * block_bytes + kBlockCodes;
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          zeros[q] = q4_zero<kF16>(ld_operand32(entries + (q * p.spans >> 2) * kEntryBytes + t * 4) & 15u);
-      }
-      if (!mbar_wait_warp(smem_u32(&bar_code_full[cs]), cph, abortp, 64) || !mbar_wait_warp(smem_u32(&bar_a_empty[as]), aph ^ 1, abortp, 64)) {
+      if (!mbar_wait_warp(smem_u32(&bar_a_empty[as]), aph ^ 1, abortp, 64)) {
         ok = false;
         break;
       }
-      const uint8_t* in = smem_gen + Cfg::CODE_OFFSET + cs * Cfg::CODE_BYTES;
-      uint8_t* out = smem_gen + Cfg::A_OFFSET + as * kSpanBytes + (t >> 3) * 512 + (t & 7) * 16;
-      if constexpr (kQ8) {
-#pragma unroll 4
-        for (int c = 0; c < 16; ++c)
-          *reinterpret_cast<uint4*>(out + (c >> 2) * kPanelBytes + (c & 3) * 128) =
-              q8_expand<kF16>(*reinterpret_cast<const uint2*>(in + c * 1024 + t * 8));
-      } else {
-#pragma unroll
-        for (int c = 0; c < 16; ++c)
-          *reinterpret_cast<uint4*>(out + (c >> 2) * kPanelBytes + (c & 3) * 128) =
-              q4_expand<kF16>(reinterpret_cast<const uint32_t*>(in)[q4_word(t, c)], zeros[c >> 2]);
-      }
+      held.expand(smem_gen + Cfg::A_OFFSET + as * Cfg::A_BYTES, kb + 1 < kb_end ? codes + static_cast<size_t>(kb + 1) * Cfg::BLOCK_BYTES : nullptr);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(smem_u32(&bar_a_full[as]));
-        mbar_arrive(smem_u32(&bar_code_empty[cs]));
-      }
-      if (++cs == Cfg::CODE_STAGES) cs = 0, cph ^= 1;
+      if (lane == 0) mbar_arrive(smem_u32(&bar_a_full[as]));
       if (++as == Cfg::A_STAGES) as = 0, aph ^= 1;
     }
     if (!ok) {
@@ -399,36 +441,45 @@ __global__ void __launch_bounds__(512, 1) tcec_gemm_codes_kernel(const GemmCodes
     const int q = warp & 3, r = q * 32 + lane, first_col = (warp >= 12 ? Cfg::NC : 0);
     const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + first_col;
     const bool any = first_col < cols;
+    const int rounds = kGroups > 1 ? p.parts : 1;  // of the groups of a block
     uint32_t fold = 0;
     bool ok = true;
-    auto scale_of = [&](int kb, int f) {
-      const uint8_t* at = codes + static_cast<size_t>(kb) * block_bytes + kBlockCodes + (p.spans == 1 ? 0 : f % p.spans) * kEntryBytes + r * 4;
-      return __uint_as_float(kQ8 ? ld_operand32(at) : ld_operand32(at) & ~15u);
+    float scale[kGroups], next[kGroups];
+    auto load_scales = [&](int kb) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+        next[g] = __uint_as_float(ld_ahead32(codes + static_cast<size_t>(kb) * Cfg::BLOCK_BYTES + Cfg::CODE_BYTES + g * kEntryBytes + r * 4) &
+                                  (Cfg::Q8 ? ~0u : ~15u));
     };
-    float next = kb_first < kb_end ? scale_of(kb_first, 0) : 0.f;
+    if (kb_first < kb_end) load_scales(kb_first);
     for (int kb = kb_first; kb < kb_end && ok; ++kb) {
-      for (int f = 0; f < folds; ++f, ++fold) {
-        const float s = next;
-        if (f + 1 < folds) next = scale_of(kb, f + 1);
-        else if (kb + 1 < kb_end) next = scale_of(kb + 1, 0);
-        if (!mbar_wait_warp(smem_u32(&bar_acc_full[fold & 1]), (fold >> 1) & 1, abortp, 64)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        if (any) {
 #pragma unroll
-          for (int i = 0; i < Cfg::NC; i += 32) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(taddr + (fold & 1) * BN + i, v);
-            tmem_ld_wait();
+      for (int g = 0; g < kGroups; ++g) scale[g] = next[g];
+      if (kb + 1 < kb_end) load_scales(kb + 1);
+      for (int round = 0; round < rounds && ok; ++round) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) fma2(acc[i + j], acc[i + j + 1], __uint_as_float(v[j]), __uint_as_float(v[j + 1]), s);
+        for (int g = 0; g < kGroups; ++g, ++fold) {
+          if (!mbar_wait_warp(smem_u32(&bar_acc_full[fold & 1]), (fold >> 1) & 1, abortp, 64)) {
+            ok = false;
+            break;
           }
+          tc_fence_after();
+          if (any) {
+            uint32_t v[2][16];
+            tmem_ld_32x32b_x16(taddr + (fold & 1) * BN, v[0]);
+#pragma unroll
+            for (int i = 0; i < Cfg::NC; i += 16) {
+              tmem_ld_wait();
+              if (i + 16 < Cfg::NC) tmem_ld_32x32b_x16(taddr + (fold & 1) * BN + i + 16, v[(i / 16 + 1) & 1]);
+#pragma unroll
+              for (int j = 0; j < 16; j += 2)
+                fma2(acc[i + j], acc[i + j + 1], __uint_as_float(v[(i / 16) & 1][j]), __uint_as_float(v[(i / 16) & 1][j + 1]), scale[g]);
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bar_acc_free[fold & 1]));
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_acc_free[fold & 1]));
       }
     }
     if (!ok) {
@@ -455,39 +506,39 @@ __global__ void __launch_bounds__(512, 1) tcec_gemm_codes_kernel(const GemmCodes
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, Cfg::TMEM_COLS);
   if constexpr (!Cfg::REBALANCE) {
-   if (shares > 1) {
-    cluster_sync_all();  // nobody reads operands any more where the partial results go
-    const int per = BN / shares;  // columns that a CTA adds up and stores
-    if (warp >= 8) {
-      const int r = (warp & 3) * 32 + lane, first_col = (warp >= 12 ? Cfg::NC : 0);
+    if (shares > 1) {
+      cluster_sync_all();  // nobody reads operands any more where the partial results go
+      const int per = BN / shares;  // columns that a CTA adds up and stores
+      if (warp >= 8) {
+        const int r = (warp & 3) * 32 + lane, first_col = (warp >= 12 ? Cfg::NC : 0);
 #pragma unroll
-      for (int i = 0; i < Cfg::NC; ++i) {
-        const int col = first_col + i, to = col / per;
-        const uint32_t at = smem_base + Cfg::B_OFFSET + ((share * per + col - to * per) * 128 + r) * 4;
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(at, to)), "f"(acc[i]) : "memory");
+        for (int i = 0; i < Cfg::NC; ++i) {
+          const int col = first_col + i, to = col / per;
+          const uint32_t at = smem_base + Cfg::B_OFFSET + ((share * per + col - to * per) * 128 + r) * 4;
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(at, to)), "f"(acc[i]) : "memory");
+        }
       }
-    }
-    // A CTA whose wait ran out has no share: it tells the others, and none of them stores its part of the tile.
-    if (static_cast<int>(threadIdx.x) < shares && *abortp) raise_abort_in(&abort_flag, threadIdx.x);
-    __syncwarp();
-    cluster_sync_all();
-    if (warp >= 8 && !*abortp) {
-      const int t = threadIdx.x - 256, r = t & 127, row = rt * 128 + r;
-      if (row < p.rows) {
-        const float* parts = reinterpret_cast<const float*>(smem_gen + Cfg::B_OFFSET) + r;
-        for (int i = t >> 7; i < per; i += 2) {
-          const int col = share * per + i;
-          if (col >= cols) break;
-          float v = parts[i * 128];
-          for (int s = 1; s < shares; ++s) v += parts[(s * per + i) * 128];
-          const long long at = row * p.c_row + static_cast<long long>(ct * BN + col) * p.c_col;
-          v = __fmul_rn(p.alpha, v);
-          if (p.beta != 0.f) v = __fmaf_rn(p.beta, ld_element_as(p.c_type, p.c, at), v);
-          st_element_as(p.c_type, p.c, at, v);
+      // A CTA whose wait ran out has no share: it tells the others, and none of them stores its part of the tile.
+      if (static_cast<int>(threadIdx.x) < shares && *abortp) raise_abort_in(&abort_flag, threadIdx.x);
+      __syncwarp();
+      cluster_sync_all();
+      if (warp >= 8 && !*abortp) {
+        const int t = threadIdx.x - 256, r = t & 127, row = rt * 128 + r;
+        if (row < p.rows) {
+          const float* parts = reinterpret_cast<const float*>(smem_gen + Cfg::B_OFFSET) + r;
+          for (int i = t >> 7; i < per; i += 2) {
+            const int col = share * per + i;
+            if (col >= cols) break;
+            float v = parts[i * 128];
+            for (int s = 1; s < shares; ++s) v += parts[(s * per + i) * 128];
+            const long long at = row * p.c_row + static_cast<long long>(ct * BN + col) * p.c_col;
+            v = __fmul_rn(p.alpha, v);
+            if (p.beta != 0.f) v = __fmaf_rn(p.beta, ld_element_as(p.c_type, p.c, at), v);
+            st_element_as(p.c_type, p.c, at, v);
+          }
         }
       }
     }
-   }
   }
 }
 
