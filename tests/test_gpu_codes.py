@@ -170,6 +170,15 @@ def test_products_of_odd_sizes(m, n, k, dtype):
     check(tcec.gemm_q4(x, packed, n, group=64), exact, tol)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_products_large_enough_for_pairs(group, dtype):
+    """17 x 6 tiles of 128 x 256: the last pair of SMs has one row of tiles, the last column of tiles fewer than 128 columns."""
+    x, packed, exact, tol = product_case(1350, 2170, 700, group, dtype, 41)
+    check(tcec.gemm_q4(x, packed, 2170, group=group), exact, tol)
+    tcec.device_status()
+
+
 @pytest.mark.parametrize("m", [3, 150])
 @pytest.mark.parametrize("dtype,out", [(BF16, F32), (F16, F32), (F32, F32), (BF16, BF16)])
 @pytest.mark.parametrize("lx", ["rows", "odd", "columns"])
@@ -300,7 +309,7 @@ def gradient_case(m, n, k, dtype, seed, out=None):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 200, 130), (127, 16, 128), (128, 64, 128), (129, 65, 257), (700, 130, 300), (1030, 8, 1000),
-                                   (5000, 20, 140), (300, 1000, 2000)])
+                                   (5000, 20, 140), (300, 1000, 2000), (500, 1350, 2170)])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_gradients(m, n, k, dtype):
     dy, packed, exact, tol = gradient_case(m, n, k, dtype, m + n)

@@ -166,22 +166,21 @@ struct GemvQ4 {
 };
 
 template <int BN, bool F, int S>
-void launch_codes_as(const GemmCodesParams& gp, int shares, cudaStream_t stream) {
-  launch_clusters(tcec_gemm_codes_kernel<BN, F, S>, shares, gp.row_tiles * gp.col_tiles * shares, 512, GemmCodesCfg<BN, S>::SMEM_BYTES,
-                  stream, gp);
+void launch_codes_as(const GemmCodesParams& gp, int shares, int grid, cudaStream_t stream) {
+  launch_clusters(tcec_gemm_codes_kernel<BN, F, S>, shares, grid, 512, GemmCodesCfg<BN, S>::SMEM_BYTES, stream, gp);
 }
 template <bool F, int S>
-void launch_codes_of(int bn, const GemmCodesParams& gp, int shares, cudaStream_t stream) {
-  if (bn == 64) launch_codes_as<64, F, S>(gp, shares, stream);
-  else if (bn == 128) launch_codes_as<128, F, S>(gp, shares, stream);
-  else launch_codes_as<256, F, S>(gp, shares, stream);
+void launch_codes_of(int bn, const GemmCodesParams& gp, int shares, int grid, cudaStream_t stream) {
+  if (bn == 64) launch_codes_as<64, F, S>(gp, shares, grid, stream);
+  else if (bn == 128) launch_codes_as<128, F, S>(gp, shares, grid, stream);
+  else launch_codes_as<256, F, S>(gp, shares, grid, stream);
 }
 template <bool F>
-void launch_codes(int spans, int bn, const GemmCodesParams& gp, int shares, cudaStream_t stream) {
-  if (spans == 0) launch_codes_of<F, 0>(bn, gp, shares, stream);
-  else if (spans == 1) launch_codes_of<F, 1>(bn, gp, shares, stream);
-  else if (spans == 2) launch_codes_of<F, 2>(bn, gp, shares, stream);
-  else launch_codes_of<F, 4>(bn, gp, shares, stream);
+void launch_codes(int spans, int bn, const GemmCodesParams& gp, int shares, int grid, cudaStream_t stream) {
+  if (spans == 0) launch_codes_of<F, 0>(bn, gp, shares, grid, stream);
+  else if (spans == 1) launch_codes_of<F, 1>(bn, gp, shares, grid, stream);
+  else if (spans == 2) launch_codes_of<F, 2>(bn, gp, shares, grid, stream);
+  else launch_codes_of<F, 4>(bn, gp, shares, grid, stream);
 }
 
 // D[row][col] of tcec_gemm_codes.cuh for an operand of codes (spans: groups of 4-bit codes in a block, 0: 8-bit codes) and a dense one whose columns and sum lie at the given steps.
@@ -217,14 +216,17 @@ int gemm_codes(const void* codes, int spans, int rows, int cols, int sum, const 
   gp.c_type = c_type;
   gp.status = here.status;
   int bn = cols <= 64 ? 64 : 128;
-  if (cols > 128 && gp.row_tiles * ceil_div(cols, 256) >= 100) bn = 256;
+  if (cols > 128 && ceil_div(gp.row_tiles, 2) * ceil_div(cols, 256) >= 50) bn = 256;
   gp.col_tiles = static_cast<int>(ceil_div(cols, bn));
-  const long long tiles = static_cast<long long>(gp.row_tiles) * gp.col_tiles;
-  int shares = 1;
-  while (bn < 256 && shares < 8 && tiles * shares * 2 <= 148 && blocks >= 4 * shares) shares *= 2;
-  if (tiles * shares > kMostBlocks) return TCEC_ERR_UNSUPPORTED;
-  if (type == TCEC_TYPE_F16) launch_codes<true>(spans, bn, gp, shares, stream);
-  else launch_codes<false>(spans, bn, gp, shares, stream);
+  const long long tiles = (bn == 256 ? ceil_div(gp.row_tiles, 2) : gp.row_tiles) * static_cast<long long>(gp.col_tiles);
+  if (tiles > kMostBlocks) return TCEC_ERR_UNSUPPORTED;
+  int ctas = bn == 256 ? 2 : 1;  // of a cluster
+  while (bn < 256 && ctas < 8 && tiles * ctas * 2 <= 148 && blocks >= 4 * ctas) ctas *= 2;
+  // One cluster a tile where the sum is divided; else as many as run at a time.
+  const long long most = bn == 256 ? here.sm_count / 2 : ctas > 1 ? tiles : here.sm_count;
+  const int grid = static_cast<int>(tiles < most ? tiles : most) * ctas;
+  if (type == TCEC_TYPE_F16) launch_codes<true>(spans, bn, gp, ctas, grid, stream);
+  else launch_codes<false>(spans, bn, gp, ctas, grid, stream);
   return launched();
 }
 

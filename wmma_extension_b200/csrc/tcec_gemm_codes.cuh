@@ -86,7 +86,8 @@ __global__ void __launch_bounds__(256) stage_panels_kernel(const StagePanelsPara
 #pragma unroll
       for (int j = 0; j < 4; ++j) split3_bf16(v[2 * j], v[2 * j + 1], part[0][j], part[1][j], part[2][j]);
 #pragma unroll
-      for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(to + q * kSpanBytes) = make_uint4(part[q][0], part[q][1], part[q][2], part[q][3]);
+      for (int q = 0; q < 3; ++q)  // the small parts first, so that the accumulator, which truncates, cuts off less
+        *reinterpret_cast<uint4*>(to + q * kSpanBytes) = make_uint4(part[2 - q][0], part[2 - q][1], part[2 - q][2], part[2 - q][3]);
     } else {
       uint4 o = make_uint4(0, 0, 0, 0);
       const uint16_t* src = static_cast<const uint16_t*>(p.src);
@@ -156,6 +157,7 @@ struct GemmCodesParams {
 template <int BN, int kSpans>
 struct GemmCodesCfg {
   static constexpr bool Q8 = kSpans == 0;
+  static constexpr bool PAIR = BN == 256;                     // 256 x 256 tiles on two SMs
   static constexpr int GROUPS = Q8 ? 1 : kSpans;
   static constexpr int THREADS = 512;
   static constexpr int CODE_BYTES = Q8 ? kQ8CodeBytes : kQ4CodeBytes;
@@ -164,18 +166,23 @@ struct GemmCodesCfg {
   // multiple of 128, so that lanes with rows g, g + 1 of four chunks write to all banks at once.
   static constexpr int CHUNK_BYTES = 128 * 16 + 32;
   static constexpr int A_BYTES = 16 * CHUNK_BYTES;
-  static constexpr int A_STAGES = 2;
-  static constexpr int B_BYTES = BN * 128;                    // 64 of the sum, one part
-  static constexpr int B_STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+  static constexpr int A_STAGES = 3;
+  static constexpr int BC = PAIR ? 128 : BN;                  // columns of the dense operand that a CTA brings in
+  static constexpr int B_BYTES = BC * 128;                    // 64 of the sum, one part
+  static constexpr int B_STAGES = BN == 64 ? 6 : 4;
+  static constexpr int CODE_STAGES = 3;
+  static constexpr int SCALE_SLOTS = 6;                       // blocks; see the converters
   static constexpr int B_OFFSET = 0;
   static constexpr int A_OFFSET = B_STAGES * B_BYTES;
-  static constexpr int SMEM_BYTES = A_OFFSET + A_STAGES * A_BYTES + 1024;
+  static constexpr int CODE_OFFSET = A_OFFSET + A_STAGES * A_BYTES;
+  static constexpr int SCALE_OFFSET = CODE_OFFSET + CODE_STAGES * BLOCK_BYTES;
+  static constexpr int SMEM_BYTES = SCALE_OFFSET + SCALE_SLOTS * GROUPS * 512 + 1024;
   static_assert(SMEM_BYTES <= 232448 - 512, "dynamic + static shared memory exceed an SM");
-  static_assert(B_STAGES * B_BYTES >= 128 * BN * 4, "partial results go where the dense operand was");
+  static_assert(PAIR || B_STAGES * B_BYTES >= 128 * BN * 4, "partial results go where the dense operand was");
   static constexpr int TMEM_COLS = 2 * BN;
   static constexpr int NC = BN / 2;                           // columns of an epilogue thread
-  // 512 threads x 128 registers at launch: 128 x (40 + 72) + 2 x 128 x 200 = 65536
-  static constexpr bool REBALANCE = BN == 256;
+  // 512 threads x 128 registers at launch: 128 x (40 + 56) + 2 x 128 x 208 = 65536
+  static constexpr bool REBALANCE = PAIR;
 };
 
 __device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float s) {
@@ -185,92 +192,75 @@ __device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float
       : "+f"(x), "+f"(y)
       : "f"(a), "f"(b), "f"(s));
 }
-// Loads that are issued where they stand, ahead of the waits that follow.
-__device__ __forceinline__ uint32_t ld_ahead32(const void* p) {
-  uint32_t v;
-  asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ld_ahead64(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint4 ld_ahead128(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+// All lanes poll, which they notice sooner than one lane that tells the others.
+__device__ __forceinline__ bool mbar_wait_lanes(uint32_t bar, uint32_t parity, volatile uint32_t* abortp) {
+  const bool ok = mbar_wait(bar, parity, abortp, 0);
+  return __all_sync(0xffffffffu, ok);
 }
 
-// What a converter thread holds of one block: the codes of 16 chunks, one block ahead of the one it expands.
+// Expands the codes of one block (shared memory) to 16-bit operands and hands its scales on.
 template <bool kF16, int kSpans>
-struct Converter {  // 4 bits: two strips of 16 rows, lane 4 g + t has rows g and g + 8 of both
-  uint4 w[2][2];
-  uint32_t entry[kSpans][2][2];
-  int code_at, entry_at, out_at;
-  __device__ __forceinline__ Converter(int warp, int lane) {
-    code_at = warp * 2048 + lane * 16;
-    entry_at = kQ4CodeBytes + (warp * 32 + (lane >> 2)) * 4;
-    out_at = (lane & 3) * GemmCodesCfg<128, kSpans>::CHUNK_BYTES + warp * 512 + (lane >> 2) * 16;
-  }
-  __device__ __forceinline__ void load_strip(const uint8_t* block, int s) {
-    w[s][0] = ld_ahead128(block + code_at + s * 1024);
-    w[s][1] = ld_ahead128(block + code_at + s * 1024 + 512);
-#pragma unroll
-    for (int q = 0; q < kSpans; ++q) {
-      entry[q][s][0] = ld_ahead32(block + entry_at + q * kEntryBytes + s * 64);
-      entry[q][s][1] = ld_ahead32(block + entry_at + q * kEntryBytes + s * 64 + 32);
-    }
-  }
-  __device__ __forceinline__ void load(const uint8_t* block) {
-    load_strip(block, 0);
-    load_strip(block, 1);
-  }
-  // Expands what it holds to `out` and loads from `next` in its place.
-  __device__ __forceinline__ void expand(uint8_t* out, const uint8_t* next) {
+struct Converter {  // 4 bits: two strips of 16 rows a warp, lane 4 g + t has rows g and g + 8 of both
+  static __device__ __forceinline__ void expand(const uint8_t* block, uint8_t* out, int warp, int lane) {
     constexpr int kChunk = GemmCodesCfg<128, kSpans>::CHUNK_BYTES;
+    const uint8_t* codes = block + warp * 2048 + lane * 16;
+    const uint32_t* entries = reinterpret_cast<const uint32_t*>(block + kQ4CodeBytes) + warp * 32 + (lane >> 2);
+    uint8_t* to = out + (lane & 3) * kChunk + warp * 512 + (lane >> 2) * 16;
+    uint4 w[2][2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int panel = 0; panel < 4; ++panel) {
-        const uint4 pair = w[s][panel >> 1];
-        uint8_t* to = out + out_at + panel * 4 * kChunk + s * 256;
-        const int q = panel * kSpans / 4;
-        *reinterpret_cast<uint4*>(to) = q4_expand<kF16>(panel & 1 ? pair.z : pair.x, q4_zero<kF16>(entry[q][s][0] & 15u));
-        *reinterpret_cast<uint4*>(to + 128) = q4_expand<kF16>(panel & 1 ? pair.w : pair.y, q4_zero<kF16>(entry[q][s][1] & 15u));
+      for (int h = 0; h < 2; ++h) w[s][h] = *reinterpret_cast<const uint4*>(codes + s * 1024 + h * 512);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int q = 0; q < kSpans; ++q) {
+        const uint32_t zero0 = q4_zero<kF16>(entries[q * 128 + s * 16] & 15u), zero1 = q4_zero<kF16>(entries[q * 128 + s * 16 + 8] & 15u);
+#pragma unroll
+        for (int panel = q * 4 / kSpans; panel < (q + 1) * 4 / kSpans; ++panel) {
+          const uint4 pair = w[s][panel >> 1];
+          uint8_t* at = to + panel * 4 * kChunk + s * 256;
+          *reinterpret_cast<uint4*>(at) = q4_expand<kF16>(panel & 1 ? pair.z : pair.x, zero0);
+          *reinterpret_cast<uint4*>(at + 128) = q4_expand<kF16>(panel & 1 ? pair.w : pair.y, zero1);
+        }
       }
-      if (next) load_strip(next, s);
-    }
   }
 };
 template <bool kF16>
-struct Converter<kF16, 0> {  // 8 bits: one row
-  uint2 w[16];
-  int code_at, out_at;
-  __device__ __forceinline__ Converter(int warp, int lane) {
-    code_at = (warp * 32 + lane) * 8;
-    out_at = (warp * 32 + lane) * 16;
-  }
-  __device__ __forceinline__ void load(const uint8_t* block) {
+struct Converter<kF16, 0> {  // 8 bits: a lane a row
+  static __device__ __forceinline__ void expand(const uint8_t* block, uint8_t* out, int warp, int lane) {
+    const int row = warp * 32 + lane;
 #pragma unroll
-    for (int c = 0; c < 16; ++c) w[c] = ld_ahead64(block + code_at + c * 1024);
-  }
-  __device__ __forceinline__ void expand(uint8_t* out, const uint8_t* next) {
+    for (int c = 0; c < 16; c += 4) {
+      uint2 w[4];
 #pragma unroll
-    for (int c = 0; c < 16; ++c) {
-      *reinterpret_cast<uint4*>(out + out_at + c * GemmCodesCfg<128, 0>::CHUNK_BYTES) = q8_expand<kF16>(w[c]);
-      if (next) w[c] = ld_ahead64(next + code_at + c * 1024);
+      for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint2*>(block + (c + i) * 1024 + row * 8);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(out + (c + i) * GemmCodesCfg<128, 0>::CHUNK_BYTES + row * 16) = q8_expand<kF16>(w[i]);
     }
   }
 };
 
-// Launched with clusters of 1, 2, 4 or 8 CTAs (256 columns: 1): one tile of 128 rows x BN columns a cluster, whose CTAs divide the sum and add up through
-// shared memory, in the order of the sum.
+// Which rows and columns a tile is.  Sixteen rows of tiles at a time go through all columns: what is on at a time shares its operands.
+struct CodeTile {
+  int row, col;
+};
+__device__ __forceinline__ CodeTile code_tile(int tile, int rows, int cols) {
+  const int width = 16 * cols, group = tile / width, in = tile - group * width, size = min(16, rows - group * 16);
+  return {group * 16 + in % size, in / size};
+}
+
+// A cluster works on a tile at a time.
+//   BN = 64, 128: tiles of 128 x BN, clusters of 1, 2, 4 or 8 CTAs, which divide the sum and add up through shared memory, in its order.
+//   BN = 256: tiles of 256 x 256 on CTA pairs (tcgen05 cta_group::2), each with its 128 rows of codes and half of the columns of the dense
+//   operand; the leader issues the MMAs of both.  The peer's operands are announced to the leader by a relay thread.
 template <int BN, bool kF16, int kSpans>
 __global__ void __launch_bounds__(512, 1) tcec_gemm_codes_kernel(const GemmCodesParams p) {
   using Cfg = GemmCodesCfg<BN, kSpans>;
   constexpr int kGroups = Cfg::GROUPS;
+  constexpr bool kPair = Cfg::PAIR;
   extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t bar_code_full[Cfg::CODE_STAGES], bar_code_empty[Cfg::CODE_STAGES];
   __shared__ uint64_t bar_a_full[Cfg::A_STAGES], bar_a_empty[Cfg::A_STAGES];
   __shared__ uint64_t bar_b_full[Cfg::B_STAGES], bar_b_empty[Cfg::B_STAGES];
   __shared__ uint64_t bar_acc_full[2], bar_acc_free[2], bar_drain[1];
@@ -280,42 +270,58 @@ __global__ void __launch_bounds__(512, 1) tcec_gemm_codes_kernel(const GemmCodes
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
   const int warp = warp_index(), lane = threadIdx.x & 31;
-  const int shares = static_cast<int>(cluster_nctarank()), share = static_cast<int>(cluster_ctarank());
-  const int tile = blockIdx.x / shares;
-  const int rt = tile % p.row_tiles, ct = tile / p.row_tiles;
-  const int kb_first = static_cast<int>(static_cast<long long>(p.blocks) * share / shares);
-  const int kb_end = static_cast<int>(static_cast<long long>(p.blocks) * (share + 1) / shares);
-  const uint8_t* codes = p.codes + static_cast<size_t>(rt) * p.blocks * Cfg::BLOCK_BYTES;
-  const int cols = min(BN, p.cols - ct * BN), cols16 = (cols + 15) & ~15;
+  const int ctas = kPair ? 2 : static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
+  const bool leader = !kPair || rank == 0;
+  const int shares = kPair ? 1 : ctas;  // of the sum
+  const int first_tile = blockIdx.x / ctas, stride = gridDim.x / ctas;
+  const int tile_rows = kPair ? (p.row_tiles + 1) / 2 : p.row_tiles, ntiles = tile_rows * p.col_tiles;
+  const int kb_first = kPair ? 0 : static_cast<int>(static_cast<long long>(p.blocks) * rank / shares);
+  const int kb_end = kPair ? p.blocks : static_cast<int>(static_cast<long long>(p.blocks) * (rank + 1) / shares);
+  const int nkb = kb_end - kb_first;
+  auto row_tile = [&](const CodeTile& t) { return kPair ? t.row * 2 + rank : t.row; };
 
   if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::CODE_STAGES; ++s) {
+      mbar_init(smem_u32(&bar_code_full[s]), 1);
+      mbar_init(smem_u32(&bar_code_empty[s]), 4);
+    }
     for (int s = 0; s < Cfg::A_STAGES; ++s) {
-      mbar_init(smem_u32(&bar_a_full[s]), 4);
+      mbar_init(smem_u32(&bar_a_full[s]), kPair && leader ? 5 : 4);  // the converters; in a leader the peer's relay too
       mbar_init(smem_u32(&bar_a_empty[s]), 1);
     }
     for (int s = 0; s < Cfg::B_STAGES; ++s) {
-      mbar_init(smem_u32(&bar_b_full[s]), 1);
+      mbar_init(smem_u32(&bar_b_full[s]), kPair && leader ? 2 : 1);
       mbar_init(smem_u32(&bar_b_empty[s]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&bar_acc_full[i]), 1);
-      mbar_init(smem_u32(&bar_acc_free[i]), 8);
+      mbar_init(smem_u32(&bar_acc_free[i]), kPair ? 16 : 8);  // of a pair the leader's is used
     }
     mbar_init(smem_u32(&bar_drain[0]), 1);
     abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(&tmem_base_s), Cfg::TMEM_COLS);
-    tmem_relinquish();
+    if constexpr (kPair) {
+      tmem_alloc_pair(smem_u32(&tmem_base_s), Cfg::TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(&tmem_base_s), Cfg::TMEM_COLS);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
-  if (shares > 1) cluster_sync_all();  // the others' shared memory exists before anything is written to it
+  if (ctas > 1) cluster_sync_all();  // the others' barriers and shared memory exist before anything is written to them
   tc_fence_after();
   const uint32_t tmem = tmem_base_s;
   volatile uint32_t* abortp = &abort_flag;
   wait_for_launch_before();
+  auto give_up = [&](int code) {
+    if constexpr (kPair) raise_abort_pair(&abort_flag);
+    else abort_flag = 1;
+    atomicCAS(p.status, 0, code);
+  };
 
   float acc[Cfg::NC];
 
@@ -326,173 +332,243 @@ __global__ void __launch_bounds__(512, 1) tcec_gemm_codes_kernel(const GemmCodes
       if (elect_one()) {
         uint32_t bs = 0, bph = 0, armed = 0, armed_parity = 0;
         bool ok = true;
-        const uint8_t* src0 = p.panels + (static_cast<size_t>(ct * BN >> 7) * p.blocks + kb_first) * p.parts * kSpanBytes + (ct * BN & 127) * 64;
-        const uint8_t* src1 = src0 + static_cast<size_t>(p.blocks) * p.parts * kSpanBytes;  // the second 128 columns of 256
-        const uint32_t rows0 = min(128, cols16) * 64, rows1 = cols16 > 128 ? (cols16 - 128) * 64 : 0;
-        for (int left = (kb_end - kb_first) * p.parts * 2; left > 0; --left) {  // a half of a block and part
-          if (!mbar_wait(smem_u32(&bar_b_empty[bs]), bph ^ 1, abortp)) {
-            ok = false;
-            break;
+        for (int tile = first_tile; tile < ntiles && ok; tile += stride) {
+          const CodeTile ti = code_tile(tile, tile_rows, p.col_tiles);
+          const int col = ti.col * BN + (kPair ? rank * 128 : 0);
+          const uint32_t bytes = max(0, min(Cfg::BC, (p.cols - col + 15) & ~15)) * 64;  // a pair's second half may have no columns
+          const uint8_t* src = p.panels + (static_cast<size_t>(col >> 7) * p.blocks + kb_first) * p.parts * kSpanBytes + (col & 127) * 64;
+          for (int left = nkb * p.parts * 2; left > 0; --left) {  // a half of a block and part
+            if (!mbar_wait(smem_u32(&bar_b_empty[bs]), bph ^ 1, abortp)) {
+              ok = false;
+              break;
+            }
+            const uint32_t bfull = smem_u32(&bar_b_full[bs]);
+            if (bytes) {
+              mbar_arrive_expect_tx(bfull, 2 * bytes);
+              armed |= 1u << bs;
+              armed_parity = (armed_parity & ~(1u << bs)) | (bph << bs);
+              const uint32_t dst = smem_base + Cfg::B_OFFSET + bs * Cfg::B_BYTES;
+              bulk_load(dst, src, bytes, bfull);
+              bulk_load(dst + Cfg::BC * 64, src + kPanelBytes, bytes, bfull);
+            } else {
+              mbar_arrive(bfull);
+            }
+            src += 2 * kPanelBytes;
+            if (++bs == Cfg::B_STAGES) bs = 0, bph ^= 1;
           }
-          const uint32_t bfull = smem_u32(&bar_b_full[bs]);
-          mbar_arrive_expect_tx(bfull, 2 * (rows0 + rows1));
-          armed |= 1u << bs;
-          armed_parity = (armed_parity & ~(1u << bs)) | (bph << bs);
-          const uint32_t dst = smem_base + Cfg::B_OFFSET + bs * Cfg::B_BYTES;
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            bulk_load(dst + q * (BN * 64), src0 + q * kPanelBytes, rows0, bfull);
-            if (BN > 128 && rows1) bulk_load(dst + q * (BN * 64) + kPanelBytes, src1 + q * kPanelBytes, rows1, bfull);
-          }
-          src0 += 2 * kPanelBytes;
-          src1 += 2 * kPanelBytes;
-          if (++bs == Cfg::B_STAGES) bs = 0, bph ^= 1;
         }
         if (!ok) {
-          abort_flag = 1;
-          atomicCAS(p.status, 0, kErrProducerWait);
+          give_up(kErrProducerWait);
           // this thread's own copies land before the CTA gives up its shared memory
           for (uint32_t q = 0; q < Cfg::B_STAGES; ++q)
             if (armed & (1u << q)) mbar_wait_plain(smem_u32(&bar_b_full[q]), (armed_parity >> q) & 1);
         }
       }
-    } else if (warp == 1) {
-      // ---------------------------------------------------------- MMAs
+    } else if (warp == 2) {
+      // ---------------------------------------------------------- copies of the codes
       if (elect_one()) {
-        const uint64_t a_const = umma_desc_kmajor_noswizzle(0, Cfg::CHUNK_BYTES, 128), b_const = umma_desc_kmajor_noswizzle(0, 128, 512);
-        const uint32_t idesc = umma_idesc(kF16 ? 0u : 1u, 128, cols16);
-        const uint32_t a16 = ((smem_base + Cfg::A_OFFSET) & 0x3ffff) >> 4, b16 = ((smem_base + Cfg::B_OFFSET) & 0x3ffff) >> 4;
+        uint32_t cs = 0, cph = 0, armed = 0, armed_parity = 0;
+        bool ok = true;
+        for (int tile = first_tile; tile < ntiles && ok; tile += stride) {
+          const int rt = min(row_tile(code_tile(tile, tile_rows, p.col_tiles)), p.row_tiles - 1);  // the last pair may have one row of tiles
+          const uint8_t* src = p.codes + (static_cast<size_t>(rt) * p.blocks + kb_first) * Cfg::BLOCK_BYTES;
+          for (int kb = 0; kb < nkb; ++kb, src += Cfg::BLOCK_BYTES) {
+            if (!mbar_wait(smem_u32(&bar_code_empty[cs]), cph ^ 1, abortp)) {
+              ok = false;
+              break;
+            }
+            const uint32_t full = smem_u32(&bar_code_full[cs]);
+            mbar_arrive_expect_tx(full, Cfg::BLOCK_BYTES);
+            armed |= 1u << cs;
+            armed_parity = (armed_parity & ~(1u << cs)) | (cph << cs);
+            bulk_load(smem_base + Cfg::CODE_OFFSET + cs * Cfg::BLOCK_BYTES, src, Cfg::BLOCK_BYTES, full);
+            if (++cs == Cfg::CODE_STAGES) cs = 0, cph ^= 1;
+          }
+        }
+        if (!ok) {
+          give_up(kErrProducerWait);
+          for (uint32_t q = 0; q < Cfg::CODE_STAGES; ++q)
+            if (armed & (1u << q)) mbar_wait_plain(smem_u32(&bar_code_full[q]), (armed_parity >> q) & 1);
+        }
+      }
+    } else if (warp == 1) {
+      if (elect_one()) {
         uint32_t as = 0, aph = 0, bs = 0, bph = 0, fold = 0;
         bool ok = true;
-        for (int kb = kb_first; kb < kb_end && ok; ++kb) {
-          if (!mbar_wait(smem_u32(&bar_a_full[as]), aph, abortp, 0)) {
-            ok = false;
-            break;
-          }
-          const uint32_t a_here = a16 + as * (Cfg::A_BYTES >> 4);
-          for (int part = 0; part < p.parts && ok; ++part) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (!mbar_wait(smem_u32(&bar_b_full[bs]), bph, abortp, 0)) {
+        if (!leader) {
+          // -------------------------------------------------------- peer: "my operands are there"
+          for (int tile = first_tile; tile < ntiles && ok; tile += stride)
+            for (int kb = 0; kb < nkb && ok; ++kb) {
+              if (!mbar_wait(smem_u32(&bar_a_full[as]), aph, abortp, 0)) {
                 ok = false;
                 break;
               }
-              tc_fence_after();
-              const uint32_t b_here = b16 + bs * (Cfg::B_BYTES >> 4);
+              mbar_arrive_cluster(map_to_cta(smem_u32(&bar_a_full[as]), 0));
+              if (++as == Cfg::A_STAGES) as = 0, aph ^= 1;
+              for (int h = 0; h < 2 * p.parts; ++h) {
+                if (!mbar_wait(smem_u32(&bar_b_full[bs]), bph, abortp, 0)) {
+                  ok = false;
+                  break;
+                }
+                mbar_arrive_cluster(map_to_cta(smem_u32(&bar_b_full[bs]), 0));
+                if (++bs == Cfg::B_STAGES) bs = 0, bph ^= 1;
+              }
+            }
+          if (!ok) give_up(kErrMmaWait);
+        } else {
+          // -------------------------------------------------------- MMAs
+          const uint64_t a_const = umma_desc_kmajor_noswizzle(0, Cfg::CHUNK_BYTES, 128), b_const = umma_desc_kmajor_noswizzle(0, 128, 512);
+          const uint32_t a16 = ((smem_base + Cfg::A_OFFSET) & 0x3ffff) >> 4, b16 = ((smem_base + Cfg::B_OFFSET) & 0x3ffff) >> 4;
+          auto commit = [&](uint64_t* bar) {
+            if constexpr (kPair) umma_commit_pair(smem_u32(bar));
+            else umma_commit(smem_u32(bar));
+          };
+          for (int tile = first_tile; tile < ntiles && ok; tile += stride) {
+            const int cols = p.cols - code_tile(tile, tile_rows, p.col_tiles).col * BN;
+            const uint32_t idesc = umma_idesc(kF16 ? 0u : 1u, kPair ? 256 : 128, kPair ? 256 : min(BN, (cols + 15) & ~15));
+            for (int kb = 0; kb < nkb && ok; ++kb) {
+              if (!mbar_wait(smem_u32(&bar_a_full[as]), aph, abortp, 0)) {
+                ok = false;
+                break;
+              }
+              const uint32_t a_here = a16 + as * (Cfg::A_BYTES >> 4);
+              for (int part = 0; part < p.parts && ok; ++part) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int step = h * 4 + j;  // of 16 along the sum
-                // an accumulator holds one group; where a block is one, all parts of it
-                const bool first = step % (8 / kGroups) == 0 && (kGroups > 1 || part == 0);
-                const bool last = step % (8 / kGroups) == 8 / kGroups - 1 && (kGroups > 1 || part == p.parts - 1);
-                if (first) {
-                  if (!mbar_wait(smem_u32(&bar_acc_free[fold & 1]), ((fold >> 1) & 1) ^ 1, abortp, 0)) {
+                for (int h = 0; h < 2; ++h) {
+                  if (!mbar_wait(smem_u32(&bar_b_full[bs]), bph, abortp, 0)) {
                     ok = false;
                     break;
                   }
                   tc_fence_after();
-                }
-                umma_ss<false>(tmem + (fold & 1) * BN, a_const | (a_here + step * (2 * Cfg::CHUNK_BYTES >> 4)),
-                               b_const | (b_here + (j >> 1) * (BN * 64 >> 4) + (j & 1) * 16), idesc, first ? 0u : 1u);
-                if (last) {
-                  umma_commit(smem_u32(&bar_acc_full[fold & 1]));
-                  ++fold;
+                  const uint32_t b_here = b16 + bs * (Cfg::B_BYTES >> 4);
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    const int step = h * 4 + j;  // of 16 along the sum
+                    // an accumulator holds one group; where a block is one, all parts of it
+                    const bool first = step % (8 / kGroups) == 0 && (kGroups > 1 || part == 0);
+                    const bool last = step % (8 / kGroups) == 8 / kGroups - 1 && (kGroups > 1 || part == p.parts - 1);
+                    if (first) {
+                      if (!mbar_wait(smem_u32(&bar_acc_free[fold & 1]), ((fold >> 1) & 1) ^ 1, abortp, 0)) {
+                        ok = false;
+                        break;
+                      }
+                      tc_fence_after();
+                    }
+                    const uint64_t da = a_const | (a_here + step * (2 * Cfg::CHUNK_BYTES >> 4));
+                    const uint64_t db = b_const | (b_here + (j >> 1) * (Cfg::BC * 64 >> 4) + (j & 1) * 16);
+                    if constexpr (kPair) umma_ss_pair<false>(tmem + (fold & 1) * BN, da, db, idesc, first ? 0u : 1u);
+                    else umma_ss<false>(tmem + (fold & 1) * BN, da, db, idesc, first ? 0u : 1u);
+                    if (last) {
+                      commit(&bar_acc_full[fold & 1]);
+                      ++fold;
+                    }
+                  }
+                  if (!ok) break;
+                  commit(&bar_b_empty[bs]);
+                  if (++bs == Cfg::B_STAGES) bs = 0, bph ^= 1;
                 }
               }
               if (!ok) break;
-              umma_commit(smem_u32(&bar_b_empty[bs]));
-              if (++bs == Cfg::B_STAGES) bs = 0, bph ^= 1;
+              commit(&bar_a_empty[as]);
+              if (++as == Cfg::A_STAGES) as = 0, aph ^= 1;
             }
           }
-          if (!ok) break;
-          umma_commit(smem_u32(&bar_a_empty[as]));
-          if (++as == Cfg::A_STAGES) as = 0, aph ^= 1;
+          if (!ok) mma_thread_gave_up<kPair>(&abort_flag, p.status, kErrMmaWait, &bar_drain[0]);
         }
-        if (!ok) mma_thread_gave_up<false>(&abort_flag, p.status, kErrMmaWait, &bar_drain[0]);
       }
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------ codes to operands
-    if constexpr (Cfg::REBALANCE) setmaxnreg_dec<72>();
-    Converter<kF16, kSpans> held(warp - 4, lane);
-    uint32_t as = 0, aph = 0;
+    if constexpr (Cfg::REBALANCE) setmaxnreg_dec<56>();
+    uint32_t cs = 0, cph = 0, as = 0, aph = 0, slot = 0;
+    const int t = threadIdx.x - 128;
     bool ok = true;
-    if (kb_first < kb_end) held.load(codes + static_cast<size_t>(kb_first) * Cfg::BLOCK_BYTES);
-    for (int kb = kb_first; kb < kb_end; ++kb) {
-      if (!mbar_wait_warp(smem_u32(&bar_a_empty[as]), aph ^ 1, abortp, 64)) {
-        ok = false;
-        break;
+    for (int tile = first_tile; tile < ntiles && ok; tile += stride)
+      for (int kb = 0; kb < nkb; ++kb) {
+        if (!mbar_wait_lanes(smem_u32(&bar_code_full[cs]), cph, abortp) || !mbar_wait_lanes(smem_u32(&bar_a_empty[as]), aph ^ 1, abortp)) {
+          ok = false;
+          break;
+        }
+        const uint8_t* block = smem_gen + Cfg::CODE_OFFSET + cs * Cfg::BLOCK_BYTES;
+        // The scales, for those who come to them when the products are made.  A slot is written again six blocks later; the stage just
+        // waited for says that the MMAs of three blocks before are done, for which the accumulators of five blocks before were free.
+        float* scales = reinterpret_cast<float*>(smem_gen + Cfg::SCALE_OFFSET) + slot * (kGroups * 128) + t;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+          scales[g * 128] = __uint_as_float(reinterpret_cast<const uint32_t*>(block + Cfg::CODE_BYTES)[g * 128 + t] & (Cfg::Q8 ? ~0u : ~15u));
+        Converter<kF16, kSpans>::expand(block, smem_gen + Cfg::A_OFFSET + as * Cfg::A_BYTES, warp - 4, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&bar_a_full[as]));
+          mbar_arrive(smem_u32(&bar_code_empty[cs]));
+        }
+        if (++cs == Cfg::CODE_STAGES) cs = 0, cph ^= 1;
+        if (++as == Cfg::A_STAGES) as = 0, aph ^= 1;
+        if (++slot == Cfg::SCALE_SLOTS) slot = 0;
       }
-      held.expand(smem_gen + Cfg::A_OFFSET + as * Cfg::A_BYTES, kb + 1 < kb_end ? codes + static_cast<size_t>(kb + 1) * Cfg::BLOCK_BYTES : nullptr);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_a_full[as]));
-      if (++as == Cfg::A_STAGES) as = 0, aph ^= 1;
-    }
-    if (!ok) {
-      abort_flag = 1;
-      if (lane == 0) atomicCAS(p.status, 0, kErrOperandWait);
-    }
+    if (!ok && lane == 0) give_up(kErrOperandWait);
   } else {
     // ------------------------------------------------------------ scales
-    if constexpr (Cfg::REBALANCE) setmaxnreg_inc<200>();
-#pragma unroll
-    for (int i = 0; i < Cfg::NC; ++i) acc[i] = 0.f;
+    if constexpr (Cfg::REBALANCE) setmaxnreg_inc<208>();
     const int q = warp & 3, r = q * 32 + lane, first_col = (warp >= 12 ? Cfg::NC : 0);
     const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + first_col;
-    const bool any = first_col < cols;
+    const float* scales = reinterpret_cast<const float*>(smem_gen + Cfg::SCALE_OFFSET) + r;
     const int rounds = kGroups > 1 ? p.parts : 1;  // of the groups of a block
-    uint32_t fold = 0;
+    uint32_t fold = 0, slot = 0;
     bool ok = true;
-    float scale[kGroups], next[kGroups];
-    auto load_scales = [&](int kb) {
+    for (int tile = first_tile; tile < ntiles && ok; tile += stride) {
+      const CodeTile ti = code_tile(tile, tile_rows, p.col_tiles);
+      const int col0 = ti.col * BN + first_col, cols = p.cols - col0;  // from this warp's first column on
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g)
-        next[g] = __uint_as_float(ld_ahead32(codes + static_cast<size_t>(kb) * Cfg::BLOCK_BYTES + Cfg::CODE_BYTES + g * kEntryBytes + r * 4) &
-                                  (Cfg::Q8 ? ~0u : ~15u));
-    };
-    if (kb_first < kb_end) load_scales(kb_first);
-    for (int kb = kb_first; kb < kb_end && ok; ++kb) {
+      for (int i = 0; i < Cfg::NC; ++i) acc[i] = 0.f;
+      for (int kb = 0; kb < nkb && ok; ++kb) {
+        for (int round = 0; round < rounds && ok; ++round) {
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) scale[g] = next[g];
-      if (kb + 1 < kb_end) load_scales(kb + 1);
-      for (int round = 0; round < rounds && ok; ++round) {
+          for (int g = 0; g < kGroups; ++g, ++fold) {
+            if (!mbar_wait_lanes(smem_u32(&bar_acc_full[fold & 1]), (fold >> 1) & 1, abortp)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            if (cols > 0) {
+              const float s = scales[(slot * kGroups + g) * 128];
+              const uint32_t from = taddr + (fold & 1) * BN;
+              if constexpr (Cfg::NC == 32) {
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(from, v);
+                tmem_ld_wait();
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g, ++fold) {
-          if (!mbar_wait_warp(smem_u32(&bar_acc_full[fold & 1]), (fold >> 1) & 1, abortp, 64)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          if (any) {
-            uint32_t v[2][16];
-            tmem_ld_32x32b_x16(taddr + (fold & 1) * BN, v[0]);
+                for (int j = 0; j < 32; j += 2) fma2(acc[j], acc[j + 1], __uint_as_float(v[j]), __uint_as_float(v[j + 1]), s);
+              } else {
+                uint32_t v[2][32];
+                tmem_ld_32x32b_x32(from, v[0]);
 #pragma unroll
-            for (int i = 0; i < Cfg::NC; i += 16) {
-              tmem_ld_wait();
-              if (i + 16 < Cfg::NC) tmem_ld_32x32b_x16(taddr + (fold & 1) * BN + i + 16, v[(i / 16 + 1) & 1]);
+                for (int i = 0; i < Cfg::NC; i += 32) {
+                  tmem_ld_wait();
+                  if (i + 32 < Cfg::NC) tmem_ld_32x32b_x32(from + i + 32, v[(i / 32 + 1) & 1]);
 #pragma unroll
-              for (int j = 0; j < 16; j += 2)
-                fma2(acc[i + j], acc[i + j + 1], __uint_as_float(v[(i / 16) & 1][j]), __uint_as_float(v[(i / 16) & 1][j + 1]), scale[g]);
+                  for (int j = 0; j < 32; j += 2)
+                    fma2(acc[i + j], acc[i + j + 1], __uint_as_float(v[(i / 32) & 1][j]), __uint_as_float(v[(i / 32) & 1][j + 1]), s);
+                }
+              }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (kPair) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_acc_free[fold & 1]), 0));
+              else mbar_arrive(smem_u32(&bar_acc_free[fold & 1]));
             }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&bar_acc_free[fold & 1]));
         }
+        if (++slot == Cfg::SCALE_SLOTS) slot = 0;
       }
-    }
-    if (!ok) {
-      abort_flag = 1;
-      if (lane == 0) atomicCAS(p.status, 0, kErrEpilogueWait);
-    }
-    if (shares == 1 && ok) {
-      const int row = rt * 128 + r;
-      if (row < p.rows) {
-        const long long base = row * p.c_row + static_cast<long long>(ct * BN + first_col) * p.c_col;
+      const int row = row_tile(ti) * 128 + r;
+      if (shares == 1 && ok && row < p.rows) {
+        const long long base = row * p.c_row + col0 * p.c_col;
 #pragma unroll
         for (int i = 0; i < Cfg::NC; ++i)
-          if (first_col + i < cols) {
+          if (i < cols) {
             const long long at = base + i * p.c_col;
             float v = __fmul_rn(p.alpha, acc[i]);
             if (p.beta != 0.f) v = __fmaf_rn(p.beta, ld_element_as(p.c_type, p.c, at), v);
@@ -500,21 +576,26 @@ __global__ void __launch_bounds__(512, 1) tcec_gemm_codes_kernel(const GemmCodes
           }
       }
     }
+    if (!ok && lane == 0) give_up(kErrEpilogueWait);
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, Cfg::TMEM_COLS);
-  if constexpr (!Cfg::REBALANCE) {
-    if (shares > 1) {
+  if constexpr (kPair) {
+    cluster_sync_all();  // neither CTA leaves while the other may still signal it or read its operands
+    if (warp == 1) tmem_dealloc_pair(tmem, Cfg::TMEM_COLS);
+  } else {
+    if (warp == 1) tmem_dealloc(tmem, Cfg::TMEM_COLS);
+    if (shares > 1) {  // then a cluster has one tile
       cluster_sync_all();  // nobody reads operands any more where the partial results go
+      const CodeTile ti = code_tile(first_tile, tile_rows, p.col_tiles);
       const int per = BN / shares;  // columns that a CTA adds up and stores
       if (warp >= 8) {
         const int r = (warp & 3) * 32 + lane, first_col = (warp >= 12 ? Cfg::NC : 0);
 #pragma unroll
         for (int i = 0; i < Cfg::NC; ++i) {
           const int col = first_col + i, to = col / per;
-          const uint32_t at = smem_base + Cfg::B_OFFSET + ((share * per + col - to * per) * 128 + r) * 4;
+          const uint32_t at = smem_base + Cfg::B_OFFSET + ((rank * per + col - to * per) * 128 + r) * 4;
           asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(at, to)), "f"(acc[i]) : "memory");
         }
       }
@@ -523,15 +604,15 @@ __global__ void __launch_bounds__(512, 1) tcec_gemm_codes_kernel(const GemmCodes
       __syncwarp();
       cluster_sync_all();
       if (warp >= 8 && !*abortp) {
-        const int t = threadIdx.x - 256, r = t & 127, row = rt * 128 + r;
+        const int t = threadIdx.x - 256, r = t & 127, row = ti.row * 128 + r;
         if (row < p.rows) {
           const float* parts = reinterpret_cast<const float*>(smem_gen + Cfg::B_OFFSET) + r;
           for (int i = t >> 7; i < per; i += 2) {
-            const int col = share * per + i;
-            if (col >= cols) break;
+            const int col = ti.col * BN + rank * per + i;
+            if (col >= p.cols) break;
             float v = parts[i * 128];
             for (int s = 1; s < shares; ++s) v += parts[(s * per + i) * 128];
-            const long long at = row * p.c_row + static_cast<long long>(ct * BN + col) * p.c_col;
+            const long long at = row * p.c_row + col * p.c_col;
             v = __fmul_rn(p.alpha, v);
             if (p.beta != 0.f) v = __fmaf_rn(p.beta, ld_element_as(p.c_type, p.c, at), v);
             st_element_as(p.c_type, p.c, at, v);
