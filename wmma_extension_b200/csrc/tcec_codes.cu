@@ -85,6 +85,9 @@ cudaError_t set_all_codes_attrs() {
   return e;
 }
 
+template <int T>
+cudaError_t set_gemv_attrs();
+
 // What a launch needs to know of the current device.
 struct Here {
   int* status;
@@ -98,6 +101,9 @@ int get_here(Here* out) {
   if (!st->codes_attrs_done) {
     TCEC_CUDA(set_all_codes_attrs<false>());
     TCEC_CUDA(set_all_codes_attrs<true>());
+    TCEC_CUDA(set_gemv_attrs<kTypeF32>());
+    TCEC_CUDA(set_gemv_attrs<kTypeF16>());
+    TCEC_CUDA(set_gemv_attrs<kTypeBf16>());
     st->codes_attrs_done = true;
   }
   *out = {st->status, st->sm_count};
@@ -150,13 +156,19 @@ template <int T>
 struct StagePanels {
   static void go(int grid, cudaStream_t stream, const StagePanelsParams& p) { launch_early(stage_panels_kernel<T>, grid, 256, 0, stream, p); }
 };
+template <int T, int G, int C, int S>
+void launch_gemv(cudaStream_t stream, const GemvQ4Params& p) {
+  using Cfg = GemvQ4Cfg<T, G, C, S>;
+  launch_early(gemv_q4_kernel<T, G, C, S>, static_cast<int>(ceil_div(p.n, Cfg::ROWS)), 32 * Cfg::WARPS, Cfg::SMEM_BYTES, stream, p);
+}
 template <int T>
 struct GemvQ4 {
   template <int G>
   static void of_group(int columns, cudaStream_t stream, const GemvQ4Params& p) {
-    if (columns <= 8) launch_early(gemv_q4_kernel<T, G, 1, 1>, static_cast<int>(ceil_div(p.n, 16)), 256, 0, stream, p);
-    else if (columns <= 16) launch_early(gemv_q4_kernel<T, G, 2, 2>, static_cast<int>(ceil_div(p.n, 32)), 256, 0, stream, p);
-    else launch_early(gemv_q4_kernel<T, G, 4, 2>, static_cast<int>(ceil_div(p.n, 32)), 256, 0, stream, p);
+    if (columns <= 8 && p.n <= 8192) launch_gemv<T, G, 1, 1>(stream, p);
+    else if (columns <= 8) launch_gemv<T, G, 1, 2>(stream, p);
+    else if (columns <= 16) launch_gemv<T, G, 2, 2>(stream, p);
+    else launch_gemv<T, G, 4, 2>(stream, p);
   }
   static void go(int group, int columns, cudaStream_t stream, const GemvQ4Params& p) {
     if (group == 32) of_group<32>(columns, stream, p);
@@ -164,6 +176,17 @@ struct GemvQ4 {
     else of_group<128>(columns, stream, p);
   }
 };
+template <int T, int G, int C, int S>
+cudaError_t set_gemv_attr() {
+  return cudaFuncSetAttribute(gemv_q4_kernel<T, G, C, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, GemvQ4Cfg<T, G, C, S>::SMEM_BYTES);
+}
+template <int T>
+cudaError_t set_gemv_attrs() {  // the others stay below what needs no permission
+  cudaError_t e = set_gemv_attr<T, 32, 4, 2>();
+  if (e == cudaSuccess) e = set_gemv_attr<T, 64, 4, 2>();
+  if (e == cudaSuccess) e = set_gemv_attr<T, 128, 4, 2>();
+  return e;
+}
 
 template <int BN, bool F, int S>
 void launch_codes_as(const GemmCodesParams& gp, int shares, int grid, cudaStream_t stream) {
@@ -356,10 +379,9 @@ int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, c
     Here here;
     const int rc = get_here(&here);
     if (rc != TCEC_OK) return rc;
-    const bool vec = layout_x == TCEC_ROW_MAJOR && dx.wide(16);
     if (!streamed(m, type_x))
-      return gemm_codes(packed, kCodeSpan / group, n, m, sum, x, dx.row_step(), dx.col_step(), type_x, vec, alpha, beta, c, dc.col_step(),
-                        dc.row_step(), type_c, workspace, here, static_cast<cudaStream_t>(stream));
+      return gemm_codes(packed, kCodeSpan / group, n, m, sum, x, dx.row_step(), dx.col_step(), type_x, layout_x == TCEC_ROW_MAJOR && dx.wide(16), alpha,
+                        beta, c, dc.col_step(), dc.row_step(), type_c, workspace, here, static_cast<cudaStream_t>(stream));
     GemvQ4Params p{};
     p.codes = static_cast<const uint8_t*>(packed);
     p.x = x;
@@ -369,7 +391,7 @@ int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, c
     p.k = sum;
     p.tokens = m;
     p.blocks = static_cast<int>(ceil_div(sum, kCodeSpan));
-    p.vec = vec;
+    p.vec = layout_x == TCEC_ROW_MAJOR && dx.wide(4 * type_bytes(type_x));
     p.alpha = alpha;
     p.beta = beta;
     p.c = c;

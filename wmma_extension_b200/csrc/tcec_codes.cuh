@@ -16,7 +16,7 @@
 //   nibble j of them k = 2 j (j < 4) and 2 (j - 4) + 1, so that (w >> 4 i) & 0x000f000f is the pair (2 i, 2 i + 1).  Words are in the
 //   order of the registers of mma.m16n8k16: lane 4 g + t of a warp finds rows g and g + 8, k = 8 t .. 8 t + 7 of each 32, in two
 //   128-bit loads.  An entry is the scale as FP32 (its low 12 bits or more are zero) with the zero point in the low 4 bits.
-//   8-bit block: 16 chunks of 8 tokens x 128 features x 8 bytes (sign and magnitude), then 128 FP32 scales.
+//   8-bit block: 8 x 16 tokens x 128 features x 16 bytes (sign and magnitude; tokens 0 2 1 3 of each four), then 128 FP32 scales.
 //
 // Packing and unpacking are bound by memory: every value is read once and written once.
 #pragma once
@@ -24,6 +24,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "sm100_ptx.cuh"
 
@@ -99,21 +100,54 @@ __device__ __forceinline__ float ld_element(const void* base, long long at) {
     return __uint_as_float(static_cast<uint32_t>(ld_operand16(static_cast<const uint16_t*>(base) + at)) << 16);
   }
 }
-// Four consecutive elements of an address that is aligned for them.
+// Four elements as they come, to be widened later: loads that are widened behind a branch wait for one another.
 template <int kType>
-__device__ __forceinline__ void ld_elements4(const void* base, long long at, float (&v)[4]) {
-  if constexpr (kType == kTypeF32) {
-    const float4 f = ld_operand(reinterpret_cast<const float4*>(static_cast<const float*>(base) + at));
-    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-  } else {
-    const uint2 w = ld_operand64(static_cast<const uint16_t*>(base) + at);
-    if constexpr (kType == kTypeF16) {
-      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+struct Four {
+  typename std::conditional<kType == kTypeF32, float4, uint2>::type raw;
+  // Consecutive ones, of an address that is aligned for them.
+  __device__ __forceinline__ void load(const void* base, long long at) {
+    if constexpr (kType == kTypeF32) raw = ld_operand(reinterpret_cast<const float4*>(static_cast<const float*>(base) + at));
+    else raw = ld_operand64(static_cast<const uint16_t*>(base) + at);
+  }
+  __device__ __forceinline__ void get(float (&v)[4]) const {
+    if constexpr (kType == kTypeF32) {
+      v[0] = raw.x, v[1] = raw.y, v[2] = raw.z, v[3] = raw.w;
+    } else if constexpr (kType == kTypeF16) {
+      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&raw.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
       v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
     } else {
-      v[0] = __uint_as_float(w.x << 16), v[1] = __uint_as_float(w.x & 0xffff0000u);
-      v[2] = __uint_as_float(w.y << 16), v[3] = __uint_as_float(w.y & 0xffff0000u);
+      v[0] = __uint_as_float(raw.x << 16), v[1] = __uint_as_float(raw.x & 0xffff0000u);
+      v[2] = __uint_as_float(raw.y << 16), v[3] = __uint_as_float(raw.y & 0xffff0000u);
     }
+  }
+};
+// kLines x 4 elements: line i < lines_left at base + i * line_step, in it element j < left at + j * step; zeros for those beyond.  Addresses stay
+// among the elements that exist.  `wide`: four elements lie side by side, aligned.
+template <int kType, int kLines>
+__device__ __forceinline__ void ld_lines4(const void* base, long long at, long long line_step, long long step, int lines_left, int left, bool wide,
+                                          float (&v)[kLines][4]) {
+  if (lines_left <= 0 || left <= 0) {
+#pragma unroll
+    for (int i = 0; i < kLines; ++i) v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
+  } else if (wide && left >= 4) {
+    Four<kType> f[kLines];
+#pragma unroll
+    for (int i = 0; i < kLines; ++i) f[i].load(base, at + min(i, lines_left - 1) * line_step);
+#pragma unroll
+    for (int i = 0; i < kLines; ++i) {
+      f[i].get(v[i]);
+      if (i >= lines_left) v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kLines; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = ld_element<kType>(base, at + min(i, lines_left - 1) * line_step + min(j, left - 1) * step);
+#pragma unroll
+    for (int i = 0; i < kLines; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i >= lines_left || j >= left) v[i][j] = 0.f;
   }
 }
 template <int kType>
@@ -132,24 +166,34 @@ __device__ __forceinline__ float ld_element_as(int type, const void* base, long 
 }
 
 // ---------------------------------------------------------------- arithmetic of the codes
-// rint(x / s) of the exact quotient, ties to even, for |x / s| below 2^8.
+// rint(x / s) of the exact quotient, ties to even, for |x / s| below 2^8, without a branch: with values of few bits, as bf16 has, one in
+// some hundred quotients is a tie or next to one, so hardly a warp is without (8192 x 4096 bf16 to 8 bits 125 us with the exact way in a branch).
 //
-// q0 = rint(x * (1 / s)) is off by at most one (a scale below the normal numbers, whose inverse may overflow, is divided by).  The
-// remainder r = x - q0 s is exact in FP32: x and q0 s are both multiples of half the last place of s whenever |x| is at least s / 2, and
-// |r| stays below 2 s; where |x| is smaller, q0 is 0 or +-1.  Comparing 2 r with s decides.
+// q = x * (1 / s) + 1.5 * 2^23, whose last place is 1, is off by at most one.  The remainder r = x - q s is exact in FP32: x and q s are both
+// multiples of half the last place of s whenever |x| is at least s / 2, and |r| stays below 2 s; where |x| is smaller, q is 0 or +-1.  The sign of
+// 2 |r| - s decides; a tie (0) of an odd q does too, as the number whose bits are that one bit.
+constexpr float kRintBase = 12582912.0f;
 struct Quotient {
   float s, inv;
   __device__ __forceinline__ explicit Quotient(float scale) {
     s = scale;
     inv = scale < 0x1p-126f ? 0.0f : __fdiv_rn(1.0f, scale);
   }
-  __device__ __forceinline__ float rint_of(float x) const {
-    float q = rintf(inv != 0.0f ? x * inv : __fdiv_rn(x, s));
-    const float r = __fmaf_rn(-q, s, x), r2 = r + r;
-    const bool odd = (static_cast<int>(q) & 1) != 0;
-    if (r2 > s || (r2 == s && odd)) q += 1.0f;
-    else if (r2 < -s || (r2 == -s && odd)) q -= 1.0f;
-    return q;
+  // A scale below the normal numbers, whose inverse may overflow, is not for nearest().
+  __device__ __forceinline__ bool tiny() const { return inv == 0.0f; }
+  // kRintBase + rint(x / s), as bits.
+  __device__ __forceinline__ int nearest(float x) const {
+    const float q = __fmaf_rn(x, inv, kRintBase), r = __fmaf_rn(kRintBase - q, s, x);
+    const int bits = __float_as_int(q);
+    const float past = __fmaf_rn(2.0f, fabsf(r), -s) + __int_as_float(bits & 1);
+    return past > 0.0f ? bits + ((__float_as_int(r) >> 31) | 1) : bits;
+  }
+  __device__ __forceinline__ int nearest_of_tiny(float x) const {
+    const float q = rintf(__fdiv_rn(x, s)), r = __fmaf_rn(-q, s, x), r2 = r + r;
+    int n = __float_as_int(q + kRintBase);
+    if (r2 > s || (r2 == s && (n & 1))) ++n;
+    else if (r2 < -s || (r2 == -s && (n & 1))) --n;
+    return n;
   }
 };
 __device__ __forceinline__ bool not_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
@@ -175,64 +219,84 @@ struct PackQ4Params {
 
 __device__ __forceinline__ uint32_t q4_entry(float s, int z) { return (__float_as_uint(s) & ~15u) | static_cast<uint32_t>(z); }
 
-// One CTA a block: a warp takes a row at a time, a lane four consecutive k of it; words gather in shared memory and leave together.
+// One CTA a block.  A warp takes eight rows at a time, four lanes a row: lane 4 g + t has k = 16 j + 4 t .. + 3 of row g for j < 8, so a
+// group is two exchanges away at most.  Words gather in shared memory and leave together.
 template <int kType, int kGroup>
 __global__ void __launch_bounds__(256) pack_q4_kernel(const PackQ4Params p) {
-  __shared__ __align__(16) uint32_t words[2048 + 128 * (kCodeSpan / kGroup)];
+  constexpr int kSpans = kCodeSpan / kGroup;
+  __shared__ __align__(16) uint32_t words[2048 + 128 * kSpans];
   wait_for_launch_before();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int kb = blockIdx.x % p.blocks, tile = blockIdx.x / p.blocks;
-  const int k0 = kb * kCodeSpan + lane * 4;
-#pragma unroll 4
-  for (int i = 0; i < 16; ++i) {
-    const int r = warp * 16 + i, row = tile * kCodeRows + r;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (row < p.n) {
-      const long long at = row * p.row_step + k0 * p.k_step;
-      if (p.vec && k0 + 4 <= p.k) {
-        ld_elements4<kType>(p.w, at, v);
-      } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (k0 + j < p.k) v[j] = ld_element<kType>(p.w, at + j * p.k_step);
+  for (int half = 0; half < 2; ++half) {
+    const int r = warp * 16 + half * 8 + g, row = tile * kCodeRows + r, k0 = kb * kCodeSpan + t * 4;
+    float v[8][4];
+    const int left = row < p.n ? p.k - k0 : 0;
+    if (p.vec && left >= 7 * 16 + 4) {
+      Four<kType> f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j].load(p.w, row * p.row_step + k0 + j * 16);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j].get(v[j]);
+    } else if (left > 0) {  // unaligned, column-major or at the edge: addresses stay inside the row
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[j][i] = ld_element<kType>(p.w, row * p.row_step + (k0 + min(j * 16 + i, left - 1)) * p.k_step);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (j * 16 + i >= left) v[j][i] = 0.f;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j][0] = v[j][1] = v[j][2] = v[j][3] = 0.f;
+    }
+    if (half == 1) let_next_launch_start();
+#pragma unroll
+    for (int q = 0; q < kSpans; ++q) {  // groups; 128 / kSpans = 16 * 8 / kSpans
+      float lo = 0.f, hi = 0.f;
+      uint32_t most = 0;  // magnitude as bits, among which infinities and NaN come last
+#pragma unroll
+      for (int j = q * 8 / kSpans; j < (q + 1) * 8 / kSpans; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo = fminf(lo, v[j][i]);
+          hi = fmaxf(hi, v[j][i]);
+          most = max(most, __float_as_uint(v[j][i]) & 0x7fffffffu);
+        }
+#pragma unroll
+      for (int d = 1; d <= 2; d <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
       }
-    }
-    float lo = 0.f, hi = 0.f;
-    bool bad = false;
+      const float want = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
+      const float s = p.scale_bf16 ? __bfloat162float(__float2bfloat16_rn(want)) : __half2float(__float2half_rn(want));
+      const bool bad = most >= 0x7f800000u || not_finite(s), some = !bad && s > 0.f;
+      const Quotient by(some ? s : 1.0f);
+      const int base = __float_as_int(kRintBase), z = !some ? 0 : min((by.tiny() ? by.nearest_of_tiny(-lo) : by.nearest(-lo)) - base, 15);
+      uint32_t code[8 / kSpans];
+      auto make_codes = [&](auto nearest) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      lo = fminf(lo, v[j]);
-      hi = fmaxf(hi, v[j]);
-      bad |= not_finite(v[j]);
-    }
+        for (int j = 0; j < 8 / kSpans; ++j) {
+          code[j] = 0;
 #pragma unroll
-    for (int d = kGroup / 8; d >= 1; d >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-    }
-    const uint32_t bads = __ballot_sync(0xffffffffu, bad);
-    constexpr uint32_t kOfGroup = kGroup == 128 ? 0xffffffffu : kGroup == 64 ? 0xffffu : 0xffu;
-    bad = ((bads >> (lane & ~(kGroup / 4 - 1))) & kOfGroup) != 0;
-    const float want = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
-    const float s = p.scale_bf16 ? __bfloat162float(__float2bfloat16_rn(want)) : __half2float(__float2half_rn(want));
-    bad |= not_finite(s);
-    uint32_t code = 0;
-    float z = 0.f;
-    if (!bad && s > 0.f) {
-      const Quotient by(s);
-      z = fminf(by.rint_of(-lo), 15.0f);
+          for (int i = 0; i < 4; ++i)  // half of a word
+            code[j] |= static_cast<uint32_t>(min(max(nearest(v[q * 8 / kSpans + j][i]) + (z - base), 0), 15)) << ((i & 1) * 16 + (i >> 1) * 4);
+        }
+      };
+      if (!by.tiny()) make_codes([&](float x) { return by.nearest(x); });
+      else make_codes([&](float x) { return by.nearest_of_tiny(x); });
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int q = static_cast<int>(fminf(fmaxf(by.rint_of(v[j]) + z, 0.0f), 15.0f));
-        code |= static_cast<uint32_t>(q) << ((j & 1) * 16 + (j >> 1) * 4);  // the first half of a word; the odd lane's is 8 higher
+      for (int j = 0; j < 8 / kSpans; ++j) {
+        const uint32_t mine = some ? code[j] : 0, other = __shfl_xor_sync(0xffffffffu, mine, 1);  // the odd lane's half is 8 bits higher
+        if ((t & 1) == 0) words[q4_word(r, (q * 8 / kSpans + j) * 2 + (t >> 1))] = mine | (other << 8);
       }
+      if (t == 0) words[2048 + q * 128 + r] = q4_entry(bad ? nan32() : s, z);
     }
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, code, 1);
-    if ((lane & 1) == 0) words[q4_word(r, lane >> 1)] = code | (other << 8);
-    if ((lane & (kGroup / 4 - 1)) == 0)
-      words[2048 + (lane / (kGroup / 4)) * 128 + r] = q4_entry(bad ? nan32() : s, static_cast<int>(z));
   }
-  let_next_launch_start();
   __syncthreads();
   uint4* out = reinterpret_cast<uint4*>(p.packed + (static_cast<size_t>(tile) * p.blocks + kb) * q4_block_bytes(kGroup));
   for (int i = threadIdx.x; i < q4_block_bytes(kGroup) / 16; i += 256) out[i] = reinterpret_cast<const uint4*>(words)[i];
@@ -340,23 +404,10 @@ __global__ void __launch_bounds__(256) pack_q8_kernel(const PackQ8Params p) {
   __shared__ float4 most[8][32];
   wait_for_launch_before();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tile = blockIdx.x / p.token_blocks, tb = blockIdx.x % p.token_blocks;
+  const int tiles = (p.features + kCodeRows - 1) / kCodeRows, tile = blockIdx.x % tiles, tb = blockIdx.x / tiles;  // whole rows at a time
   const int f0 = tile * kCodeRows + lane * 4, t0 = tb * kCodeSpan + warp * 16;
   float v[16][4];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
-    if (t0 + i < p.tokens) {
-      const long long at = (t0 + i) * p.token_step + f0 * p.feature_step;
-      if (p.vec && f0 + 4 <= p.features) {
-        ld_elements4<kType>(p.x, at, v[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (f0 + j < p.features) v[i][j] = ld_element<kType>(p.x, at + j * p.feature_step);
-      }
-    }
-  }
+  ld_lines4<kType, 16>(p.x, t0 * p.token_step + f0 * p.feature_step, p.token_step, p.feature_step, p.tokens - t0, p.features - f0, p.vec, v);
   let_next_launch_start();
   float m[4] = {0.f, 0.f, 0.f, 0.f};  // the largest magnitude as bits, among which infinities and NaN come last
 #pragma unroll
@@ -375,73 +426,67 @@ __global__ void __launch_bounds__(256) pack_q8_kernel(const PackQ8Params p) {
   }
   uint8_t* block = p.packed + (static_cast<size_t>(tile) * p.token_blocks + tb) * kQ8BlockBytes;
   float scale[4];
-  uint32_t w[2][4][2] = {};  // chunk of eight tokens, feature, half of the chunk
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const bool bad = not_finite(m[j]);
-    const float s = fmaxf(__fdiv_rn(m[j], 127.0f), 0x1p-120f);
+    const float s = bad ? 1.0f : fmaxf(__fdiv_rn(m[j], 127.0f), 0x1p-120f);
     scale[j] = bad ? nan32() : s;
-    if (bad) continue;
     const Quotient by(s);
+    uint32_t q[16];  // magnitudes, in the low bytes
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int q = static_cast<int>(by.rint_of(v[i][j]));
-      const uint32_t code = static_cast<uint32_t>(q < 0 ? 128 - q : q);
-      w[i >> 3][j][(i >> 2) & 1] |= code << ((i & 3) * 8);
+    for (int i = 0; i < 16; ++i) q[i] = by.nearest(fabsf(v[i][j]));
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // tokens 0 2 1 3 of each four, and their signs
+      const uint32_t size = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 2], 0x0040), __byte_perm(q[4 * i + 1], q[4 * i + 3], 0x0040), 0x5410);
+      const uint32_t sign = __byte_perm(__byte_perm(__float_as_uint(v[4 * i][j]), __float_as_uint(v[4 * i + 2][j]), 0x0073),
+                                        __byte_perm(__float_as_uint(v[4 * i + 1][j]), __float_as_uint(v[4 * i + 3][j]), 0x0073), 0x5410);
+      w[i] = bad ? 0 : (size & 0x7f7f7f7fu) | (sign & 0x80808080u);
     }
-  }
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint4* to = reinterpret_cast<uint4*>(block + (warp * 2 + c) * 1024 + lane * 32);
-    to[0] = make_uint4(w[c][0][0], w[c][0][1], w[c][1][0], w[c][1][1]);
-    to[1] = make_uint4(w[c][2][0], w[c][2][1], w[c][3][0], w[c][3][1]);
+    *reinterpret_cast<uint4*>(block + warp * 2048 + (lane * 4 + j) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
   }
   if (warp == 0) reinterpret_cast<float4*>(block + kQ8CodeBytes)[lane] = make_float4(scale[0], scale[1], scale[2], scale[3]);
 }
 
-// A lane takes four features of eight tokens.
+// A lane takes four features of 16 tokens.
 template <int kType>
 __global__ void __launch_bounds__(256) unpack_q8_kernel(const UnpackParams p) {
   wait_for_launch_before();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tile = blockIdx.x / p.blocks, tb = blockIdx.x % p.blocks;
+  const int tiles = (p.rows + kCodeRows - 1) / kCodeRows, tile = blockIdx.x % tiles, tb = blockIdx.x / tiles;
   const uint8_t* block = p.packed + (static_cast<size_t>(tile) * p.blocks + tb) * kQ8BlockBytes;
-  const int f0 = tile * kCodeRows + lane * 4;
+  const int f0 = tile * kCodeRows + lane * 4, t0 = tb * kCodeSpan + warp * 16;
   const uint4 sc = ld_operand128(block + kQ8CodeBytes + lane * 16);
   const float s[4] = {__uint_as_float(sc.x), __uint_as_float(sc.y), __uint_as_float(sc.z), __uint_as_float(sc.w)};
-  uint4 in[2][2];
+  uint32_t w[4][4];
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    in[c][0] = ld_operand128(block + (warp * 2 + c) * 1024 + lane * 32);
-    in[c][1] = ld_operand128(block + (warp * 2 + c) * 1024 + lane * 32 + 16);
+  for (int j = 0; j < 4; ++j) {
+    const uint4 in = ld_operand128(block + warp * 2048 + (lane * 4 + j) * 16);
+    w[j][0] = in.x, w[j][1] = in.y, w[j][2] = in.z, w[j][3] = in.w;
   }
   let_next_launch_start();
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const uint32_t w[4][2] = {{in[c][0].x, in[c][0].y}, {in[c][0].z, in[c][0].w}, {in[c][1].x, in[c][1].y}, {in[c][1].z, in[c][1].w}};
+  for (int i = 0; i < 16; ++i) {
+    const int token = t0 + i;
+    if (token >= p.sum) continue;
+    float v[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int token = tb * kCodeSpan + (warp * 2 + c) * 8 + i;
-      if (token >= p.sum) continue;
-      float v[4];
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t code = w[j][i >> 2] >> ((i & 1) * 16 + (i & 2) * 4);
+      const float q = __uint_as_float(0x4b000000u | (code & 127u)) - 8388608.0f;  // 2^23 + the magnitude
+      v[j] = __fmaf_rn(s[j], code & 128u ? -q : q, 0.0f);  // no negative zeros
+    }
+    const long long at = f0 * p.row_step + token * p.sum_step;
+    if (p.vec && f0 + 4 <= p.rows) {
+      typename Element<kType>::type o[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t code = (w[j][i >> 2] >> ((i & 3) * 8)) & 255u;
-        const float q = static_cast<float>(code & 127u);
-        v[j] = s[j] * (code & 128u ? -q : q);
-      }
-      const long long at = f0 * p.row_step + token * p.sum_step;
-      if (p.vec && f0 + 4 <= p.rows) {
-        typename Element<kType>::type o[4];
+      for (int j = 0; j < 4; ++j) o[j] = Element<kType>::put(v[j]);
+      if constexpr (kType == kTypeF32) *reinterpret_cast<uint4*>(static_cast<float*>(p.out) + at) = *reinterpret_cast<const uint4*>(o);
+      else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = *reinterpret_cast<const uint2*>(o);
+    } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = Element<kType>::put(v[j]);
-        if constexpr (kType == kTypeF32) *reinterpret_cast<uint4*>(static_cast<float*>(p.out) + at) = *reinterpret_cast<const uint4*>(o);
-        else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = *reinterpret_cast<const uint2*>(o);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (f0 + j < p.rows) st_element<kType>(p.out, at + j * p.row_step, v[j]);
-      }
+      for (int j = 0; j < 4; ++j)
+        if (f0 + j < p.rows) st_element<kType>(p.out, at + j * p.row_step, v[j]);
     }
   }
 }

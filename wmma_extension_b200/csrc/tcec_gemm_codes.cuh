@@ -45,7 +45,18 @@ __device__ __forceinline__ void split3_bf16(float x, float y, uint32_t& hi, uint
   lo = __byte_perm(__float_as_uint(lx), __float_as_uint(ly), 0x7632);
 }
 
-// One CTA a block of 128 columns x 128 of the sum; an item is 16 bytes of a panel, eight consecutive values of one column.
+// Eight FP32 values to an item of each part; the small parts first, so that the accumulator, which truncates, cuts off less.
+template <class Put>
+__device__ __forceinline__ void put_split(const Put& put, int it, const float (&v)[8], bool none) {
+  uint32_t part[3][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) split3_bf16(none ? 0.f : v[2 * j], none ? 0.f : v[2 * j + 1], part[0][j], part[1][j], part[2][j]);
+#pragma unroll
+  for (int q = 0; q < 3; ++q) put(it, q, make_uint4(part[2 - q][0], part[2 - q][1], part[2 - q][2], part[2 - q][3]));
+}
+
+// One CTA a block of 128 columns x 128 of the sum; an item is 16 bytes of a panel, eight consecutive values of one column.  Addresses stay
+// among the elements that exist, so that all loads of some items go out before the first is waited for.
 template <int kType>
 __global__ void __launch_bounds__(256) stage_panels_kernel(const StagePanelsParams p) {
   constexpr int kParts = kType == kTypeF32 ? 3 : 1;
@@ -53,54 +64,68 @@ __global__ void __launch_bounds__(256) stage_panels_kernel(const StagePanelsPara
   const int kb = blockIdx.x % p.blocks, cb = blockIdx.x / p.blocks;
   uint8_t* out = p.panels + static_cast<size_t>(blockIdx.x) * kParts * kSpanBytes;
   const int cols = min(kCodeRows, (p.cols - cb * kCodeRows + 15) & ~15);  // columns that an MMA may read
-#pragma unroll 2
-  for (int it = 0; it < 8; ++it) {
-    const int item = threadIdx.x + it * 256;
-    int r, c, panel;
-    if (p.sum_step == 1) {  // a warp: 8 columns x 64 bytes
-      r = (item & 7) + ((item >> 5) & 15) * 8;
-      c = (item >> 3) & 3;
-      panel = item >> 9;
-    } else {                // a warp: 32 columns
-      r = item & 127;
-      c = (item >> 7) & 3;
-      panel = item >> 9;
-    }
-    if (r >= cols) continue;
-    const int col = cb * kCodeRows + r, i0 = kb * kCodeSpan + panel * 32 + c * 8;
-    const long long at = col * p.col_step + i0 * p.sum_step;
-    uint8_t* to = out + panel * kPanelBytes + (r >> 3) * 512 + c * 128 + (r & 7) * 16;
-    const bool whole = col < p.cols && i0 + 8 <= p.sum;
-    if constexpr (kType == kTypeF32) {
-      float v[8] = {};
-      if (whole && p.vec) {
-        const float4 a = ld_operand(reinterpret_cast<const float4*>(static_cast<const float*>(p.src) + at));
-        const float4 b = ld_operand(reinterpret_cast<const float4*>(static_cast<const float*>(p.src) + at + 4));
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-      } else {
+  const int first = threadIdx.x;
+  // Item `it` of a thread: column r, chunk c of panel it / 2.
+  const bool along = p.sum_step == 1;
+  const int r0 = along ? (first & 7) + ((first >> 5) & 7) * 8 : first & 127;   // a warp: 8 columns x 64 bytes, or 32 columns
+  const int c0 = along ? (first >> 3) & 3 : first >> 7;
+  auto column = [&](int it) { return along ? r0 + (it & 1) * 64 : r0; };
+  auto chunk = [&](int it) { return along ? c0 : c0 + (it & 1) * 2; };
+  auto put = [&](int it, int part, const uint4& v) {
+    const int r = column(it);
+    if (r < cols)
+      *reinterpret_cast<uint4*>(out + part * kSpanBytes + (it >> 1) * kPanelBytes + (r >> 3) * 512 + chunk(it) * 128 + (r & 7) * 16) = v;
+  };
+  constexpr int kAtOnce = kType == kTypeF32 ? 2 : 4;  // items whose loads are under way together
+  const int cols_here = p.cols - cb * kCodeRows, sum_here = p.sum - kb * kCodeSpan;
+  const long long origin = static_cast<long long>(cb) * kCodeRows * p.col_step + static_cast<long long>(kb) * kCodeSpan * p.sum_step;
+#pragma unroll 1
+  for (int it0 = 0; it0 < 8; it0 += kAtOnce) {
+    if (p.vec && sum_here >= kCodeSpan) {
+      uint4 raw[kAtOnce][kType == kTypeF32 ? 2 : 1];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (col < p.cols && i0 + j < p.sum) v[j] = ld_operand(static_cast<const float*>(p.src) + at + j * p.sum_step);
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int it = it0 + i;
+        const long long at = origin + min(column(it), cols_here - 1) * p.col_step + (it >> 1) * 32 + chunk(it) * 8;
+        if constexpr (kType == kTypeF32) {
+          raw[i][0] = ld_operand128(static_cast<const float*>(p.src) + at);
+          raw[i][1] = ld_operand128(static_cast<const float*>(p.src) + at + 4);
+        } else {
+          raw[i][0] = ld_operand128(static_cast<const uint16_t*>(p.src) + at);
+        }
       }
-      uint32_t part[3][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) split3_bf16(v[2 * j], v[2 * j + 1], part[0][j], part[1][j], part[2][j]);
-#pragma unroll
-      for (int q = 0; q < 3; ++q)  // the small parts first, so that the accumulator, which truncates, cuts off less
-        *reinterpret_cast<uint4*>(to + q * kSpanBytes) = make_uint4(part[2 - q][0], part[2 - q][1], part[2 - q][2], part[2 - q][3]);
+      for (int i = 0; i < kAtOnce; ++i) {
+        const bool none = column(it0 + i) >= cols_here;
+        if constexpr (kType == kTypeF32) {
+          const float v[8] = {__uint_as_float(raw[i][0].x), __uint_as_float(raw[i][0].y), __uint_as_float(raw[i][0].z), __uint_as_float(raw[i][0].w),
+                              __uint_as_float(raw[i][1].x), __uint_as_float(raw[i][1].y), __uint_as_float(raw[i][1].z), __uint_as_float(raw[i][1].w)};
+          put_split(put, it0 + i, v, none);
+        } else {
+          put(it0 + i, 0, none ? make_uint4(0, 0, 0, 0) : raw[i][0]);
+        }
+      }
     } else {
-      uint4 o = make_uint4(0, 0, 0, 0);
-      const uint16_t* src = static_cast<const uint16_t*>(p.src);
-      if (whole && p.vec) {
-        o = ld_operand128(src + at);
-      } else {
-        uint32_t w[8] = {};
+      typename std::conditional<kType == kTypeF32, float, uint32_t>::type w[kAtOnce][8];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int it = it0 + i, at_sum = (it >> 1) * 32 + chunk(it) * 8 + j;
+          const long long at = origin + min(column(it), cols_here - 1) * p.col_step + min(at_sum, sum_here - 1) * p.sum_step;
+          if constexpr (kType == kTypeF32) w[i][j] = ld_operand(static_cast<const float*>(p.src) + at);
+          else w[i][j] = ld_operand16(static_cast<const uint16_t*>(p.src) + at);
+        }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int it = it0 + i, at_sum = (it >> 1) * 32 + chunk(it) * 8;
+        const bool none = column(it) >= cols_here;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (col < p.cols && i0 + j < p.sum) w[j] = ld_operand16(src + at + j * p.sum_step);
-        o = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+          if (none || at_sum + j >= sum_here) w[i][j] = 0;
+        if constexpr (kType == kTypeF32) put_split(put, it, w[i], false);
+        else put(it, 0, make_uint4(w[i][0] | w[i][1] << 16, w[i][2] | w[i][3] << 16, w[i][4] | w[i][5] << 16, w[i][6] | w[i][7] << 16));
       }
-      *reinterpret_cast<uint4*>(to) = o;
     }
   }
   let_next_launch_start();
@@ -126,17 +151,13 @@ __device__ __forceinline__ uint4 q4_expand(uint32_t w, uint32_t zero) {
   return make_uint4(sub16x2((w & kMask) | kMagic, zero, kF16), sub16x2(((w >> 4) & kMask) | kMagic, zero, kF16),
                     sub16x2(((w >> 8) & kMask) | kMagic, zero, kF16), sub16x2(((w >> 12) & kMask) | kMagic, zero, kF16));
 }
-// Two codes of 8 bits (sign and magnitude) in bits 0-7 and 16-23: +-(magic + magnitude) -+ magic.
+// Eight 8-bit codes (sign and magnitude) in the bytes 0 2, 1 3 of two words, to operands in order: +-(magic + magnitude) -+ magic.
 template <bool kF16>
-__device__ __forceinline__ uint32_t q8_expand2(uint32_t x) {
-  constexpr uint32_t kMagic = kF16 ? 0x64006400u : 0x43004300u;
-  const uint32_t base = ((x << 8) & 0x80008000u) | kMagic;
-  return sub16x2(base | (x & 0x007f007fu), base, kF16);
-}
-template <bool kF16>
-__device__ __forceinline__ uint4 q8_expand(uint2 w) {
-  return make_uint4(q8_expand2<kF16>(__byte_perm(w.x, 0, 0x4140)), q8_expand2<kF16>(__byte_perm(w.x, 0, 0x4342)),
-                    q8_expand2<kF16>(__byte_perm(w.y, 0, 0x4140)), q8_expand2<kF16>(__byte_perm(w.y, 0, 0x4342)));
+__device__ __forceinline__ uint4 q8_expand(uint32_t w0, uint32_t w1) {
+  constexpr uint32_t kMagic = kF16 ? 0x64006400u : 0x43004300u, kSign = 0x80008000u, kSize = 0x007f007fu;
+  const uint32_t a = ((w0 << 8) & kSign) | kMagic, b = (w0 & kSign) | kMagic, c = ((w1 << 8) & kSign) | kMagic, d = (w1 & kSign) | kMagic;
+  return make_uint4(sub16x2((w0 & kSize) | a, a, kF16), sub16x2(((w0 >> 8) & kSize) | b, b, kF16), sub16x2((w1 & kSize) | c, c, kF16),
+                    sub16x2(((w1 >> 8) & kSize) | d, d, kF16));
 }
 
 // ---------------------------------------------------------------- the product
@@ -181,6 +202,7 @@ struct GemmCodesCfg {
   static_assert(PAIR || B_STAGES * B_BYTES >= 128 * BN * 4, "partial results go where the dense operand was");
   static constexpr int TMEM_COLS = 2 * BN;
   static constexpr int NC = BN / 2;                           // columns of an epilogue thread
+  static constexpr int LOAD_COLS = PAIR ? 16 : 32;            // of them at a time, twice
   // 512 threads x 128 registers at launch: 128 x (40 + 56) + 2 x 128 x 208 = 65536
   static constexpr bool REBALANCE = PAIR;
 };
@@ -192,6 +214,8 @@ __device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float
       : "+f"(x), "+f"(y)
       : "f"(a), "f"(b), "f"(s));
 }
+__device__ __forceinline__ void tmem_ld_32x32b(uint32_t taddr, uint32_t (&v)[32]) { tmem_ld_32x32b_x32(taddr, v); }
+__device__ __forceinline__ void tmem_ld_32x32b(uint32_t taddr, uint32_t (&v)[16]) { tmem_ld_32x32b_x16(taddr, v); }
 // All lanes poll, which they notice sooner than one lane that tells the others.
 __device__ __forceinline__ bool mbar_wait_lanes(uint32_t bar, uint32_t parity, volatile uint32_t* abortp) {
   const bool ok = mbar_wait(bar, parity, abortp, 0);
@@ -229,14 +253,15 @@ struct Converter {  // 4 bits: two strips of 16 rows a warp, lane 4 g + t has ro
 template <bool kF16>
 struct Converter<kF16, 0> {  // 8 bits: a lane a row
   static __device__ __forceinline__ void expand(const uint8_t* block, uint8_t* out, int warp, int lane) {
-    const int row = warp * 32 + lane;
+    constexpr int kChunk = GemmCodesCfg<128, 0>::CHUNK_BYTES;
+    const int at = (warp * 32 + lane) * 16;  // of this row, among 16 tokens of codes and among 8 of operands
 #pragma unroll
-    for (int c = 0; c < 16; c += 4) {
-      uint2 w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint2*>(block + (c + i) * 1024 + row * 8);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(out + (c + i) * GemmCodesCfg<128, 0>::CHUNK_BYTES + row * 16) = q8_expand<kF16>(w[i]);
+    for (int c = 0; c < 8; c += 2) {
+      const uint4 v = *reinterpret_cast<const uint4*>(block + c * 2048 + at), w = *reinterpret_cast<const uint4*>(block + (c + 1) * 2048 + at);
+      *reinterpret_cast<uint4*>(out + (2 * c) * kChunk + at) = q8_expand<kF16>(v.x, v.y);
+      *reinterpret_cast<uint4*>(out + (2 * c + 1) * kChunk + at) = q8_expand<kF16>(v.z, v.w);
+      *reinterpret_cast<uint4*>(out + (2 * c + 2) * kChunk + at) = q8_expand<kF16>(w.x, w.y);
+      *reinterpret_cast<uint4*>(out + (2 * c + 3) * kChunk + at) = q8_expand<kF16>(w.z, w.w);
     }
   }
 };
@@ -531,33 +556,27 @@ __global__ void __launch_bounds__(512, 1) tcec_gemm_codes_kernel(const GemmCodes
               break;
             }
             tc_fence_after();
-            if (cols > 0) {
-              const float s = scales[(slot * kGroups + g) * 128];
-              const uint32_t from = taddr + (fold & 1) * BN;
-              if constexpr (Cfg::NC == 32) {
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(from, v);
-                tmem_ld_wait();
+            const float s = scales[(slot * kGroups + g) * 128];
+            const uint32_t from = taddr + (fold & 1) * BN;
+            constexpr int kAtOnce = Cfg::LOAD_COLS;
+            uint32_t v[2][kAtOnce];
+            tmem_ld_32x32b(from, v[0]);
 #pragma unroll
-                for (int j = 0; j < 32; j += 2) fma2(acc[j], acc[j + 1], __uint_as_float(v[j]), __uint_as_float(v[j + 1]), s);
-              } else {
-                uint32_t v[2][32];
-                tmem_ld_32x32b_x32(from, v[0]);
-#pragma unroll
-                for (int i = 0; i < Cfg::NC; i += 32) {
-                  tmem_ld_wait();
-                  if (i + 32 < Cfg::NC) tmem_ld_32x32b_x32(from + i + 32, v[(i / 32 + 1) & 1]);
-#pragma unroll
-                  for (int j = 0; j < 32; j += 2)
-                    fma2(acc[i + j], acc[i + j + 1], __uint_as_float(v[(i / 32) & 1][j]), __uint_as_float(v[(i / 32) & 1][j + 1]), s);
+            for (int i = 0; i < Cfg::NC; i += kAtOnce) {
+              tmem_ld_wait();
+              if (i + kAtOnce < Cfg::NC) {
+                tmem_ld_32x32b(from + i + kAtOnce, v[(i / kAtOnce + 1) & 1]);
+              } else {  // all of it is in registers: the next products may go there
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                  if constexpr (kPair) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_acc_free[fold & 1]), 0));
+                  else mbar_arrive(smem_u32(&bar_acc_free[fold & 1]));
                 }
               }
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if constexpr (kPair) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_acc_free[fold & 1]), 0));
-              else mbar_arrive(smem_u32(&bar_acc_free[fold & 1]));
+#pragma unroll
+              for (int j = 0; j < kAtOnce; j += 2)
+                fma2(acc[i + j], acc[i + j + 1], __uint_as_float(v[(i / kAtOnce) & 1][j]), __uint_as_float(v[(i / kAtOnce) & 1][j + 1]), s);
             }
           }
         }

@@ -20,7 +20,7 @@ struct GemvQ4Params {
   const void* x;              // element (token, i) at token * x_token + i * x_k
   long long x_token, x_k;
   int n, k, tokens, blocks;
-  int vec;                    // x_k 1 and aligned for 16 bytes
+  int vec;                    // x_k 1 and four values at a time aligned
   float alpha, beta;
   void* c;                    // element (token, row) at token * c_token + row * c_row
   long long c_token, c_row;
@@ -39,63 +39,143 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Eight consecutive values of a column's token from k0 on, as 16-bit operands.
-template <int kType>
-__device__ __forceinline__ uint4 load_column8(const GemvQ4Params& p, int col, int k0) {
-  constexpr int kParts = kType == kTypeF32 ? 3 : 1;
-  const int token = col / kParts;
-  uint4 o = make_uint4(0, 0, 0, 0);
-  if (token >= p.tokens) return o;
-  const long long at = token * p.x_token + k0 * p.x_k;
-  if constexpr (kType == kTypeF32) {
-    const int part = col - token * kParts;
-    float v[8] = {};
-    if (p.vec && k0 + 8 <= p.k) {
-      const float4 a = ld_operand(reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + at));
-      const float4 b = ld_operand(reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + at + 4));
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+// A warp's x of one block in shared memory: columns of 128 values in 16 bits, 320 bytes apart, so that lanes of two columns and four
+// times 16 bytes read from all banks at once.
+constexpr int kXPitch = 320;
+
+template <int kType, int kGroup, int kCols, int kStrips>
+struct GemvQ4Cfg {
+  static constexpr int PARTS = kType == kTypeF32 ? 3 : 1;
+  static constexpr int WIDTH = kCols * 8;                     // columns
+  static constexpr int TOKENS = WIDTH / PARTS;
+  static constexpr int ROWS = 16 * kStrips;
+  static constexpr int WARPS = 8;
+  static constexpr int AHEAD = kCols == 1 ? 2 : 1;            // blocks loaded ahead of the one at work
+  static constexpr int X_BYTES = WIDTH * kXPitch;             // of a warp
+  static constexpr int SUM_PITCH = WIDTH + 1;
+  static constexpr int SUM_BYTES = WARPS * ROWS * SUM_PITCH * 4;
+  static constexpr int SMEM_BYTES = WARPS * X_BYTES > SUM_BYTES ? WARPS * X_BYTES : SUM_BYTES;
+};
+
+// What a lane holds of one block: codes and entries of its rows, and four values of every token.
+template <int kType, int kGroup, int kCols, int kStrips>
+struct GemvQ4Block {
+  using Cfg = GemvQ4Cfg<kType, kGroup, kCols, kStrips>;
+  static constexpr int kSpans = kCodeSpan / kGroup;
+  uint4 w[kStrips][2];
+  uint32_t entry[kStrips][kSpans][2];
+  Four<kType> x[Cfg::TOKENS];
+
+  __device__ __forceinline__ void load(const GemvQ4Params& p, const uint8_t* block, int kb, int in_tile, int lane) {
+    const uint8_t* strip = block + in_tile * 64 + lane * 16;
+    const uint8_t* e = block + kQ4CodeBytes + (in_tile + (lane >> 2)) * 4;
+#pragma unroll
+    for (int s = 0; s < kStrips; ++s) {
+      w[s][0] = ld_once128(strip + s * 1024);
+      w[s][1] = ld_once128(strip + s * 1024 + 512);
+#pragma unroll
+      for (int q = 0; q < kSpans; ++q) {
+        entry[s][q][0] = ld_operand32(e + q * kEntryBytes + s * 64);
+        entry[s][q][1] = ld_operand32(e + q * kEntryBytes + s * 64 + 32);
+      }
+    }
+    const int k0 = kb * kCodeSpan + lane * 4, left = p.k - k0;
+    if (p.vec && (kb + 1) * kCodeSpan <= p.k) {
+#pragma unroll
+      for (int i = 0; i < Cfg::TOKENS; ++i)
+        if (i < p.tokens) x[i].load(p.x, i * p.x_token + k0);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (k0 + j < p.k) v[j] = ld_operand(static_cast<const float*>(p.x) + at + j * p.x_k);
-    }
-    uint32_t w[4];
+      for (int i = 0; i < Cfg::TOKENS; ++i)
+        if (i < p.tokens) {
+          uint32_t v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t hi, mid, lo;
-      split3_bf16(v[2 * j], v[2 * j + 1], hi, mid, lo);
-      w[j] = part == 0 ? hi : part == 1 ? mid : lo;
-    }
-    o = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
-    const uint16_t* x = static_cast<const uint16_t*>(p.x);
-    if (p.vec && k0 + 8 <= p.k) {
-      o = ld_operand128(x + at);
-    } else {
-      uint32_t w[8] = {};
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (k0 + j < p.k) w[j] = ld_operand16(x + at + j * p.x_k);
-      o = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+          for (int j = 0; j < 4; ++j) {
+            const long long at = i * p.x_token + min(k0 + j, p.k - 1) * p.x_k;
+            if constexpr (kType == kTypeF32) v[j] = ld_operand32(static_cast<const uint32_t*>(p.x) + at);
+            else v[j] = ld_operand16(static_cast<const uint16_t*>(p.x) + at);
+            if (j >= left) v[j] = 0;
+          }
+          if constexpr (kType == kTypeF32) x[i].raw = make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
+          else x[i].raw = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+        }
     }
   }
-  return o;
-}
+  // x in its columns, for the lanes that need it as operand.
+  __device__ __forceinline__ void share_x(const GemvQ4Params& p, uint8_t* mine, int lane) const {
+#pragma unroll
+    for (int i = 0; i < Cfg::TOKENS; ++i)
+      if (i < p.tokens) {
+        uint8_t* to = mine + i * Cfg::PARTS * kXPitch + lane * 8;
+        if constexpr (kType == kTypeF32) {
+          uint2 hi, mid, lo;
+          split3_bf16(x[i].raw.x, x[i].raw.y, hi.x, mid.x, lo.x);
+          split3_bf16(x[i].raw.z, x[i].raw.w, hi.y, mid.y, lo.y);
+          *reinterpret_cast<uint2*>(to) = hi;
+          *reinterpret_cast<uint2*>(to + kXPitch) = mid;
+          *reinterpret_cast<uint2*>(to + 2 * kXPitch) = lo;
+        } else {
+          *reinterpret_cast<uint2*>(to) = x[i].raw;
+        }
+      }
+  }
+  __device__ __forceinline__ void multiply(float (&acc)[kStrips][kCols][4], const uint8_t* mine, int lane) const {
+    constexpr bool kF16 = kType == kTypeF16;
+#pragma unroll
+    for (int q = 0; q < kSpans; ++q) {
+      float d[kStrips][kCols][4];
+#pragma unroll
+      for (int s = 0; s < kStrips; ++s)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) d[s][c][0] = d[s][c][1] = d[s][c][2] = d[s][c][3] = 0.f;
+#pragma unroll
+      for (int panel = q * 4 / kSpans; panel < (q + 1) * 4 / kSpans; ++panel) {
+        uint4 b[kCols];
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+          b[c] = *reinterpret_cast<const uint4*>(mine + (c * 8 + (lane >> 2)) * kXPitch + panel * 64 + (lane & 3) * 16);
+#pragma unroll
+        for (int s = 0; s < kStrips; ++s) {
+          const uint4 pair = w[s][panel >> 1];
+          const uint4 r0 = q4_expand<kF16>(panel & 1 ? pair.z : pair.x, q4_zero<kF16>(entry[s][q][0] & 15u));
+          const uint4 r1 = q4_expand<kF16>(panel & 1 ? pair.w : pair.y, q4_zero<kF16>(entry[s][q][1] & 15u));
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) {
+            mma16816<kF16>(d[s][c], r0.x, r1.x, r0.y, r1.y, b[c].x, b[c].y);
+            mma16816<kF16>(d[s][c], r0.z, r1.z, r0.w, r1.w, b[c].z, b[c].w);
+          }
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < kStrips; ++s) {
+        const float s0 = __uint_as_float(entry[s][q][0] & ~15u), s1 = __uint_as_float(entry[s][q][1] & ~15u);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          acc[s][c][0] = __fmaf_rn(s0, d[s][c][0], acc[s][c][0]);
+          acc[s][c][1] = __fmaf_rn(s0, d[s][c][1], acc[s][c][1]);
+          acc[s][c][2] = __fmaf_rn(s1, d[s][c][2], acc[s][c][2]);
+          acc[s][c][3] = __fmaf_rn(s1, d[s][c][3], acc[s][c][3]);
+        }
+      }
+    }
+  }
+};
 
 // kCols: columns in eights.
 template <int kType, int kGroup, int kCols, int kStrips>
 __global__ void __launch_bounds__(256) gemv_q4_kernel(const GemvQ4Params p) {
-  constexpr bool kF16 = kType == kTypeF16;
-  constexpr int kParts = kType == kTypeF32 ? 3 : 1, kSpans = kCodeSpan / kGroup, kWarps = 8;
-  constexpr int kRows = 16 * kStrips, kWidth = kCols * 8;
-  __shared__ float sums[kWarps][kRows][kWidth + 1];
+  using Cfg = GemvQ4Cfg<kType, kGroup, kCols, kStrips>;
+  using Block = GemvQ4Block<kType, kGroup, kCols, kStrips>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* mine = smem + warp * Cfg::X_BYTES;
+  for (int i = lane; i < Cfg::X_BYTES / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);  // columns that nobody has
+  const int row0 = blockIdx.x * Cfg::ROWS, in_tile = row0 % kCodeRows;
+  constexpr size_t kBlockBytes = q4_block_bytes(kGroup);
+  const uint8_t* base = p.codes + static_cast<size_t>(row0 / kCodeRows) * p.blocks * kBlockBytes;
+  __syncwarp();
   wait_for_launch_before();
   let_next_launch_start();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int row0 = blockIdx.x * kRows;
-  const size_t block_bytes = q4_block_bytes(kGroup);
-  const uint8_t* base = p.codes + static_cast<size_t>(row0 / kCodeRows) * p.blocks * block_bytes;
-  const int in_tile = row0 % kCodeRows;
 
   float acc[kStrips][kCols][4];
 #pragma unroll
@@ -103,71 +183,42 @@ __global__ void __launch_bounds__(256) gemv_q4_kernel(const GemvQ4Params p) {
 #pragma unroll
     for (int c = 0; c < kCols; ++c) acc[s][c][0] = acc[s][c][1] = acc[s][c][2] = acc[s][c][3] = 0.f;
 
-  for (int kb = warp; kb < p.blocks; kb += kWarps) {
-    const uint8_t* block = base + kb * block_bytes;
-    uint4 w[kStrips][2];
-    uint32_t entries[kStrips][kSpans][2];
+  constexpr int kHeld = Cfg::AHEAD + 1;
+  Block held[kHeld];
 #pragma unroll
-    for (int s = 0; s < kStrips; ++s) {
-      const uint8_t* strip = block + (in_tile / 16 + s) * 1024 + lane * 16;
-      w[s][0] = ld_once128(strip);
-      w[s][1] = ld_once128(strip + 512);
+  for (int i = 0; i < Cfg::AHEAD; ++i)
+    if (warp + i * Cfg::WARPS < p.blocks) held[i].load(p, base + (warp + i * Cfg::WARPS) * kBlockBytes, warp + i * Cfg::WARPS, in_tile, lane);
+  for (int kb = warp; kb < p.blocks; kb += kHeld * Cfg::WARPS) {
 #pragma unroll
-      for (int q = 0; q < kSpans; ++q) {
-        const uint8_t* e = block + kQ4CodeBytes + q * kEntryBytes + (in_tile + s * 16 + g) * 4;
-        entries[s][q][0] = ld_operand32(e);
-        entries[s][q][1] = ld_operand32(e + 32);
-      }
+    for (int i = 0; i < kHeld; ++i) {
+      const int now = kb + i * Cfg::WARPS, next = now + Cfg::AHEAD * Cfg::WARPS;
+      if (now >= p.blocks) break;
+      if (next < p.blocks) held[(i + Cfg::AHEAD) % kHeld].load(p, base + next * kBlockBytes, next, in_tile, lane);
+      held[i].share_x(p, mine, lane);
+      __syncwarp();
+      held[i].multiply(acc, mine, lane);
+      __syncwarp();
     }
-    uint4 x[kCols][4];
-#pragma unroll
-    for (int c = 0; c < kCols; ++c)
-#pragma unroll
-      for (int panel = 0; panel < 4; ++panel) x[c][panel] = load_column8<kType>(p, c * 8 + g, kb * kCodeSpan + panel * 32 + t * 8);
-#pragma unroll
-    for (int s = 0; s < kStrips; ++s)
-#pragma unroll
-      for (int q = 0; q < kSpans; ++q) {
-        const uint32_t zero0 = q4_zero<kF16>(entries[s][q][0] & 15u), zero1 = q4_zero<kF16>(entries[s][q][1] & 15u);
-        const float s0 = __uint_as_float(entries[s][q][0] & ~15u), s1 = __uint_as_float(entries[s][q][1] & ~15u);
-        float d[kCols][4];
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) d[c][0] = d[c][1] = d[c][2] = d[c][3] = 0.f;
-#pragma unroll
-        for (int panel = q * 4 / kSpans; panel < (q + 1) * 4 / kSpans; ++panel) {
-          const uint4 pair = w[s][panel >> 1];
-          const uint4 a = q4_expand<kF16>(panel & 1 ? pair.z : pair.x, zero0), b = q4_expand<kF16>(panel & 1 ? pair.w : pair.y, zero1);
-#pragma unroll
-          for (int c = 0; c < kCols; ++c) {
-            mma16816<kF16>(d[c], a.x, b.x, a.y, b.y, x[c][panel].x, x[c][panel].y);
-            mma16816<kF16>(d[c], a.z, b.z, a.w, b.w, x[c][panel].z, x[c][panel].w);
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          acc[s][c][0] = __fmaf_rn(s0, d[c][0], acc[s][c][0]);
-          acc[s][c][1] = __fmaf_rn(s0, d[c][1], acc[s][c][1]);
-          acc[s][c][2] = __fmaf_rn(s1, d[c][2], acc[s][c][2]);
-          acc[s][c][3] = __fmaf_rn(s1, d[c][3], acc[s][c][3]);
-        }
-      }
   }
 
+  __syncthreads();  // x is read, sums take its place
+  float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int s = 0; s < kStrips; ++s)
 #pragma unroll
     for (int c = 0; c < kCols; ++c)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sums[warp][s * 16 + g + (j >> 1) * 8][c * 8 + t * 2 + (j & 1)] = acc[s][c][j];
+      for (int j = 0; j < 4; ++j)
+        sums[(warp * Cfg::ROWS + s * 16 + (lane >> 2) + (j >> 1) * 8) * Cfg::SUM_PITCH + c * 8 + (lane & 3) * 2 + (j & 1)] = acc[s][c][j];
   __syncthreads();
-  for (int i = threadIdx.x; i < kRows * p.tokens; i += 256) {
-    const int r = i % kRows, token = i / kRows, row = row0 + r;
+  for (int i = threadIdx.x; i < Cfg::ROWS * p.tokens; i += 256) {
+    const int r = i % Cfg::ROWS, token = i / Cfg::ROWS, row = row0 + r;
     if (row >= p.n) continue;
     float v = 0.f;
 #pragma unroll
-    for (int part = kParts - 1; part >= 0; --part)  // the small ones first
+    for (int part = Cfg::PARTS - 1; part >= 0; --part)  // the small ones first
 #pragma unroll
-      for (int wq = 0; wq < kWarps; ++wq) v += sums[wq][r][token * kParts + part];
+      for (int w = 0; w < Cfg::WARPS; ++w) v += sums[(w * Cfg::ROWS + r) * Cfg::SUM_PITCH + token * Cfg::PARTS + part];
     const long long at = token * p.c_token + row * p.c_row;
     v = __fmul_rn(p.alpha, v);
     if (p.beta != 0.f) v = __fmaf_rn(p.beta, ld_element_as(p.c_type, p.c, at), v);
