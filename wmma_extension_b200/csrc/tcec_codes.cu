@@ -6,10 +6,10 @@
 #include <mutex>
 
 #include "tcec_codes.cuh"
-#include "tcec_gemm_codes.cuh"
-#include "tcec_gemv_q4.cuh"
+#include "tcec_codes_launch.h"
 #include "tcec_internal.h"
 #include "tcec_launch.h"
+#include "tcec_stage.cuh"
 
 using namespace tcec_sm100;
 
@@ -60,34 +60,6 @@ size_t panel_bytes(int cols, int sum, int type) {
   return static_cast<size_t>(ceil_div(cols, kCodeRows)) * ceil_div(sum, kCodeSpan) * (type == TCEC_TYPE_F32 ? 3 : 1) * kSpanBytes;
 }
 
-template <int BN, bool F, int S>
-cudaError_t set_codes_attr() {
-  const cudaError_t e = cudaFuncSetAttribute(tcec_gemm_codes_kernel<BN, F, S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             GemmCodesCfg<BN, S>::SMEM_BYTES);
-  if (e != cudaSuccess || !GemmCodesCfg<BN, S>::REBALANCE) return e;
-  cudaFuncAttributes a{};  // the split of the registers among the warps is made for a launch with 128 a thread
-  const cudaError_t got = cudaFuncGetAttributes(&a, tcec_gemm_codes_kernel<BN, F, S>);
-  return got != cudaSuccess ? got : a.numRegs == 128 ? cudaSuccess : cudaErrorInvalidConfiguration;
-}
-template <bool F, int S>
-cudaError_t set_codes_attrs() {
-  cudaError_t e = set_codes_attr<64, F, S>();
-  if (e == cudaSuccess) e = set_codes_attr<128, F, S>();
-  if (e == cudaSuccess) e = set_codes_attr<256, F, S>();
-  return e;
-}
-template <bool F>
-cudaError_t set_all_codes_attrs() {
-  cudaError_t e = set_codes_attrs<F, 0>();
-  if (e == cudaSuccess) e = set_codes_attrs<F, 1>();
-  if (e == cudaSuccess) e = set_codes_attrs<F, 2>();
-  if (e == cudaSuccess) e = set_codes_attrs<F, 4>();
-  return e;
-}
-
-template <int T>
-cudaError_t set_gemv_attrs();
-
 // What a launch needs to know of the current device.
 struct Here {
   int* status;
@@ -99,11 +71,8 @@ int get_here(Here* out) {
   const int rc = get_device_state(&st);
   if (rc != TCEC_OK) return rc;
   if (!st->codes_attrs_done) {
-    TCEC_CUDA(set_all_codes_attrs<false>());
-    TCEC_CUDA(set_all_codes_attrs<true>());
-    TCEC_CUDA(set_gemv_attrs<kTypeF32>());
-    TCEC_CUDA(set_gemv_attrs<kTypeF16>());
-    TCEC_CUDA(set_gemv_attrs<kTypeBf16>());
+    TCEC_CUDA(set_gemm_codes_attrs());
+    TCEC_CUDA(set_gemv_q4_attrs());
     st->codes_attrs_done = true;
   }
   *out = {st->status, st->sm_count};
@@ -153,59 +122,13 @@ struct UnpackQ8 {
   static void go(int grid, cudaStream_t stream, const UnpackParams& p) { launch_early(unpack_q8_kernel<T>, grid, 256, 0, stream, p); }
 };
 template <int T>
+struct StageColumns {
+  static void go(dim3 grid, cudaStream_t stream, const StageColumnsParams& p) { launch_early(stage_columns_kernel<T>, grid, 128, 0, stream, p); }
+};
+template <int T>
 struct StagePanels {
   static void go(int grid, cudaStream_t stream, const StagePanelsParams& p) { launch_early(stage_panels_kernel<T>, grid, 256, 0, stream, p); }
 };
-template <int T, int G, int C, int S>
-void launch_gemv(cudaStream_t stream, const GemvQ4Params& p) {
-  using Cfg = GemvQ4Cfg<T, G, C, S>;
-  launch_early(gemv_q4_kernel<T, G, C, S>, static_cast<int>(ceil_div(p.n, Cfg::ROWS)), 32 * Cfg::WARPS, Cfg::SMEM_BYTES, stream, p);
-}
-template <int T>
-struct GemvQ4 {
-  template <int G>
-  static void of_group(int columns, cudaStream_t stream, const GemvQ4Params& p) {
-    if (columns <= 8 && p.n <= 8192) launch_gemv<T, G, 1, 1>(stream, p);
-    else if (columns <= 8) launch_gemv<T, G, 1, 2>(stream, p);
-    else if (columns <= 16) launch_gemv<T, G, 2, 2>(stream, p);
-    else launch_gemv<T, G, 4, 2>(stream, p);
-  }
-  static void go(int group, int columns, cudaStream_t stream, const GemvQ4Params& p) {
-    if (group == 32) of_group<32>(columns, stream, p);
-    else if (group == 64) of_group<64>(columns, stream, p);
-    else of_group<128>(columns, stream, p);
-  }
-};
-template <int T, int G, int C, int S>
-cudaError_t set_gemv_attr() {
-  return cudaFuncSetAttribute(gemv_q4_kernel<T, G, C, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, GemvQ4Cfg<T, G, C, S>::SMEM_BYTES);
-}
-template <int T>
-cudaError_t set_gemv_attrs() {  // the others stay below what needs no permission
-  cudaError_t e = set_gemv_attr<T, 32, 4, 2>();
-  if (e == cudaSuccess) e = set_gemv_attr<T, 64, 4, 2>();
-  if (e == cudaSuccess) e = set_gemv_attr<T, 128, 4, 2>();
-  return e;
-}
-
-template <int BN, bool F, int S>
-void launch_codes_as(const GemmCodesParams& gp, int shares, int grid, cudaStream_t stream) {
-  launch_clusters(tcec_gemm_codes_kernel<BN, F, S>, shares, grid, 512, GemmCodesCfg<BN, S>::SMEM_BYTES, stream, gp);
-}
-template <bool F, int S>
-void launch_codes_of(int bn, const GemmCodesParams& gp, int shares, int grid, cudaStream_t stream) {
-  if (bn == 64) launch_codes_as<64, F, S>(gp, shares, grid, stream);
-  else if (bn == 128) launch_codes_as<128, F, S>(gp, shares, grid, stream);
-  else launch_codes_as<256, F, S>(gp, shares, grid, stream);
-}
-template <bool F>
-void launch_codes(int spans, int bn, const GemmCodesParams& gp, int shares, int grid, cudaStream_t stream) {
-  if (spans == 0) launch_codes_of<F, 0>(bn, gp, shares, grid, stream);
-  else if (spans == 1) launch_codes_of<F, 1>(bn, gp, shares, grid, stream);
-  else if (spans == 2) launch_codes_of<F, 2>(bn, gp, shares, grid, stream);
-  else launch_codes_of<F, 4>(bn, gp, shares, grid, stream);
-}
-
 // D[row][col] of tcec_gemm_codes.cuh for an operand of codes (spans: groups of 4-bit codes in a block, 0: 8-bit codes) and a dense one whose columns and sum lie at the given steps.
 int gemm_codes(const void* codes, int spans, int rows, int cols, int sum, const void* dense, long long col_step, long long sum_step,
                int type, bool vec, float alpha, float beta, void* c, long long c_row, long long c_col, int c_type, void* workspace,
@@ -248,8 +171,7 @@ int gemm_codes(const void* codes, int spans, int rows, int cols, int sum, const 
   // One cluster a tile where the sum is divided; else as many as run at a time.
   const long long most = bn == 256 ? here.sm_count / 2 : ctas > 1 ? tiles : here.sm_count;
   const int grid = static_cast<int>(tiles < most ? tiles : most) * ctas;
-  if (type == TCEC_TYPE_F16) launch_codes<true>(spans, bn, gp, ctas, grid, stream);
-  else launch_codes<false>(spans, bn, gp, ctas, grid, stream);
+  launch_gemm_codes(type == TCEC_TYPE_F16, spans, bn, gp, ctas, grid, stream);
   return launched();
 }
 
@@ -257,6 +179,7 @@ int gemm_codes(const void* codes, int spans, int rows, int cols, int sum, const 
 // registers (tcec_gemv_q4.cuh).
 long long columns_of(int m, int type) { return static_cast<long long>(m) * (type == TCEC_TYPE_F32 ? 3 : 1); }
 bool streamed(int m, int type) { return columns_of(m, type) <= 32; }
+int eights_of(int m, int type) { return columns_of(m, type) <= 8 ? 1 : columns_of(m, type) <= 16 ? 2 : 4; }
 
 }  // namespace
 }  // namespace tcec_host
@@ -355,7 +278,9 @@ int tcec_unpack_q4(int layout_w, int n, int k, const void* packed, int group, vo
 }
 
 size_t tcec_gemm_q4_workspace_bytes(int m, int n, int k, int type_x) {
-  return m < 0 || n < 0 || k < 0 || bad_type(type_x) || streamed(m, type_x) ? 0 : panel_bytes(m, k, type_x);
+  if (m < 0 || n < 0 || k < 0 || bad_type(type_x) || m <= 1) return 0;
+  if (streamed(m, type_x)) return static_cast<size_t>(ceil_div(k, kCodeSpan)) * eights_of(m, type_x) * 2048;
+  return panel_bytes(m, k, type_x);
 }
 
 int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, const void* x, long long ldx, int type_x, const void* packed,
@@ -382,15 +307,29 @@ int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, c
     if (!streamed(m, type_x))
       return gemm_codes(packed, kCodeSpan / group, n, m, sum, x, dx.row_step(), dx.col_step(), type_x, layout_x == TCEC_ROW_MAJOR && dx.wide(16), alpha,
                         beta, c, dc.col_step(), dc.row_step(), type_c, workspace, here, static_cast<cudaStream_t>(stream));
+    const cudaStream_t on = static_cast<cudaStream_t>(stream);
+    const int blocks = static_cast<int>(ceil_div(sum, kCodeSpan)), eights = eights_of(m, type_x);
+    if (m > 1 && blocks) {
+      StageColumnsParams sp{};
+      sp.src = x;
+      sp.col_step = dx.row_step();
+      sp.sum_step = dx.col_step();
+      sp.tokens = m;
+      sp.sum = sum;
+      sp.eights = eights;
+      sp.out = static_cast<uint8_t*>(workspace);
+      sp.vec = layout_x == TCEC_ROW_MAJOR && dx.wide(16);
+      by_type<StageColumns>(type_x, dim3(blocks, eights), on, sp);
+    }
     GemvQ4Params p{};
     p.codes = static_cast<const uint8_t*>(packed);
+    p.staged = m > 1 && blocks ? static_cast<const uint8_t*>(workspace) : nullptr;
     p.x = x;
-    p.x_token = dx.row_step();
     p.x_k = dx.col_step();
     p.n = n;
     p.k = sum;
     p.tokens = m;
-    p.blocks = static_cast<int>(ceil_div(sum, kCodeSpan));
+    p.blocks = blocks;
     p.vec = layout_x == TCEC_ROW_MAJOR && dx.wide(4 * type_bytes(type_x));
     p.alpha = alpha;
     p.beta = beta;
@@ -398,7 +337,9 @@ int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, c
     p.c_token = dc.row_step();
     p.c_row = dc.col_step();
     p.c_type = type_c;
-    by_type<GemvQ4>(type_x, group, static_cast<int>(columns_of(m, type_x)), static_cast<cudaStream_t>(stream), p);
+    p.status = here.status;
+    if (m > 1 && !blocks) return gemm_codes(packed, kCodeSpan / group, n, m, 0, x, 0, 0, type_x, false, alpha, beta, c, dc.col_step(), dc.row_step(), type_c, workspace, here, on);
+    launch_gemv_q4(type_x, group, eights, p, on);
     return launched();
   });
 }

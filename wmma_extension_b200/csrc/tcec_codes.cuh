@@ -12,7 +12,7 @@
 // activations; the sum runs over k or over tokens).  The scale of a code is then the same for a whole row of a tensor-core tile, and
 // is applied to the FP32 sum of a group: the tensor cores multiply whole numbers, which bf16 and f16 hold exactly.
 //
-//   4-bit block: 8 strips of 16 rows x 256 words of 8 codes, then 128 / group x 128 entries.  A word holds 8 consecutive k of one row,
+//   4-bit block: 8 strips of 16 rows, each 256 words of 8 codes and then 128 / group x 16 entries.  A word holds 8 consecutive k of one row,
 //   nibble j of them k = 2 j (j < 4) and 2 (j - 4) + 1, so that (w >> 4 i) & 0x000f000f is the pair (2 i, 2 i + 1).  Words are in the
 //   order of the registers of mma.m16n8k16: lane 4 g + t of a warp finds rows g and g + 8, k = 8 t .. 8 t + 7 of each 32, in two
 //   128-bit loads.  An entry is the scale as FP32 (its low 12 bits or more are zero) with the zero point in the low 4 bits.
@@ -36,10 +36,17 @@ constexpr int kQ4CodeBytes = 8192, kQ8CodeBytes = 16384, kEntryBytes = 512;  // 
 __host__ __device__ constexpr int q4_block_bytes(int group) { return kQ4CodeBytes + kEntryBytes * (kCodeSpan / group); }
 constexpr int kQ8BlockBytes = kQ8CodeBytes + kEntryBytes;
 
-// Where the word of (row, chunk of 8 k) lies in a 4-bit block.
+constexpr int kStripCodeBytes = 1024;
+__host__ __device__ constexpr int q4_strip_bytes(int group) { return kStripCodeBytes + 64 * (kCodeSpan / group); }
+// Where the word of (row, chunk of 8 k), and the entry of (row, group), lie in a 4-bit block, in words.
+template <int kGroup>
 __host__ __device__ __forceinline__ int q4_word(int row, int chunk) {
   const int lane = (row & 7) * 4 + (chunk & 3), panel = chunk >> 2;
-  return (row >> 4) * 256 + (panel >> 1) * 128 + lane * 4 + (panel & 1) * 2 + ((row >> 3) & 1);
+  return (row >> 4) * (q4_strip_bytes(kGroup) / 4) + (panel >> 1) * 128 + lane * 4 + (panel & 1) * 2 + ((row >> 3) & 1);
+}
+template <int kGroup>
+__host__ __device__ __forceinline__ int q4_entry_word(int row, int group) {
+  return (row >> 4) * (q4_strip_bytes(kGroup) / 4) + kStripCodeBytes / 4 + group * 16 + (row & 15);
 }
 
 // ---------------------------------------------------------------- typed elements
@@ -292,9 +299,9 @@ __global__ void __launch_bounds__(256) pack_q4_kernel(const PackQ4Params p) {
 #pragma unroll
       for (int j = 0; j < 8 / kSpans; ++j) {
         const uint32_t mine = some ? code[j] : 0, other = __shfl_xor_sync(0xffffffffu, mine, 1);  // the odd lane's half is 8 bits higher
-        if ((t & 1) == 0) words[q4_word(r, (q * 8 / kSpans + j) * 2 + (t >> 1))] = mine | (other << 8);
+        if ((t & 1) == 0) words[q4_word<kGroup>(r, (q * 8 / kSpans + j) * 2 + (t >> 1))] = mine | (other << 8);
       }
-      if (t == 0) words[2048 + q * 128 + r] = q4_entry(bad ? nan32() : s, z);
+      if (t == 0) words[q4_entry_word<kGroup>(r, q)] = q4_entry(bad ? nan32() : s, z);
     }
   }
   __syncthreads();
@@ -317,12 +324,12 @@ __global__ void __launch_bounds__(256) pack_q4_codes_kernel(const PackQ4Params p
       const float s = p.scale_bf16 ? ld_element<kTypeBf16>(p.scales, at) : ld_element<kTypeF16>(p.scales, at);
       entry = q4_entry(not_finite(s) ? nan32() : s, p.zeros ? (p.zeros[at] & 15) : 8);
     }
-    words[2048 + i] = entry;
+    words[q4_entry_word<kGroup>(r, i >> 7)] = entry;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 2048; i += 256) {
     const int r = i >> 4, chunk = i & 15, row = tile * kCodeRows + r, k0 = kb * kCodeSpan + chunk * 8;
-    const uint32_t z = words[2048 + (chunk * 8 / kGroup) * 128 + r] & 15u;  // what is beyond the matrix stands for zero
+    const uint32_t z = words[q4_entry_word<kGroup>(r, chunk * 8 / kGroup)] & 15u;  // what is beyond the matrix stands for zero
     uint32_t w = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -334,7 +341,7 @@ __global__ void __launch_bounds__(256) pack_q4_codes_kernel(const PackQ4Params p
       }
       w |= lo << (4 * j) | hi << (4 * j + 16);
     }
-    words[q4_word(r, chunk)] = w;
+    words[q4_word<kGroup>(r, chunk)] = w;
   }
   let_next_launch_start();
   __syncthreads();
@@ -365,8 +372,8 @@ __global__ void __launch_bounds__(256) unpack_q4_kernel(const UnpackParams p) {
   for (int i = threadIdx.x; i < 4096; i += 256) {  // four values at a time
     const int r = i >> 5, part = i & 31, chunk = part >> 1, row = tile * kCodeRows + r, k0 = kb * kCodeSpan + part * 4;
     if (row >= p.rows || k0 >= p.sum) continue;
-    const uint32_t w = words[q4_word(r, chunk)] >> ((part & 1) * 8);
-    const uint32_t entry = words[2048 + (chunk * 8 / kGroup) * 128 + r];
+    const uint32_t w = words[q4_word<kGroup>(r, chunk)] >> ((part & 1) * 8);
+    const uint32_t entry = words[q4_entry_word<kGroup>(r, chunk * 8 / kGroup)];
     const float s = __uint_as_float(entry & ~15u);
     const int z = static_cast<int>(entry & 15u);
     float v[4];

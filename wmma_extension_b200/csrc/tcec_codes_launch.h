@@ -1,0 +1,47 @@
+// What the host side of the products with codes hands to their kernels, and the launches, each in a translation unit of its own.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace tcec_sm100 {
+
+struct GemmCodesParams {
+  const uint8_t* codes;       // [row tile][block]
+  const uint8_t* panels;      // [128 columns][block][part]
+  int rows, cols, blocks;     // blocks along the sum
+  int parts;                  // of the dense operand: 1, or 3 (FP32)
+  int row_tiles, col_tiles;
+  float alpha, beta;
+  void* c;
+  long long c_row, c_col;     // steps between elements of C along rows and columns of this product
+  int c_type;
+  int* status;
+};
+
+struct GemvQ4Params {
+  const uint8_t* codes;
+  const uint8_t* staged;      // x as operands of the MMAs (stage_columns_kernel), or null: one token, from x
+  const void* x;              // one token: element i at i * x_k
+  long long x_k;
+  int n, k, tokens, blocks;
+  int vec;                    // x_k 1 and x aligned for four values at a time
+  float alpha, beta;
+  void* c;                    // element (token, row) at token * c_token + row * c_row
+  long long c_token, c_row;
+  int c_type;
+  int* status;
+};
+
+}  // namespace tcec_sm100
+
+namespace tcec_host {
+
+cudaError_t set_gemm_codes_attrs();
+// eights: of columns (1, 2 or 4), which staged x has.
+void launch_gemv_q4(int type, int group, int eights, const tcec_sm100::GemvQ4Params& p, cudaStream_t stream);
+// spans: groups of 4-bit codes in a block, 0: 8-bit codes.  ctas: of a cluster.
+void launch_gemm_codes(bool f16, int spans, int bn, const tcec_sm100::GemmCodesParams& gp, int ctas, int grid, cudaStream_t stream);
+cudaError_t set_gemv_q4_attrs();
+
+}  // namespace tcec_host

@@ -15,18 +15,6 @@
 
 namespace tcec_sm100 {
 
-struct GemvQ4Params {
-  const uint8_t* codes;
-  const void* x;              // element (token, i) at token * x_token + i * x_k
-  long long x_token, x_k;
-  int n, k, tokens, blocks;
-  int vec;                    // x_k 1 and four values at a time aligned
-  float alpha, beta;
-  void* c;                    // element (token, row) at token * c_token + row * c_row
-  long long c_token, c_row;
-  int c_type;
-};
-
 template <bool kF16>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (kF16)
@@ -39,174 +27,214 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A warp's x of one block in shared memory: columns of 128 values in 16 bits, 320 bytes apart, so that lanes of two columns and four
-// times 16 bytes read from all banks at once.
-constexpr int kXPitch = 320;
+// Loads that are issued where they stand, ahead of the waits that follow.
+__device__ __forceinline__ uint4 ld_ahead128(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
 
-template <int kType, int kGroup, int kCols, int kStrips>
+// kEights: columns in eights.  kOne: one token, taken from x as it is; else x comes staged (tcec_stage.cuh).
+template <int kType, int kGroup, int kEights, int kStrips, bool kOne>
 struct GemvQ4Cfg {
   static constexpr int PARTS = kType == kTypeF32 ? 3 : 1;
-  static constexpr int WIDTH = kCols * 8;                     // columns
-  static constexpr int TOKENS = WIDTH / PARTS;
   static constexpr int ROWS = 16 * kStrips;
   static constexpr int WARPS = 8;
-  static constexpr int AHEAD = kCols == 1 ? 2 : 1;            // blocks loaded ahead of the one at work
-  static constexpr int X_BYTES = WIDTH * kXPitch;             // of a warp
-  static constexpr int SUM_PITCH = WIDTH + 1;
+  static constexpr int STAGE_BYTES = kStrips * q4_strip_bytes(kGroup);
+  static constexpr int STAGES = 4;                            // blocks of codes under way, of each warp
+  static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int X_PITCH = 320;                         // of a column in shared memory: two columns' lanes read from all banks
+  static constexpr int X_BYTES = kOne ? 8 * X_PITCH : 0;
+  static constexpr int SUM_PITCH = kEights * 8 + 1;
   static constexpr int SUM_BYTES = WARPS * ROWS * SUM_PITCH * 4;
-  static constexpr int SMEM_BYTES = WARPS * X_BYTES > SUM_BYTES ? WARPS * X_BYTES : SUM_BYTES;
+  static constexpr int USED = WARPS * (RING_BYTES + X_BYTES);
+  static constexpr int SMEM_BYTES = (USED > SUM_BYTES ? USED : SUM_BYTES) + 128;
 };
 
-// What a lane holds of one block: codes and entries of its rows, and four values of every token.
-template <int kType, int kGroup, int kCols, int kStrips>
-struct GemvQ4Block {
-  using Cfg = GemvQ4Cfg<kType, kGroup, kCols, kStrips>;
-  static constexpr int kSpans = kCodeSpan / kGroup;
-  uint4 w[kStrips][2];
-  uint32_t entry[kStrips][kSpans][2];
-  Four<kType> x[Cfg::TOKENS];
-
-  __device__ __forceinline__ void load(const GemvQ4Params& p, const uint8_t* block, int kb, int in_tile, int lane) {
-    const uint8_t* strip = block + in_tile * 64 + lane * 16;
-    const uint8_t* e = block + kQ4CodeBytes + (in_tile + (lane >> 2)) * 4;
-#pragma unroll
-    for (int s = 0; s < kStrips; ++s) {
-      w[s][0] = ld_once128(strip + s * 1024);
-      w[s][1] = ld_once128(strip + s * 1024 + 512);
-#pragma unroll
-      for (int q = 0; q < kSpans; ++q) {
-        entry[s][q][0] = ld_operand32(e + q * kEntryBytes + s * 64);
-        entry[s][q][1] = ld_operand32(e + q * kEntryBytes + s * 64 + 32);
-      }
-    }
-    const int k0 = kb * kCodeSpan + lane * 4, left = p.k - k0;
-    if (p.vec && (kb + 1) * kCodeSpan <= p.k) {
-#pragma unroll
-      for (int i = 0; i < Cfg::TOKENS; ++i)
-        if (i < p.tokens) x[i].load(p.x, i * p.x_token + k0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < Cfg::TOKENS; ++i)
-        if (i < p.tokens) {
-          uint32_t v[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const long long at = i * p.x_token + min(k0 + j, p.k - 1) * p.x_k;
-            if constexpr (kType == kTypeF32) v[j] = ld_operand32(static_cast<const uint32_t*>(p.x) + at);
-            else v[j] = ld_operand16(static_cast<const uint16_t*>(p.x) + at);
-            if (j >= left) v[j] = 0;
-          }
-          if constexpr (kType == kTypeF32) x[i].raw = make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
-          else x[i].raw = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
-        }
-    }
-  }
-  // x in its columns, for the lanes that need it as operand.
-  __device__ __forceinline__ void share_x(const GemvQ4Params& p, uint8_t* mine, int lane) const {
-#pragma unroll
-    for (int i = 0; i < Cfg::TOKENS; ++i)
-      if (i < p.tokens) {
-        uint8_t* to = mine + i * Cfg::PARTS * kXPitch + lane * 8;
-        if constexpr (kType == kTypeF32) {
-          uint2 hi, mid, lo;
-          split3_bf16(x[i].raw.x, x[i].raw.y, hi.x, mid.x, lo.x);
-          split3_bf16(x[i].raw.z, x[i].raw.w, hi.y, mid.y, lo.y);
-          *reinterpret_cast<uint2*>(to) = hi;
-          *reinterpret_cast<uint2*>(to + kXPitch) = mid;
-          *reinterpret_cast<uint2*>(to + 2 * kXPitch) = lo;
-        } else {
-          *reinterpret_cast<uint2*>(to) = x[i].raw;
-        }
-      }
-  }
-  __device__ __forceinline__ void multiply(float (&acc)[kStrips][kCols][4], const uint8_t* mine, int lane) const {
-    constexpr bool kF16 = kType == kTypeF16;
-#pragma unroll
-    for (int q = 0; q < kSpans; ++q) {
-      float d[kStrips][kCols][4];
-#pragma unroll
-      for (int s = 0; s < kStrips; ++s)
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) d[s][c][0] = d[s][c][1] = d[s][c][2] = d[s][c][3] = 0.f;
-#pragma unroll
-      for (int panel = q * 4 / kSpans; panel < (q + 1) * 4 / kSpans; ++panel) {
-        uint4 b[kCols];
-#pragma unroll
-        for (int c = 0; c < kCols; ++c)
-          b[c] = *reinterpret_cast<const uint4*>(mine + (c * 8 + (lane >> 2)) * kXPitch + panel * 64 + (lane & 3) * 16);
-#pragma unroll
-        for (int s = 0; s < kStrips; ++s) {
-          const uint4 pair = w[s][panel >> 1];
-          const uint4 r0 = q4_expand<kF16>(panel & 1 ? pair.z : pair.x, q4_zero<kF16>(entry[s][q][0] & 15u));
-          const uint4 r1 = q4_expand<kF16>(panel & 1 ? pair.w : pair.y, q4_zero<kF16>(entry[s][q][1] & 15u));
-#pragma unroll
-          for (int c = 0; c < kCols; ++c) {
-            mma16816<kF16>(d[s][c], r0.x, r1.x, r0.y, r1.y, b[c].x, b[c].y);
-            mma16816<kF16>(d[s][c], r0.z, r1.z, r0.w, r1.w, b[c].z, b[c].w);
-          }
-        }
-      }
-#pragma unroll
-      for (int s = 0; s < kStrips; ++s) {
-        const float s0 = __uint_as_float(entry[s][q][0] & ~15u), s1 = __uint_as_float(entry[s][q][1] & ~15u);
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          acc[s][c][0] = __fmaf_rn(s0, d[s][c][0], acc[s][c][0]);
-          acc[s][c][1] = __fmaf_rn(s0, d[s][c][1], acc[s][c][1]);
-          acc[s][c][2] = __fmaf_rn(s1, d[s][c][2], acc[s][c][2]);
-          acc[s][c][3] = __fmaf_rn(s1, d[s][c][3], acc[s][c][3]);
-        }
-      }
-    }
-  }
-};
-
-// kCols: columns in eights.
-template <int kType, int kGroup, int kCols, int kStrips>
-__global__ void __launch_bounds__(256) gemv_q4_kernel(const GemvQ4Params p) {
-  using Cfg = GemvQ4Cfg<kType, kGroup, kCols, kStrips>;
-  using Block = GemvQ4Block<kType, kGroup, kCols, kStrips>;
-  extern __shared__ __align__(16) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint8_t* mine = smem + warp * Cfg::X_BYTES;
-  for (int i = lane; i < Cfg::X_BYTES / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);  // columns that nobody has
-  const int row0 = blockIdx.x * Cfg::ROWS, in_tile = row0 % kCodeRows;
-  constexpr size_t kBlockBytes = q4_block_bytes(kGroup);
-  const uint8_t* base = p.codes + static_cast<size_t>(row0 / kCodeRows) * p.blocks * kBlockBytes;
-  __syncwarp();
-  wait_for_launch_before();
-  let_next_launch_start();
-
-  float acc[kStrips][kCols][4];
+// The codes of a block, a strip at a time, times the operands b(panel, eight); sums folded into acc.
+template <int kType, int kGroup, int kEights, int kStrips, class B>
+__device__ __forceinline__ void multiply_block(float (&acc)[kStrips][kEights][4], const uint8_t* stage, int lane, const B& operands) {
+  constexpr bool kF16 = kType == kTypeF16;
+  constexpr int kSpans = kCodeSpan / kGroup;
+  uint4 w[kStrips][2];  // rows g and g + 8, of two panels each
 #pragma unroll
   for (int s = 0; s < kStrips; ++s)
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) acc[s][c][0] = acc[s][c][1] = acc[s][c][2] = acc[s][c][3] = 0.f;
+    for (int h = 0; h < 2; ++h) w[s][h] = *reinterpret_cast<const uint4*>(stage + s * q4_strip_bytes(kGroup) + h * 512 + lane * 16);
+#pragma unroll
+  for (int q = 0; q < kSpans; ++q) {
+    float d[kStrips][kEights][4];
+    uint32_t entry[kStrips][2];
+#pragma unroll
+    for (int s = 0; s < kStrips; ++s) {
+      const uint32_t* e = reinterpret_cast<const uint32_t*>(stage + s * q4_strip_bytes(kGroup) + kStripCodeBytes) + q * 16 + (lane >> 2);
+      entry[s][0] = e[0];
+      entry[s][1] = e[8];
+#pragma unroll
+      for (int c = 0; c < kEights; ++c) d[s][c][0] = d[s][c][1] = d[s][c][2] = d[s][c][3] = 0.f;
+    }
+#pragma unroll
+    for (int panel = q * 4 / kSpans; panel < (q + 1) * 4 / kSpans; ++panel) {
+      uint4 b[kEights];
+      operands(panel, b);
+#pragma unroll
+      for (int s = 0; s < kStrips; ++s) {
+        const uint4 pair = w[s][panel >> 1];
+        const uint4 r0 = q4_expand<kF16>(panel & 1 ? pair.z : pair.x, q4_zero<kF16>(entry[s][0] & 15u));
+        const uint4 r1 = q4_expand<kF16>(panel & 1 ? pair.w : pair.y, q4_zero<kF16>(entry[s][1] & 15u));
+#pragma unroll
+        for (int c = 0; c < kEights; ++c) {
+          mma16816<kF16>(d[s][c], r0.x, r1.x, r0.y, r1.y, b[c].x, b[c].y);
+          mma16816<kF16>(d[s][c], r0.z, r1.z, r0.w, r1.w, b[c].z, b[c].w);
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kStrips; ++s) {
+      const float s0 = __uint_as_float(entry[s][0] & ~15u), s1 = __uint_as_float(entry[s][1] & ~15u);
+#pragma unroll
+      for (int c = 0; c < kEights; ++c) {
+        acc[s][c][0] = __fmaf_rn(s0, d[s][c][0], acc[s][c][0]);
+        acc[s][c][1] = __fmaf_rn(s0, d[s][c][1], acc[s][c][1]);
+        acc[s][c][2] = __fmaf_rn(s1, d[s][c][2], acc[s][c][2]);
+        acc[s][c][3] = __fmaf_rn(s1, d[s][c][3], acc[s][c][3]);
+      }
+    }
+  }
+}
 
-  constexpr int kHeld = Cfg::AHEAD + 1;
-  Block held[kHeld];
+template <int kType, int kGroup, int kEights, int kStrips, bool kOne>
+__global__ void __launch_bounds__(256) gemv_q4_kernel(const GemvQ4Params p) {
+  using Cfg = GemvQ4Cfg<kType, kGroup, kEights, kStrips, kOne>;
+  static_assert(!kOne || kEights == 1, "one token has at most three columns");
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t bars[Cfg::WARPS][Cfg::STAGES];
+  __shared__ uint32_t abort_flag;
+  uint8_t* const smem = smem_raw + ((0u - smem_u32(smem_raw)) & 127u);
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  uint8_t* const ring = smem + warp * Cfg::RING_BYTES;
+  [[maybe_unused]] uint8_t* const x_shared = smem + Cfg::WARPS * Cfg::RING_BYTES + warp * Cfg::X_BYTES;
+  if (lane == 0) {
+    for (int s = 0; s < Cfg::STAGES; ++s) mbar_init(smem_u32(&bars[warp][s]), 1);
+    fence_mbar_init();
+  }
+  if (threadIdx.x == 0) abort_flag = 0;
+  if constexpr (kOne)  // columns that no part of the token has
+    for (int i = lane; i < Cfg::X_BYTES / 16; i += 32) reinterpret_cast<uint4*>(x_shared)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  const int row0 = blockIdx.x * Cfg::ROWS;
+  constexpr size_t kBlockBytes = q4_block_bytes(kGroup);
+  const uint8_t* codes = p.codes + static_cast<size_t>(row0 / kCodeRows) * p.blocks * kBlockBytes + row0 % kCodeRows / 16 * q4_strip_bytes(kGroup);
+  auto fetch = [&](int kb, int stage) {  // lane 0
+    const uint32_t bar = smem_u32(&bars[warp][stage]);
+    mbar_arrive_expect_tx(bar, Cfg::STAGE_BYTES);
+    bulk_load(smem_u32(ring + stage * Cfg::STAGE_BYTES), codes + kb * kBlockBytes, Cfg::STAGE_BYTES, bar);
+  };
+  // Staged x is written by the kernel before this one, which was through its own wait when this one could start: whatever the codes
+  // come from has ended, and they are fetched without waiting for x.
+  if constexpr (kOne) wait_for_launch_before();
+  if (lane == 0)
+    for (int i = 0; i < Cfg::STAGES; ++i)
+      if (warp + i * Cfg::WARPS < p.blocks) fetch(warp + i * Cfg::WARPS, i);
+  if constexpr (!kOne) wait_for_launch_before();
+  let_next_launch_start();
+
+  float acc[kStrips][kEights][4];
 #pragma unroll
-  for (int i = 0; i < Cfg::AHEAD; ++i)
-    if (warp + i * Cfg::WARPS < p.blocks) held[i].load(p, base + (warp + i * Cfg::WARPS) * kBlockBytes, warp + i * Cfg::WARPS, in_tile, lane);
-  for (int kb = warp; kb < p.blocks; kb += kHeld * Cfg::WARPS) {
+  for (int s = 0; s < kStrips; ++s)
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      const int now = kb + i * Cfg::WARPS, next = now + Cfg::AHEAD * Cfg::WARPS;
-      if (now >= p.blocks) break;
-      if (next < p.blocks) held[(i + Cfg::AHEAD) % kHeld].load(p, base + next * kBlockBytes, next, in_tile, lane);
-      held[i].share_x(p, mine, lane);
-      __syncwarp();
-      held[i].multiply(acc, mine, lane);
-      __syncwarp();
+    for (int c = 0; c < kEights; ++c) acc[s][c][0] = acc[s][c][1] = acc[s][c][2] = acc[s][c][3] = 0.f;
+
+  // x of the next block, on its way while this one is worked on: the token's four values of this lane, or whole operands
+  [[maybe_unused]] Four<kType> four;
+  [[maybe_unused]] uint4 b_ahead[4][kEights];
+  auto load_four = [&](int kb) {
+    const int k0 = kb * kCodeSpan + lane * 4, left = p.k - k0;
+    if (p.vec && left >= 4) {
+      four.load(p.x, k0);
+    } else {
+      uint32_t v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const long long at = min(k0 + j, p.k - 1) * p.x_k;
+        if constexpr (kType == kTypeF32) v[j] = ld_operand32(static_cast<const uint32_t*>(p.x) + at);
+        else v[j] = ld_operand16(static_cast<const uint16_t*>(p.x) + at);
+        if (j >= left) v[j] = 0;
+      }
+      if constexpr (kType == kTypeF32) four.raw = make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
+      else four.raw = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+    }
+  };
+  const uint8_t* const staged = kOne ? nullptr : after_wait(p.staged) + lane * 16;
+  auto load_operands = [&](int kb, int panel) {
+#pragma unroll
+    for (int c = 0; c < kEights; ++c) b_ahead[panel][c] = ld_ahead128(staged + static_cast<size_t>(kb) * (kEights * 2048) + panel * (kEights * 512) + c * 512);
+  };
+  if (warp < p.blocks) {
+    if constexpr (kOne) {
+      load_four(warp);
+    } else {
+#pragma unroll
+      for (int panel = 0; panel < 4; ++panel) load_operands(warp, panel);
+    }
+  }
+  int stage = 0;
+  uint32_t parity = 0;
+  bool ok = true;
+  int kb = warp;
+  for (; kb < p.blocks; kb += Cfg::WARPS) {
+    const int next = kb + Cfg::WARPS;
+    if constexpr (kOne) {
+      uint8_t* to = x_shared + lane * 8;
+      if constexpr (kType == kTypeF32) {
+        uint2 hi, mid, lo;
+        split3_bf16(four.raw.x, four.raw.y, hi.x, mid.x, lo.x);
+        split3_bf16(four.raw.z, four.raw.w, hi.y, mid.y, lo.y);
+        *reinterpret_cast<uint2*>(to) = hi;
+        *reinterpret_cast<uint2*>(to + Cfg::X_PITCH) = mid;
+        *reinterpret_cast<uint2*>(to + 2 * Cfg::X_PITCH) = lo;
+      } else {
+        *reinterpret_cast<uint2*>(to) = four.raw;
+      }
+      if (next < p.blocks) load_four(next);
+    }
+    ok = mbar_wait_lanes(smem_u32(&bars[warp][stage]), parity, &abort_flag);  // brings the lanes together, too
+    if (!ok) break;
+    const uint8_t* const here = ring + stage * Cfg::STAGE_BYTES;
+    if constexpr (kOne) {
+      multiply_block<kType, kGroup, kEights, kStrips>(acc, here, lane, [&](int panel, uint4(&b)[kEights]) {
+        b[0] = *reinterpret_cast<const uint4*>(x_shared + (lane >> 2) * Cfg::X_PITCH + panel * 64 + (lane & 3) * 16);
+      });
+    } else {
+      multiply_block<kType, kGroup, kEights, kStrips>(acc, here, lane, [&](int panel, uint4(&b)[kEights]) {
+#pragma unroll
+        for (int c = 0; c < kEights; ++c) b[c] = b_ahead[panel][c];
+        if (next < p.blocks) load_operands(next, panel);
+      });
+    }
+    __syncwarp();  // all have read the stage
+    if (lane == 0 && kb + Cfg::STAGES * Cfg::WARPS < p.blocks) fetch(kb + Cfg::STAGES * Cfg::WARPS, stage);
+    if (++stage == Cfg::STAGES) stage = 0, parity ^= 1;
+  }
+  if (!ok) {
+    abort_flag = 1;
+    if (lane == 0) {
+      atomicCAS(p.status, 0, kErrOperandWait);
+      // this warp's own copies land before the CTA gives up its shared memory
+      for (int i = 0; i < Cfg::STAGES && kb < p.blocks; ++i, kb += Cfg::WARPS) {
+        mbar_wait_plain(smem_u32(&bars[warp][stage]), parity);
+        if (++stage == Cfg::STAGES) stage = 0, parity ^= 1;
+      }
     }
   }
 
-  __syncthreads();  // x is read, sums take its place
+  __syncthreads();  // all codes have been read: sums take their place
+  if (abort_flag) return;
   float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int s = 0; s < kStrips; ++s)
 #pragma unroll
-    for (int c = 0; c < kCols; ++c)
+    for (int c = 0; c < kEights; ++c)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         sums[(warp * Cfg::ROWS + s * 16 + (lane >> 2) + (j >> 1) * 8) * Cfg::SUM_PITCH + c * 8 + (lane & 3) * 2 + (j & 1)] = acc[s][c][j];

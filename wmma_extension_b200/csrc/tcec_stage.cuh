@@ -1,0 +1,184 @@
+// The dense operand of a product with codes, whatever its type, order and alignment, laid out for the tensor cores: 16-bit values, FP32 in three
+// bf16 parts of 8 bits each, which together are exactly it; what is beyond the matrix is zero.
+//
+// Bound by memory: every value is read once and written once (FP32: 6 bytes for 4).
+#pragma once
+#include "tcec_codes.cuh"
+#include "tcec_panels.cuh"
+
+namespace tcec_sm100 {
+
+constexpr int kSpanPanels = kCodeSpan / 32;                  // panels of one block and part
+constexpr int kSpanBytes = kSpanPanels * kPanelBytes;        // 32 KB
+struct StagePanelsParams {
+  const void* src;            // element (col, i) at col * col_step + i * sum_step
+  long long col_step, sum_step;
+  int cols, sum;
+  int blocks;                 // along the sum
+  uint8_t* panels;            // [128 columns][block][part][panel]
+  int vec;                    // sum_step 1 and aligned for 16 bytes
+};
+// x = hi + mid + lo, 8 bits each, two values at a time.  Exactly so unless lo falls below the smallest bf16 number; what is not finite
+// stays in hi alone.
+__device__ __forceinline__ void split3_bf16(float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  const uint32_t bx = x != x ? 0x7fc00000u : __float_as_uint(x), by = y != y ? 0x7fc00000u : __float_as_uint(y);
+  float rx = x - __uint_as_float(bx & 0xffff0000u), ry = y - __uint_as_float(by & 0xffff0000u);
+  if (not_finite(x)) rx = 0.f;
+  if (not_finite(y)) ry = 0.f;
+  hi = __byte_perm(bx, by, 0x7632);
+  const uint32_t mx = __float_as_uint(rx), my = __float_as_uint(ry);
+  mid = __byte_perm(mx, my, 0x7632);
+  const float lx = rx - __uint_as_float(mx & 0xffff0000u), ly = ry - __uint_as_float(my & 0xffff0000u);
+  lo = __byte_perm(__float_as_uint(lx), __float_as_uint(ly), 0x7632);
+}
+
+// Eight FP32 values to an item of each part; the small parts first, so that the accumulator, which truncates, cuts off less.
+template <class Put>
+__device__ __forceinline__ void put_split(const Put& put, int it, const float (&v)[8], bool none) {
+  uint32_t part[3][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) split3_bf16(none ? 0.f : v[2 * j], none ? 0.f : v[2 * j + 1], part[0][j], part[1][j], part[2][j]);
+#pragma unroll
+  for (int q = 0; q < 3; ++q) put(it, q, make_uint4(part[2 - q][0], part[2 - q][1], part[2 - q][2], part[2 - q][3]));
+}
+
+// One CTA a block of 128 columns x 128 of the sum; an item is 16 bytes of a panel, eight consecutive values of one column.  Addresses stay
+// among the elements that exist, so that all loads of some items go out before the first is waited for.
+template <int kType>
+__global__ void __launch_bounds__(256) stage_panels_kernel(const StagePanelsParams p) {
+  constexpr int kParts = kType == kTypeF32 ? 3 : 1;
+  wait_for_launch_before();
+  const int kb = blockIdx.x % p.blocks, cb = blockIdx.x / p.blocks;
+  uint8_t* out = p.panels + static_cast<size_t>(blockIdx.x) * kParts * kSpanBytes;
+  const int cols = min(kCodeRows, (p.cols - cb * kCodeRows + 15) & ~15);  // columns that an MMA may read
+  const int first = threadIdx.x;
+  // Item `it` of a thread: column r, chunk c of panel it / 2.
+  const bool along = p.sum_step == 1;
+  const int r0 = along ? (first & 7) + ((first >> 5) & 7) * 8 : first & 127;   // a warp: 8 columns x 64 bytes, or 32 columns
+  const int c0 = along ? (first >> 3) & 3 : first >> 7;
+  auto column = [&](int it) { return along ? r0 + (it & 1) * 64 : r0; };
+  auto chunk = [&](int it) { return along ? c0 : c0 + (it & 1) * 2; };
+  auto put = [&](int it, int part, const uint4& v) {
+    const int r = column(it);
+    if (r < cols)
+      *reinterpret_cast<uint4*>(out + part * kSpanBytes + (it >> 1) * kPanelBytes + (r >> 3) * 512 + chunk(it) * 128 + (r & 7) * 16) = v;
+  };
+  constexpr int kAtOnce = kType == kTypeF32 ? 2 : 4;  // items whose loads are under way together
+  const int cols_here = p.cols - cb * kCodeRows, sum_here = p.sum - kb * kCodeSpan;
+  const long long origin = static_cast<long long>(cb) * kCodeRows * p.col_step + static_cast<long long>(kb) * kCodeSpan * p.sum_step;
+#pragma unroll 1
+  for (int it0 = 0; it0 < 8; it0 += kAtOnce) {
+    if (p.vec && sum_here >= kCodeSpan) {
+      uint4 raw[kAtOnce][kType == kTypeF32 ? 2 : 1];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int it = it0 + i;
+        const long long at = origin + min(column(it), cols_here - 1) * p.col_step + (it >> 1) * 32 + chunk(it) * 8;
+        if constexpr (kType == kTypeF32) {
+          raw[i][0] = ld_operand128(static_cast<const float*>(p.src) + at);
+          raw[i][1] = ld_operand128(static_cast<const float*>(p.src) + at + 4);
+        } else {
+          raw[i][0] = ld_operand128(static_cast<const uint16_t*>(p.src) + at);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const bool none = column(it0 + i) >= cols_here;
+        if constexpr (kType == kTypeF32) {
+          const float v[8] = {__uint_as_float(raw[i][0].x), __uint_as_float(raw[i][0].y), __uint_as_float(raw[i][0].z), __uint_as_float(raw[i][0].w),
+                              __uint_as_float(raw[i][1].x), __uint_as_float(raw[i][1].y), __uint_as_float(raw[i][1].z), __uint_as_float(raw[i][1].w)};
+          put_split(put, it0 + i, v, none);
+        } else {
+          put(it0 + i, 0, none ? make_uint4(0, 0, 0, 0) : raw[i][0]);
+        }
+      }
+    } else {
+      typename std::conditional<kType == kTypeF32, float, uint32_t>::type w[kAtOnce][8];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int it = it0 + i, at_sum = (it >> 1) * 32 + chunk(it) * 8 + j;
+          const long long at = origin + min(column(it), cols_here - 1) * p.col_step + min(at_sum, sum_here - 1) * p.sum_step;
+          if constexpr (kType == kTypeF32) w[i][j] = ld_operand(static_cast<const float*>(p.src) + at);
+          else w[i][j] = ld_operand16(static_cast<const uint16_t*>(p.src) + at);
+        }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int it = it0 + i, at_sum = (it >> 1) * 32 + chunk(it) * 8;
+        const bool none = column(it) >= cols_here;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (none || at_sum + j >= sum_here) w[i][j] = 0;
+        if constexpr (kType == kTypeF32) put_split(put, it, w[i], false);
+        else put(it, 0, make_uint4(w[i][0] | w[i][1] << 16, w[i][2] | w[i][3] << 16, w[i][4] | w[i][5] << 16, w[i][6] | w[i][7] << 16));
+      }
+    }
+  }
+  let_next_launch_start();
+}
+
+// Columns of mma.m16n8k16: for each block of 128 of the sum, 32 of it and eight columns, lane 4 g + t has 8 values of column g from
+// 8 t on, 16 bytes.  A column is a token, or a part of one (FP32).  One CTA a block of the sum; a thread an item and all its parts.
+struct StageColumnsParams {
+  const void* src;
+  long long col_step, sum_step;
+  int tokens, sum;
+  int eights;                 // of columns
+  uint8_t* out;
+  int vec;                    // sum_step 1 and aligned for 16 bytes
+};
+template <int kType>
+__global__ void __launch_bounds__(128) stage_columns_kernel(const StageColumnsParams p) {
+  constexpr int kParts = kType == kTypeF32 ? 3 : 1;
+  wait_for_launch_before();
+  let_next_launch_start();
+  const int kb = blockIdx.x, chunk = threadIdx.x & 15, sum_here = p.sum - kb * kCodeSpan - chunk * 8;
+  uint8_t* out = p.out + static_cast<size_t>(kb) * p.eights * 2048 + (chunk >> 2) * p.eights * 512 + (chunk & 3) * 16;
+  const int columns = p.eights * 8;
+  for (int token = blockIdx.y * 8 + (threadIdx.x >> 4); token * kParts < columns; token += gridDim.y * 8) {
+    const long long at = token * p.col_step + (static_cast<long long>(kb) * kCodeSpan + chunk * 8) * p.sum_step;
+    uint4 o[kParts] = {};
+    if (token < p.tokens && sum_here > 0) {
+      if constexpr (kType == kTypeF32) {
+        const float* src = static_cast<const float*>(p.src) + at;
+        float v[8];
+        if (p.vec && sum_here >= 8) {
+          const float4 a = ld_operand(reinterpret_cast<const float4*>(src)), b = ld_operand(reinterpret_cast<const float4*>(src + 4));
+          v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = ld_operand(src + min(j, sum_here - 1) * p.sum_step);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j >= sum_here) v[j] = 0.f;
+        }
+        uint32_t w[3][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split3_bf16(v[2 * j], v[2 * j + 1], w[0][j], w[1][j], w[2][j]);
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) o[q] = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+      } else {
+        const uint16_t* src = static_cast<const uint16_t*>(p.src) + at;
+        if (p.vec && sum_here >= 8) {
+          o[0] = ld_operand128(src);
+        } else {
+          uint32_t w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = ld_operand16(src + min(j, sum_here - 1) * p.sum_step);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j >= sum_here) w[j] = 0;
+          o[0] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) {
+      const int col = token * kParts + q;
+      if (col < columns) *reinterpret_cast<uint4*>(out + (col >> 3) * 512 + (col & 7) * 64) = o[q];
+    }
+  }
+}
+
+}  // namespace tcec_sm100
