@@ -1,5 +1,5 @@
 // The common calls of wmma_extension_b200/tcec.py without their interpreter time: one product, a strided batch, packing, and a
-// product of packed operands on plain float32 CUDA tensors of the current device.  Anything else (and everything that has to raise)
+// product of packed operands on plain float32 CUDA tensors of the current device; the operands held in few bits likewise.  Anything else (and everything that has to raise)
 // returns None, and tcec.py's own code, which accepts and checks it all, takes the call; so does every call before bind().  A status
 // other than TCEC_OK comes back as an int.
 //
@@ -8,6 +8,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <optional>
@@ -30,6 +31,22 @@ PackFn g_pack[2] = {nullptr, nullptr};
 PackedFn g_packed = nullptr;
 PackedBytesFn g_packed_bytes = nullptr;
 bool g_bound = false;  // read and written with the GIL held
+
+// Operands held in few bits.
+struct Codes {
+  decltype(&tcec_q4_bytes) q4_bytes;
+  decltype(&tcec_pack_q4) pack_q4;
+  decltype(&tcec_unpack_q4) unpack_q4;
+  decltype(&tcec_gemm_q4_workspace_bytes) gemm_workspace;
+  decltype(&tcec_gemm_q4) gemm;
+  decltype(&tcec_q8_bytes) q8_bytes;
+  decltype(&tcec_pack_q8) pack_q8;
+  decltype(&tcec_unpack_q8) unpack_q8;
+  decltype(&tcec_wgrad_q8_workspace_bytes) wgrad_workspace;
+  decltype(&tcec_wgrad_q8) wgrad;
+};
+Codes g_codes = {};
+bool g_codes_bound = false;
 
 const at::Tensor* plain_tensor(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
 bool cuda_f32(const at::Tensor& t) { return t.is_cuda() && t.scalar_type() == at::kFloat; }
@@ -206,6 +223,182 @@ PyObject* sgemm_packed(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   });
 }
 
+// A dense matrix of the current device: its type as tcec.h counts, its layout.
+struct Dense {
+  const at::Tensor* t = nullptr;
+  int type = 0, rows = 0, cols = 0;
+  Layout l{};
+};
+int type_of(at::ScalarType t) { return t == at::kFloat ? TCEC_TYPE_F32 : t == at::kHalf ? TCEC_TYPE_F16 : t == at::kBFloat16 ? TCEC_TYPE_BF16 : -1; }
+bool dense_of(const at::Tensor& t, Dense& d) {
+  if (t.dim() != 2 || !here(t) || !fits(t.size(0)) || !fits(t.size(1))) return false;
+  d.t = &t;
+  d.type = type_of(t.scalar_type());
+  d.rows = static_cast<int>(t.size(0));
+  d.cols = static_cast<int>(t.size(1));
+  return d.type >= 0 && layout_of(t, d.l);
+}
+bool dense_arg(PyObject* o, Dense& d) {
+  const at::Tensor* t = plain_tensor(o);
+  return t && dense_of(*t, d);
+}
+// The result: `given` as it is or (None) a new rows x cols matrix of `dtype` (a torch.dtype or None: the operand's).  False: not plain.
+bool result_of(PyObject* given, PyObject* dtype, const Dense& operand, int64_t rows, int64_t cols, float beta, std::optional<at::Tensor>& made,
+               Dense& c) {
+  at::ScalarType want = operand.t->scalar_type();
+  const bool named = dtype != Py_None;
+  if (named) {
+    if (!THPDtype_Check(dtype)) return false;
+    want = reinterpret_cast<THPDtype*>(dtype)->scalar_type;
+  }
+  if (given == Py_None) {
+    if (beta != 0.f || (want != operand.t->scalar_type() && want != at::kFloat)) return false;
+    made = at::empty({rows, cols}, operand.t->options().dtype(want));
+    return dense_of(*made, c);
+  }
+  return dense_arg(given, c) && c.rows == rows && c.cols == cols && (!named || c.t->scalar_type() == want) &&
+         (c.type == operand.type || c.type == TCEC_TYPE_F32);
+}
+std::optional<at::Tensor> scratch_of(size_t bytes, const at::Tensor& like) {
+  if (!bytes) return std::nullopt;
+  return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+}
+bool group_of(PyObject* o, int& group) { return extent(o, group) && (group == 32 || group == 64 || group == 128); }
+
+// gemm_q4(x, packed, n, c, group, alpha, beta, dtype)
+PyObject* gemm_q4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 8 || !g_codes_bound) Py_RETURN_NONE;
+    Dense x, c;
+    int n, group;
+    float alpha, beta;
+    const at::Tensor* packed = plain_tensor(args[1]);
+    if (!packed || !dense_arg(args[0], x) || !extent(args[2], n) || !group_of(args[4], group) || !scalar(args[5], alpha) || !scalar(args[6], beta) ||
+        !packed_here(*packed, g_codes.q4_bytes(n, x.cols, group)))
+      Py_RETURN_NONE;
+    std::optional<at::Tensor> made;
+    if (!result_of(args[3], args[7], x, x.rows, n, beta, made, c)) Py_RETURN_NONE;
+    const size_t need = g_codes.gemm_workspace(x.rows, n, x.cols, x.type);
+    const std::optional<at::Tensor> scratch = scratch_of(need, *x.t);
+    const void *px = x.t->data_ptr(), *pw = packed->data_ptr();
+    void *pc = c.t->data_ptr(), *ps = scratch ? scratch->data_ptr() : nullptr, *stream = stream_here();
+    int status;
+    {
+      const OthersRun others_run;
+      status = g_codes.gemm(x.l.order, c.l.order, x.rows, n, x.cols, alpha, px, x.l.ld, x.type, pw, group, beta, pc, c.l.ld, c.type, ps, need, stream);
+    }
+    return answer(status, args[3], made);
+  });
+}
+
+// wgrad_q8(dy, packed, k, c, alpha, beta, dtype)
+PyObject* wgrad_q8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 7 || !g_codes_bound) Py_RETURN_NONE;
+    Dense dy, c;
+    int k;
+    float alpha, beta;
+    const at::Tensor* packed = plain_tensor(args[1]);
+    if (!packed || !dense_arg(args[0], dy) || !extent(args[2], k) || !scalar(args[4], alpha) || !scalar(args[5], beta) ||
+        !packed_here(*packed, g_codes.q8_bytes(dy.rows, k)))
+      Py_RETURN_NONE;
+    std::optional<at::Tensor> made;
+    if (!result_of(args[3], args[6], dy, dy.cols, k, beta, made, c)) Py_RETURN_NONE;
+    const size_t need = g_codes.wgrad_workspace(dy.rows, dy.cols, k, dy.type);
+    const std::optional<at::Tensor> scratch = scratch_of(need, *dy.t);
+    const void *py = dy.t->data_ptr(), *px = packed->data_ptr();
+    void *pc = c.t->data_ptr(), *ps = scratch ? scratch->data_ptr() : nullptr, *stream = stream_here();
+    int status;
+    {
+      const OthersRun others_run;
+      status = g_codes.wgrad(dy.l.order, c.l.order, dy.rows, dy.cols, k, alpha, py, dy.l.ld, dy.type, px, beta, pc, c.l.ld, c.type, ps, need, stream);
+    }
+    return answer(status, args[3], made);
+  });
+}
+
+// pack_q4(w, group, scale, out) and pack_q8(x, out)
+template <bool kQ4>
+PyObject* pack_codes(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != (kQ4 ? 4 : 2) || !g_codes_bound) Py_RETURN_NONE;
+    Dense d;
+    int group = 0, scale = 0;
+    PyObject* const out = args[kQ4 ? 3 : 1];
+    const at::Tensor* given = out == Py_None ? nullptr : plain_tensor(out);
+    if (!dense_arg(args[0], d) || (!given && out != Py_None)) Py_RETURN_NONE;
+    if (kQ4) {
+      if (!group_of(args[1], group) || !THPDtype_Check(args[2])) Py_RETURN_NONE;
+      scale = type_of(reinterpret_cast<THPDtype*>(args[2])->scalar_type);
+      if (scale != TCEC_TYPE_F16 && scale != TCEC_TYPE_BF16) Py_RETURN_NONE;
+    }
+    const size_t bytes = kQ4 ? g_codes.q4_bytes(d.rows, d.cols, group) : g_codes.q8_bytes(d.rows, d.cols);
+    if (given && !packed_here(*given, bytes)) Py_RETURN_NONE;
+    std::optional<at::Tensor> made;
+    if (!given) made = at::empty({static_cast<int64_t>(bytes)}, d.t->options().dtype(at::kByte));
+    const void* src = d.t->data_ptr();
+    void *dst = (given ? *given : *made).data_ptr(), *stream = stream_here();
+    int status;
+    {
+      const OthersRun others_run;
+      status = kQ4 ? g_codes.pack_q4(d.l.order, d.rows, d.cols, src, d.l.ld, d.type, group, scale, dst, stream)
+                   : g_codes.pack_q8(d.l.order, d.rows, d.cols, src, d.l.ld, d.type, dst, stream);
+    }
+    return answer(status, out, made);
+  });
+}
+
+// unpack_q4(packed, n, k, group, dtype, out) and unpack_q8(packed, m, k, dtype, out)
+template <bool kQ4>
+PyObject* unpack_codes(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != (kQ4 ? 6 : 5) || !g_codes_bound) Py_RETURN_NONE;
+    const at::Tensor* packed = plain_tensor(args[0]);
+    int rows, cols, group = 0;
+    PyObject *const dtype = args[kQ4 ? 4 : 3], *const out = args[kQ4 ? 5 : 4];
+    if (!packed || !extent(args[1], rows) || !extent(args[2], cols) || (kQ4 && !group_of(args[3], group)) || !THPDtype_Check(dtype) ||
+        !packed_here(*packed, kQ4 ? g_codes.q4_bytes(rows, cols, group) : g_codes.q8_bytes(rows, cols)))
+      Py_RETURN_NONE;
+    std::optional<at::Tensor> made;
+    Dense d;
+    if (out == Py_None) {
+      made = at::empty({rows, cols}, packed->options().dtype(reinterpret_cast<THPDtype*>(dtype)->scalar_type));
+      if (!dense_of(*made, d)) Py_RETURN_NONE;
+    } else if (!dense_arg(out, d) || d.rows != rows || d.cols != cols) {
+      Py_RETURN_NONE;
+    }
+    const void* src = packed->data_ptr();
+    void *dst = d.t->data_ptr(), *stream = stream_here();
+    int status;
+    {
+      const OthersRun others_run;
+      status = kQ4 ? g_codes.unpack_q4(d.l.order, rows, cols, src, group, dst, d.l.ld, d.type, stream)
+                   : g_codes.unpack_q8(d.l.order, rows, cols, src, dst, d.l.ld, d.type, stream);
+    }
+    return answer(status, out, made);
+  });
+}
+
+// bind_codes(q4_bytes, pack_q4, unpack_q4, gemm_q4_workspace_bytes, gemm_q4, q8_bytes, pack_q8, unpack_q8, wgrad_q8_workspace_bytes, wgrad_q8)
+PyObject* bind_codes(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  void* p[10] = {};
+  if (n_args != 10) {
+    PyErr_SetString(PyExc_TypeError, "bind_codes() takes ten addresses");
+    return nullptr;
+  }
+  for (int i = 0; i < 10; ++i) {
+    p[i] = PyLong_AsVoidPtr(args[i]);
+    if (PyErr_Occurred()) return nullptr;
+  }
+  g_codes = {reinterpret_cast<decltype(&tcec_q4_bytes)>(p[0]),     reinterpret_cast<decltype(&tcec_pack_q4)>(p[1]),
+             reinterpret_cast<decltype(&tcec_unpack_q4)>(p[2]),    reinterpret_cast<decltype(&tcec_gemm_q4_workspace_bytes)>(p[3]),
+             reinterpret_cast<decltype(&tcec_gemm_q4)>(p[4]),      reinterpret_cast<decltype(&tcec_q8_bytes)>(p[5]),
+             reinterpret_cast<decltype(&tcec_pack_q8)>(p[6]),      reinterpret_cast<decltype(&tcec_unpack_q8)>(p[7]),
+             reinterpret_cast<decltype(&tcec_wgrad_q8_workspace_bytes)>(p[8]), reinterpret_cast<decltype(&tcec_wgrad_q8)>(p[9])};
+  g_codes_bound = true;
+  Py_RETURN_NONE;
+}
+
 // bind(sgemm, strided, pack_a, pack_b, packed, packed_bytes): addresses in the library that tcec.py has loaded
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   void* p[6] = {};
@@ -234,6 +427,13 @@ PyMethodDef kMethods[] = {
     {"pack_a", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pack<0>)), METH_FASTCALL, nullptr},
     {"pack_b", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pack<1>)), METH_FASTCALL, nullptr},
     {"sgemm_packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sgemm_packed)), METH_FASTCALL, nullptr},
+    {"bind_codes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind_codes)), METH_FASTCALL, nullptr},
+    {"gemm_q4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gemm_q4)), METH_FASTCALL, nullptr},
+    {"wgrad_q8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(wgrad_q8)), METH_FASTCALL, nullptr},
+    {"pack_q4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pack_codes<true>)), METH_FASTCALL, nullptr},
+    {"pack_q8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pack_codes<false>)), METH_FASTCALL, nullptr},
+    {"unpack_q4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(unpack_codes<true>)), METH_FASTCALL, nullptr},
+    {"unpack_q8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(unpack_codes<false>)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

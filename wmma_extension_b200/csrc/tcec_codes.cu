@@ -123,7 +123,10 @@ struct UnpackQ8 {
 };
 template <int T>
 struct StageColumns {
-  static void go(dim3 grid, cudaStream_t stream, const StageColumnsParams& p) { launch_early(stage_columns_kernel<T>, grid, 128, 0, stream, p); }
+  static void go(cudaStream_t stream, const StageColumnsParams& p) {
+    const int parts = T == kTypeF32 ? 3 : 1, tokens = static_cast<int>(ceil_div(p.eights * 8, parts));
+    launch_early(stage_columns_kernel<T>, p.blocks, (tokens * 16 + 31) / 32 * 32, 0, stream, p);
+  }
 };
 template <int T>
 struct StagePanels {
@@ -279,7 +282,7 @@ int tcec_unpack_q4(int layout_w, int n, int k, const void* packed, int group, vo
 
 size_t tcec_gemm_q4_workspace_bytes(int m, int n, int k, int type_x) {
   if (m < 0 || n < 0 || k < 0 || bad_type(type_x) || m <= 1) return 0;
-  if (streamed(m, type_x)) return static_cast<size_t>(ceil_div(k, kCodeSpan)) * eights_of(m, type_x) * 2048;
+  if (streamed(m, type_x)) return static_cast<size_t>(staged_bytes(ceil_div(k, kCodeSpan), eights_of(m, type_x)));
   return panel_bytes(m, k, type_x);
 }
 
@@ -316,10 +319,12 @@ int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, c
       sp.sum_step = dx.col_step();
       sp.tokens = m;
       sp.sum = sum;
+      sp.blocks = blocks;
       sp.eights = eights;
+      sp.group = group;
       sp.out = static_cast<uint8_t*>(workspace);
       sp.vec = layout_x == TCEC_ROW_MAJOR && dx.wide(16);
-      by_type<StageColumns>(type_x, dim3(blocks, eights), on, sp);
+      by_type<StageColumns>(type_x, on, sp);
     }
     GemvQ4Params p{};
     p.codes = static_cast<const uint8_t*>(packed);

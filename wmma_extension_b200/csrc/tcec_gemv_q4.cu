@@ -10,29 +10,45 @@ namespace tcec_host {
 namespace {
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
-// Launches for so many eights of columns and strips of rows a CTA, or (launch false) allows the kernel its shared memory.
+// As many warps divide the k of a CTA's rows as let all CTAs run at a time: a second round of them would leave SMs idle at its end, and as
+// every CTA goes through all of k it is long (16384 x 16384 with one token: ROUNDS).  So many SMs are assumed whatever the device has, so that the order of the sums
+// follows from sizes.
+int warps_of(int ctas, int warps_of_sm, int least, int most) {
+  const int warps = warps_of_sm / ceil_div(ctas, 148);
+  return warps < least ? least : warps > most ? most : warps;
+}
+// Launches for so many eights of columns and strips of rows a CTA, or (p null) allows the kernel its shared memory.
 template <int T, int G, int E, int S, bool One>
 cudaError_t one_gemv(const GemvQ4Params* p, cudaStream_t stream) {
   using Cfg = GemvQ4Cfg<T, G, E, S, One>;
-  if (!p) return cudaFuncSetAttribute(gemv_q4_kernel<T, G, E, S, One>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
-  launch_early(gemv_q4_kernel<T, G, E, S, One>, ceil_div(p->n, Cfg::ROWS), 32 * Cfg::WARPS, Cfg::SMEM_BYTES, stream, *p);
+  constexpr int kMost = One ? 16 : 8;
+  if (!p) return cudaFuncSetAttribute(gemv_q4_kernel<T, G, E, S, One>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem_bytes(kMost));
+  const int ctas = ceil_div(p->n, Cfg::ROWS), warps = warps_of(ctas, Cfg::WARPS_OF_SM, E == 1 ? 5 : 8, kMost);
+  launch_early(gemv_q4_kernel<T, G, E, S, One>, ctas, 32 * warps, Cfg::smem_bytes(warps), stream, *p);
   return cudaSuccess;
 }
 template <int T, int G>
 cudaError_t gemv_of(int eights, const GemvQ4Params& p, cudaStream_t stream) {
   if (!p.staged && p.n <= 8192) return one_gemv<T, G, 1, 1, true>(&p, stream);
   if (!p.staged) return one_gemv<T, G, 1, 2, true>(&p, stream);
+  if (eights == 1 && p.n <= 8192) return one_gemv<T, G, 1, 1, false>(&p, stream);
   if (eights == 1) return one_gemv<T, G, 1, 2, false>(&p, stream);
-  if (eights == 2) return one_gemv<T, G, 2, 2, false>(&p, stream);
-  return one_gemv<T, G, 4, 2, false>(&p, stream);
+  // An SM runs one of these CTAs at a time.  What it does for its columns is about two thirds of the work of a strip, and CTAs of two strips do
+  // it half as often; those of one strip leave fewer SMs idle at the end.
+  const bool two = ceil_div(ceil_div(p.n, 32), 148) * (2 * 3 + 2) <= ceil_div(ceil_div(p.n, 16), 148) * (3 + 2);
+  if (eights == 2) return two ? one_gemv<T, G, 2, 2, false>(&p, stream) : one_gemv<T, G, 2, 1, false>(&p, stream);
+  return two ? one_gemv<T, G, 4, 2, false>(&p, stream) : one_gemv<T, G, 4, 1, false>(&p, stream);
 }
 template <int T, int G>
 cudaError_t set_attrs() {
   cudaError_t e = one_gemv<T, G, 1, 1, true>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 1, 2, true>(nullptr, nullptr);
+  if (e == cudaSuccess) e = one_gemv<T, G, 1, 1, false>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 1, 2, false>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 2, 2, false>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 4, 2, false>(nullptr, nullptr);
+  if (e == cudaSuccess) e = one_gemv<T, G, 2, 1, false>(nullptr, nullptr);
+  if (e == cudaSuccess) e = one_gemv<T, G, 4, 1, false>(nullptr, nullptr);
   return e;
 }
 template <int T>

@@ -1,9 +1,14 @@
 // Few tokens times 4-bit weights: C[token][row] = alpha * sum_g s[row, g] sum_{i in g} (q[row][i] - z[row, g]) x[token][i] + beta C.
 //
-// Bound by the bytes of the weights, which go from global memory into the registers of mma.m16n8k16 and nowhere else: a block
-// of codes is stored in the order of those registers (tcec_codes.cuh), so a lane's two 128-bit loads are the operands of eight MMAs once
-// the codes are expanded (logic and one exact subtraction for two codes).  The tensor cores of mma.sync are plenty for up to 16 columns, and
-// unlike tcgen05.mma they take their operands from registers.
+// Bound by the bytes of the weights and by the instructions that make operands of them.  Codes go from global memory through a ring of bulk
+// copies into the registers of mma.m16n8k16, in whose order they are stored (tcec_codes.cuh).  Five logic instructions make operands of a
+// word of eight codes: a 4-bit code in the low 8 bits of a 16-bit number that is otherwise zero is that code (or 16 times it, in the upper
+// half) times the smallest number there is, 2^-24 in f16 and 2^-133 in bf16, subnormal or not; nothing is added or taken off.  The upper ones
+// have an accumulator of their own.  What the zero points take off is z times the sum of x over the group, and the power of two goes
+// into the last factor.  (Codes made to numbers first, by a magic number and a subtraction: seven logic instructions and four
+// subtractions; 16384 x 16384 37.0 us instead of WITHSUB.)  To stay among the normal FP32 numbers with such small factors, bf16 operands come times 2^100,
+// unless a token has a value of 2^27 or more among the 128 k: then times 2^6, and what is lost lies 2^-49 below the largest.  (Values
+// of 2^122 and more count as infinite.)
 //
 // Columns are tokens; an FP32 token takes three, its bf16 parts of 8 bits each, which together are exactly it.  Every product
 // of a code and a part is exact; a group's sum is made in the MMA's FP32 accumulator, then multiplied by its scale and added in
@@ -39,23 +44,34 @@ template <int kType, int kGroup, int kEights, int kStrips, bool kOne>
 struct GemvQ4Cfg {
   static constexpr int PARTS = kType == kTypeF32 ? 3 : 1;
   static constexpr int ROWS = 16 * kStrips;
-  static constexpr int WARPS = 8;
+  static constexpr int MOST_WARPS = 16;
   static constexpr int STAGE_BYTES = kStrips * q4_strip_bytes(kGroup);
-  static constexpr int STAGES = 4;                            // blocks of codes under way, of each warp
+  static constexpr int STAGES = 2;                            // blocks of codes under way, of each warp
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int X_PITCH = 320;                         // of a column in shared memory: two columns' lanes read from all banks
   static constexpr int X_BYTES = kOne ? 8 * X_PITCH : 0;
   static constexpr int SUM_PITCH = kEights * 8 + 1;
-  static constexpr int SUM_BYTES = WARPS * ROWS * SUM_PITCH * 4;
-  static constexpr int USED = WARPS * (RING_BYTES + X_BYTES);
-  static constexpr int SMEM_BYTES = (USED > SUM_BYTES ? USED : SUM_BYTES) + 128;
+  static constexpr int SUM_BYTES = ROWS * SUM_PITCH * 4;      // of a warp
+  static constexpr int WARP_BYTES = RING_BYTES + X_BYTES > SUM_BYTES ? RING_BYTES + X_BYTES : SUM_BYTES;
+  static constexpr int smem_bytes(int warps) { return warps * WARP_BYTES + 128; }
+  // Registers a thread, and with them the warps of an SM: 64 (32 warps) for one token, else what the operands of the columns need.
+  static constexpr int WARPS_OF_SM = kOne ? 32 : kEights == 1 ? 20 : kEights == 2 ? 12 : 8;
 };
 
-// The codes of a block, a strip at a time, times the operands b(panel, eight); sums folded into acc.
-template <int kType, int kGroup, int kEights, int kStrips, class B>
-__device__ __forceinline__ void multiply_block(float (&acc)[kStrips][kEights][4], const uint8_t* stage, int lane, const B& operands) {
+template <bool kF16>
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bool zero) {
+  if (zero) d[0] = d[1] = d[2] = d[3] = 0.f;
+  mma16816<kF16>(d, a0, a1, a2, a3, b0, b1);
+}
+
+// The codes of a block, a strip at a time, times the operands that take(panel, b) gives; sums folded into acc.  sum_of(q, c, j) gives the sum of x
+// over group q for this lane's two columns (j) of eight c, unit_of(c, j) what makes their products values (StagedUnit).
+template <int kType, int kGroup, int kEights, int kStrips, class Take, class SumOf, class UnitOf>
+__device__ __forceinline__ void multiply_block(float (&acc)[kStrips][kEights][4], const uint8_t* stage, int lane, const Take& take,
+                                               const SumOf& sum_of, const UnitOf& unit_of) {
   constexpr bool kF16 = kType == kTypeF16;
   constexpr int kSpans = kCodeSpan / kGroup;
+  constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
   uint4 w[kStrips][2];  // rows g and g + 8, of two panels each
 #pragma unroll
   for (int s = 0; s < kStrips; ++s)
@@ -63,57 +79,57 @@ __device__ __forceinline__ void multiply_block(float (&acc)[kStrips][kEights][4]
     for (int h = 0; h < 2; ++h) w[s][h] = *reinterpret_cast<const uint4*>(stage + s * q4_strip_bytes(kGroup) + h * 512 + lane * 16);
 #pragma unroll
   for (int q = 0; q < kSpans; ++q) {
-    float d[kStrips][kEights][4];
-    uint32_t entry[kStrips][2];
-#pragma unroll
-    for (int s = 0; s < kStrips; ++s) {
-      const uint32_t* e = reinterpret_cast<const uint32_t*>(stage + s * q4_strip_bytes(kGroup) + kStripCodeBytes) + q * 16 + (lane >> 2);
-      entry[s][0] = e[0];
-      entry[s][1] = e[8];
-#pragma unroll
-      for (int c = 0; c < kEights; ++c) d[s][c][0] = d[s][c][1] = d[s][c][2] = d[s][c][3] = 0.f;
-    }
+    float d[kStrips][kEights][2][4];  // of codes, and of 16 times codes
 #pragma unroll
     for (int panel = q * 4 / kSpans; panel < (q + 1) * 4 / kSpans; ++panel) {
+      const bool first = panel == q * 4 / kSpans;
       uint4 b[kEights];
-      operands(panel, b);
+      take(panel, b);
 #pragma unroll
       for (int s = 0; s < kStrips; ++s) {
         const uint4 pair = w[s][panel >> 1];
-        const uint4 r0 = q4_expand<kF16>(panel & 1 ? pair.z : pair.x, q4_zero<kF16>(entry[s][0] & 15u));
-        const uint4 r1 = q4_expand<kF16>(panel & 1 ? pair.w : pair.y, q4_zero<kF16>(entry[s][1] & 15u));
+        const uint32_t w0 = panel & 1 ? pair.z : pair.x, w1 = panel & 1 ? pair.w : pair.y;  // of rows g and g + 8
+        const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
 #pragma unroll
         for (int c = 0; c < kEights; ++c) {
-          mma16816<kF16>(d[s][c], r0.x, r1.x, r0.y, r1.y, b[c].x, b[c].y);
-          mma16816<kF16>(d[s][c], r0.z, r1.z, r0.w, r1.w, b[c].z, b[c].w);
+          mma16816_zero<kF16>(d[s][c][0], w0 & kLow, w1 & kLow, v0 & kLow, v1 & kLow, b[c].x, b[c].z, first);
+          mma16816_zero<kF16>(d[s][c][1], w0 & kHigh, w1 & kHigh, v0 & kHigh, v1 & kHigh, b[c].y, b[c].w, first);
         }
       }
     }
 #pragma unroll
     for (int s = 0; s < kStrips; ++s) {
-      const float s0 = __uint_as_float(entry[s][0] & ~15u), s1 = __uint_as_float(entry[s][1] & ~15u);
+      const uint32_t* e = reinterpret_cast<const uint32_t*>(stage + s * q4_strip_bytes(kGroup) + kStripCodeBytes) + q * 16 + (lane >> 2);
 #pragma unroll
-      for (int c = 0; c < kEights; ++c) {
-        acc[s][c][0] = __fmaf_rn(s0, d[s][c][0], acc[s][c][0]);
-        acc[s][c][1] = __fmaf_rn(s0, d[s][c][1], acc[s][c][1]);
-        acc[s][c][2] = __fmaf_rn(s1, d[s][c][2], acc[s][c][2]);
-        acc[s][c][3] = __fmaf_rn(s1, d[s][c][3], acc[s][c][3]);
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t entry = e[r * 8];
+        const float scale = __uint_as_float(entry & ~15u), z = 8388608.0f - __uint_as_float(0x4b000000u | (entry & 15u));  // minus the zero point
+#pragma unroll
+        for (int c = 0; c < kEights; ++c)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float unit = unit_of(c, j), sum = __fmaf_rn(0.0625f * unit, d[s][c][1][r * 2 + j], unit * d[s][c][0][r * 2 + j]);
+            acc[s][c][r * 2 + j] = __fmaf_rn(scale, __fmaf_rn(z, sum_of(q, c, j), sum), acc[s][c][r * 2 + j]);
+          }
       }
     }
   }
 }
 
 template <int kType, int kGroup, int kEights, int kStrips, bool kOne>
-__global__ void __launch_bounds__(256) gemv_q4_kernel(const GemvQ4Params p) {
+__global__ void __launch_bounds__(32 * (kOne ? 16 : 8), kEights == 1 ? 2 : 1) gemv_q4_kernel(const GemvQ4Params p) {
   using Cfg = GemvQ4Cfg<kType, kGroup, kEights, kStrips, kOne>;
   static_assert(!kOne || kEights == 1, "one token has at most three columns");
+  constexpr int kSpans = kCodeSpan / kGroup;
+  constexpr bool kF16 = kType == kTypeF16;
+  constexpr uint32_t kOnes = 0x00010001u;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[Cfg::WARPS][Cfg::STAGES];
+  __shared__ uint64_t bars[Cfg::MOST_WARPS][Cfg::STAGES];
   __shared__ uint32_t abort_flag;
   uint8_t* const smem = smem_raw + ((0u - smem_u32(smem_raw)) & 127u);
-  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   uint8_t* const ring = smem + warp * Cfg::RING_BYTES;
-  [[maybe_unused]] uint8_t* const x_shared = smem + Cfg::WARPS * Cfg::RING_BYTES + warp * Cfg::X_BYTES;
+  [[maybe_unused]] uint8_t* const x_shared = smem + warps * Cfg::RING_BYTES + warp * Cfg::X_BYTES;
   if (lane == 0) {
     for (int s = 0; s < Cfg::STAGES; ++s) mbar_init(smem_u32(&bars[warp][s]), 1);
     fence_mbar_init();
@@ -135,7 +151,7 @@ __global__ void __launch_bounds__(256) gemv_q4_kernel(const GemvQ4Params p) {
   if constexpr (kOne) wait_for_launch_before();
   if (lane == 0)
     for (int i = 0; i < Cfg::STAGES; ++i)
-      if (warp + i * Cfg::WARPS < p.blocks) fetch(warp + i * Cfg::WARPS, i);
+      if (warp + i * warps < p.blocks) fetch(warp + i * warps, i);
   if constexpr (!kOne) wait_for_launch_before();
   let_next_launch_start();
 
@@ -170,10 +186,28 @@ __global__ void __launch_bounds__(256) gemv_q4_kernel(const GemvQ4Params p) {
 #pragma unroll
     for (int c = 0; c < kEights; ++c) b_ahead[panel][c] = ld_ahead128(staged + static_cast<size_t>(kb) * (kEights * 2048) + panel * (kEights * 512) + c * 512);
   };
+  // behind the operands of all blocks: what makes products values, and the sums of x over the groups
+  [[maybe_unused]] float2 sums_ahead[kSpans][kEights], units_ahead[kEights];
+  [[maybe_unused]] const uint8_t* const staged_sums =
+      kOne ? nullptr : after_wait(p.staged) + static_cast<size_t>(p.blocks) * (kEights * 2048) + (lane & 3) * 8;
+  auto load_sums = [&](int kb) {
+    const uint8_t* at = staged_sums + static_cast<size_t>(kb) * staged_sum_bytes(kEights);
+#pragma unroll
+    for (int c = 0; c < kEights; ++c) {
+      const uint2 u = ld_operand64(at + c * 32);
+      units_ahead[c] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+#pragma unroll
+      for (int q = 0; q < kSpans; ++q) {
+        const uint2 v = ld_operand64(at + (q + 1) * kEights * 32 + c * 32);
+        sums_ahead[q][c] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+      }
+    }
+  };
   if (warp < p.blocks) {
     if constexpr (kOne) {
       load_four(warp);
     } else {
+      load_sums(warp);
 #pragma unroll
       for (int panel = 0; panel < 4; ++panel) load_operands(warp, panel);
     }
@@ -182,17 +216,30 @@ __global__ void __launch_bounds__(256) gemv_q4_kernel(const GemvQ4Params p) {
   uint32_t parity = 0;
   bool ok = true;
   int kb = warp;
-  for (; kb < p.blocks; kb += Cfg::WARPS) {
-    const int next = kb + Cfg::WARPS;
+  for (; kb < p.blocks; kb += warps) {
+    const int next = kb + warps;
+    [[maybe_unused]] float unit = StagedUnit<kType>::UNIT;
     if constexpr (kOne) {
       uint8_t* to = x_shared + lane * 8;
+      float v[4];
+      if constexpr (kType != kTypeF16) {
+        four.get(v);
+        const bool large = __any_sync(0xffffffffu, fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))) >= kLargeX);
+        const float up = large ? kUpLarge : kUpX;
+        if (large) unit = kUnitLarge;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] *= up;
+      }
       if constexpr (kType == kTypeF32) {
         uint2 hi, mid, lo;
-        split3_bf16(four.raw.x, four.raw.y, hi.x, mid.x, lo.x);
-        split3_bf16(four.raw.z, four.raw.w, hi.y, mid.y, lo.y);
+        split3_bf16(v[0], v[1], hi.x, mid.x, lo.x);
+        split3_bf16(v[2], v[3], hi.y, mid.y, lo.y);
         *reinterpret_cast<uint2*>(to) = hi;
         *reinterpret_cast<uint2*>(to + Cfg::X_PITCH) = mid;
         *reinterpret_cast<uint2*>(to + 2 * Cfg::X_PITCH) = lo;
+      } else if constexpr (kType == kTypeBf16) {
+        *reinterpret_cast<uint2*>(to) = make_uint2(__byte_perm(__float_as_uint(v[0]), __float_as_uint(v[1]), 0x7632),
+                                                   __byte_perm(__float_as_uint(v[2]), __float_as_uint(v[3]), 0x7632));
       } else {
         *reinterpret_cast<uint2*>(to) = four.raw;
       }
@@ -202,18 +249,44 @@ __global__ void __launch_bounds__(256) gemv_q4_kernel(const GemvQ4Params p) {
     if (!ok) break;
     const uint8_t* const here = ring + stage * Cfg::STAGE_BYTES;
     if constexpr (kOne) {
-      multiply_block<kType, kGroup, kEights, kStrips>(acc, here, lane, [&](int panel, uint4(&b)[kEights]) {
-        b[0] = *reinterpret_cast<const uint4*>(x_shared + (lane >> 2) * Cfg::X_PITCH + panel * 64 + (lane & 3) * 16);
-      });
-    } else {
-      multiply_block<kType, kGroup, kEights, kStrips>(acc, here, lane, [&](int panel, uint4(&b)[kEights]) {
+      // sums of x: the same products with codes that are all one
+      uint4 b[4];
+      float sums[kSpans][4];
 #pragma unroll
-        for (int c = 0; c < kEights; ++c) b[c] = b_ahead[panel][c];
-        if (next < p.blocks) load_operands(next, panel);
-      });
+      for (int panel = 0; panel < 4; ++panel) {
+        b[panel] = *reinterpret_cast<const uint4*>(x_shared + (lane >> 2) * Cfg::X_PITCH + panel * 64 + (lane & 3) * 16);
+        const int q = panel * kSpans / 4;
+        mma16816_zero<kF16>(sums[q], kOnes, kOnes, kOnes, kOnes, b[panel].x, b[panel].z, panel == q * 4 / kSpans);
+        mma16816<kF16>(sums[q], kOnes, kOnes, kOnes, kOnes, b[panel].y, b[panel].w);
+      }
+#pragma unroll
+      for (int q = 0; q < kSpans; ++q)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) sums[q][j] *= unit;
+      multiply_block<kType, kGroup, kEights, kStrips>(
+          acc, here, lane, [&](int panel, uint4(&now)[kEights]) { now[0] = b[panel]; }, [&](int q, int, int j) { return sums[q][j]; },
+          [&](int, int) { return unit; });
+    } else {
+      float2 sums[kSpans][kEights], units[kEights];
+#pragma unroll
+      for (int c = 0; c < kEights; ++c) {
+        units[c] = units_ahead[c];
+#pragma unroll
+        for (int q = 0; q < kSpans; ++q) sums[q][c] = sums_ahead[q][c];
+      }
+      if (next < p.blocks) load_sums(next);
+      multiply_block<kType, kGroup, kEights, kStrips>(
+          acc, here, lane,
+          [&](int panel, uint4(&now)[kEights]) {
+#pragma unroll
+            for (int c = 0; c < kEights; ++c) now[c] = b_ahead[panel][c];
+            if (next < p.blocks) load_operands(next, panel);
+          },
+          [&](int q, int c, int j) { return j ? sums[q][c].y : sums[q][c].x; },
+          [&](int c, int j) { return kF16 ? StagedUnit<kType>::UNIT : j ? units[c].y : units[c].x; });
     }
     __syncwarp();  // all have read the stage
-    if (lane == 0 && kb + Cfg::STAGES * Cfg::WARPS < p.blocks) fetch(kb + Cfg::STAGES * Cfg::WARPS, stage);
+    if (lane == 0 && kb + Cfg::STAGES * warps < p.blocks) fetch(kb + Cfg::STAGES * warps, stage);
     if (++stage == Cfg::STAGES) stage = 0, parity ^= 1;
   }
   if (!ok) {
@@ -221,7 +294,7 @@ __global__ void __launch_bounds__(256) gemv_q4_kernel(const GemvQ4Params p) {
     if (lane == 0) {
       atomicCAS(p.status, 0, kErrOperandWait);
       // this warp's own copies land before the CTA gives up its shared memory
-      for (int i = 0; i < Cfg::STAGES && kb < p.blocks; ++i, kb += Cfg::WARPS) {
+      for (int i = 0; i < Cfg::STAGES && kb < p.blocks; ++i, kb += warps) {
         mbar_wait_plain(smem_u32(&bars[warp][stage]), parity);
         if (++stage == Cfg::STAGES) stage = 0, parity ^= 1;
       }
@@ -239,14 +312,14 @@ __global__ void __launch_bounds__(256) gemv_q4_kernel(const GemvQ4Params p) {
       for (int j = 0; j < 4; ++j)
         sums[(warp * Cfg::ROWS + s * 16 + (lane >> 2) + (j >> 1) * 8) * Cfg::SUM_PITCH + c * 8 + (lane & 3) * 2 + (j & 1)] = acc[s][c][j];
   __syncthreads();
-  for (int i = threadIdx.x; i < Cfg::ROWS * p.tokens; i += 256) {
+  for (int i = threadIdx.x; i < Cfg::ROWS * p.tokens; i += blockDim.x) {
     const int r = i % Cfg::ROWS, token = i / Cfg::ROWS, row = row0 + r;
     if (row >= p.n) continue;
     float v = 0.f;
 #pragma unroll
     for (int part = Cfg::PARTS - 1; part >= 0; --part)  // the small ones first
-#pragma unroll
-      for (int w = 0; w < Cfg::WARPS; ++w) v += sums[(w * Cfg::ROWS + r) * Cfg::SUM_PITCH + token * Cfg::PARTS + part];
+#pragma unroll 4
+      for (int w = 0; w < warps; ++w) v += sums[(w * Cfg::ROWS + r) * Cfg::SUM_PITCH + token * Cfg::PARTS + part];
     const long long at = token * p.c_token + row * p.c_row;
     v = __fmul_rn(p.alpha, v);
     if (p.beta != 0.f) v = __fmaf_rn(p.beta, ld_element_as(p.c_type, p.c, at), v);

@@ -118,65 +118,128 @@ __global__ void __launch_bounds__(256) stage_panels_kernel(const StagePanelsPara
   let_next_launch_start();
 }
 
+// Codes that are operands as they are, in the lowest bits of 16 (tcec_gemv_q4.cuh): bf16 operands come times kUpX, so that their products stay
+// normal numbers, or times kUpLarge where a token has a value of kLargeX or more among the 128 of a block.  The unit makes the product
+// of a code 1 and such an operand the operand's value.
+constexpr float kUpX = 0x1p100f, kLargeX = 0x1p27f, kUpLarge = 0x1p6f, kUnitLarge = 0x1p127f;
+template <int kType>
+struct StagedUnit {
+  static constexpr float UNIT = kType == kTypeF16 ? 0x1p24f : 0x1p33f;
+};
+
 // Columns of mma.m16n8k16: for each block of 128 of the sum, 32 of it and eight columns, lane 4 g + t has 8 values of column g from
-// 8 t on, 16 bytes.  A column is a token, or a part of one (FP32).  One CTA a block of the sum; a thread an item and all its parts.
+// 8 t on, 16 bytes.  A column is a token, or a part of one (FP32).  Behind the operands of all blocks, for each block: the columns'
+// units, and the sums over each group (of 32: four, of 64: two) for all columns.
 struct StageColumnsParams {
   const void* src;
   long long col_step, sum_step;
-  int tokens, sum;
+  int tokens, sum, blocks;
   int eights;                 // of columns
+  int group;
   uint8_t* out;
   int vec;                    // sum_step 1 and aligned for 16 bytes
 };
+__host__ __device__ constexpr int staged_sum_bytes(int eights) { return (1 + 4) * eights * 32; }
+__host__ __device__ constexpr long long staged_bytes(long long blocks, int eights) { return blocks * (eights * 2048 + staged_sum_bytes(eights)); }
+
+// One CTA a block; 16 threads a token, eight values each.
 template <int kType>
-__global__ void __launch_bounds__(128) stage_columns_kernel(const StageColumnsParams p) {
+__global__ void __launch_bounds__(512) stage_columns_kernel(const StageColumnsParams p) {
   constexpr int kParts = kType == kTypeF32 ? 3 : 1;
   wait_for_launch_before();
   let_next_launch_start();
-  const int kb = blockIdx.x, chunk = threadIdx.x & 15, sum_here = p.sum - kb * kCodeSpan - chunk * 8;
-  uint8_t* out = p.out + static_cast<size_t>(kb) * p.eights * 2048 + (chunk >> 2) * p.eights * 512 + (chunk & 3) * 16;
-  const int columns = p.eights * 8;
-  for (int token = blockIdx.y * 8 + (threadIdx.x >> 4); token * kParts < columns; token += gridDim.y * 8) {
-    const long long at = token * p.col_step + (static_cast<long long>(kb) * kCodeSpan + chunk * 8) * p.sum_step;
-    uint4 o[kParts] = {};
-    if (token < p.tokens && sum_here > 0) {
-      if constexpr (kType == kTypeF32) {
-        const float* src = static_cast<const float*>(p.src) + at;
-        float v[8];
-        if (p.vec && sum_here >= 8) {
-          const float4 a = ld_operand(reinterpret_cast<const float4*>(src)), b = ld_operand(reinterpret_cast<const float4*>(src + 4));
-          v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = ld_operand(src + min(j, sum_here - 1) * p.sum_step);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j >= sum_here) v[j] = 0.f;
-        }
-        uint32_t w[3][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) split3_bf16(v[2 * j], v[2 * j + 1], w[0][j], w[1][j], w[2][j]);
-#pragma unroll
-        for (int q = 0; q < kParts; ++q) o[q] = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+  const int kb = blockIdx.x, chunk = threadIdx.x & 15, token = threadIdx.x >> 4, sum_here = p.sum - kb * kCodeSpan - chunk * 8;
+  const long long at = token * p.col_step + (static_cast<long long>(kb) * kCodeSpan + chunk * 8) * p.sum_step;
+  float v[8] = {};
+  if (token < p.tokens && sum_here > 0) {
+    if constexpr (kType == kTypeF32) {
+      const float* src = static_cast<const float*>(p.src) + at;
+      if (p.vec && sum_here >= 8) {
+        const float4 a = ld_operand(reinterpret_cast<const float4*>(src)), b = ld_operand(reinterpret_cast<const float4*>(src + 4));
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
       } else {
-        const uint16_t* src = static_cast<const uint16_t*>(p.src) + at;
-        if (p.vec && sum_here >= 8) {
-          o[0] = ld_operand128(src);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = ld_operand(src + min(j, sum_here - 1) * p.sum_step);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j >= sum_here) v[j] = 0.f;
+      }
+    } else {
+      const uint16_t* src = static_cast<const uint16_t*>(p.src) + at;
+      uint32_t w[4];
+      if (p.vec && sum_here >= 8) {
+        const uint4 o = ld_operand128(src);
+        w[0] = o.x, w[1] = o.y, w[2] = o.z, w[3] = o.w;
+      } else {
+        uint32_t h[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = ld_operand16(src + min(j, sum_here - 1) * p.sum_step);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j >= sum_here) h[j] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = h[2 * j] | h[2 * j + 1] << 16;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (kType == kTypeF16) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+          v[2 * j] = f.x, v[2 * j + 1] = f.y;
         } else {
-          uint32_t w[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = ld_operand16(src + min(j, sum_here - 1) * p.sum_step);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j >= sum_here) w[j] = 0;
-          o[0] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+          v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
         }
       }
     }
+  }
+  bool large = false;
+  if constexpr (kType != kTypeF16) {
+    float most = 0.f;
 #pragma unroll
-    for (int q = 0; q < kParts; ++q) {
-      const int col = token * kParts + q;
-      if (col < columns) *reinterpret_cast<uint4*>(out + (col >> 3) * 512 + (col & 7) * 64) = o[q];
+    for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+    large = most >= kLargeX;
+    const float up = large ? kUpLarge : kUpX;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= up;
+  }
+  uint32_t part[kParts][4];
+  if constexpr (kType == kTypeF32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) split3_bf16(v[2 * j], v[2 * j + 1], part[0][j], part[1][j], part[2][j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (kType == kTypeF16) {
+        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        part[0][j] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        part[0][j] = __byte_perm(__float_as_uint(v[2 * j]), __float_as_uint(v[2 * j + 1]), 0x7632);
+      }
+    }
+  }
+  const int columns = p.eights * 8;
+  uint8_t* out = p.out + static_cast<size_t>(kb) * p.eights * 2048 + (chunk >> 2) * p.eights * 512 + (chunk & 3) * 16;
+  uint8_t* sums = p.out + static_cast<size_t>(p.blocks) * p.eights * 2048 + static_cast<size_t>(kb) * staged_sum_bytes(p.eights);
+#pragma unroll
+  for (int q = 0; q < kParts; ++q) {
+    const int col = token * kParts + q;
+    if (col < columns) *reinterpret_cast<uint4*>(out + (col >> 3) * 512 + (col & 7) * 64) = make_uint4(part[q][0], part[q][1], part[q][2], part[q][3]);
+    float sum = 0.f;
+    if constexpr (kType == kTypeF16) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += v[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += __uint_as_float(part[q][j] << 16) + __uint_as_float(part[q][j] & 0xffff0000u);
+    }
+    for (int d = 1; d < p.group / 8; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const int of_group = p.group / 8;  // threads
+    if (col < columns) {
+      if ((chunk & (of_group - 1)) == 0)
+        *reinterpret_cast<float*>(sums + ((1 + chunk / of_group) * columns + col) * 4) =
+            kType == kTypeF16 ? sum : sum * (large ? 1.0f / kUpLarge : 1.0f / kUpX);
+      if (chunk == 0) *reinterpret_cast<float*>(sums + col * 4) = large ? kUnitLarge : StagedUnit<kType>::UNIT;
     }
   }
 }

@@ -194,6 +194,10 @@ def load() -> ctypes.CDLL:
         _binding.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
             lib.tcec_sgemm, lib.tcec_sgemm_strided_batched, lib.tcec_pack_a, lib.tcec_pack_b, lib.tcec_sgemm_packed,
             lib.tcec_packed_bytes)))
+        if hasattr(_binding, "bind_codes"):
+            _binding.bind_codes(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+                lib.tcec_q4_bytes, lib.tcec_pack_q4, lib.tcec_unpack_q4, lib.tcec_gemm_q4_workspace_bytes, lib.tcec_gemm_q4, lib.tcec_q8_bytes,
+                lib.tcec_pack_q8, lib.tcec_unpack_q8, lib.tcec_wgrad_q8_workspace_bytes, lib.tcec_wgrad_q8)))
     _lib = lib  # last: other threads go into the binding as soon as they see it
     return lib
 
@@ -555,6 +559,10 @@ def pack_q4(w: torch.Tensor, group: int = 128, scale: torch.dtype = torch.float1
     Returns the uint8 buffer that gemm_q4 takes.  Every value is brought to the nearest of its group's 16 steps
     (``tcec_pack_q4``); unpack_q4 gives the values that the codes stand for.
     """
+    if _binding is not None and _lib is not None:
+        done = _binding.pack_q4(w, group, scale, out)
+        if done is not None:
+            return _answer(done, "tcec_pack_q4")
     kind = _dense_type(w, "w")
     if scale not in (torch.float16, torch.bfloat16):
         raise ValueError("scale must be float16 or bfloat16")
@@ -605,6 +613,10 @@ def pack_q4_codes(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[tor
 def unpack_q4(packed: torch.Tensor, n: int, k: int, group: int = 128, dtype: torch.dtype = torch.float32,
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The weights (n x k) that a packed buffer stands for, rounded to the result's type."""
+    if _binding is not None and _lib is not None:
+        done = _binding.unpack_q4(packed, n, k, group, dtype, out)
+        if done is not None:
+            return _answer(done, "tcec_unpack_q4")
     need = q4_bytes(n, k, group)
     _require_bytes(packed, need, "packed weights of this size")
     if out is None:
@@ -626,6 +638,10 @@ def gemm_q4(x: torch.Tensor, packed: torch.Tensor, n: int, c: Optional[torch.Ten
 
     From one token to a whole prompt.  The result is of X's type, or of ``dtype`` (X's or float32).
     """
+    if _binding is not None and _lib is not None:
+        done = _binding.gemm_q4(x, packed, n, c, group, alpha, beta, dtype)
+        if done is not None:
+            return _answer(done, "tcec_gemm_q4")
     kind = _dense_type(x, "x")
     m, k = x.shape
     need = q4_bytes(n, k, group)
@@ -652,6 +668,10 @@ def q8_bytes(m: int, k: int) -> int:
 
 def pack_q8(x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Activations x (m tokens x k features) in 8 bits, with a scale for every 128 tokens of a feature, to be kept for wgrad_q8."""
+    if _binding is not None and _lib is not None:
+        done = _binding.pack_q8(x, out)
+        if done is not None:
+            return _answer(done, "tcec_pack_q8")
     kind = _dense_type(x, "x")
     m, k = x.shape
     need = q8_bytes(m, k)
@@ -668,6 +688,10 @@ def pack_q8(x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor
 
 def unpack_q8(packed: torch.Tensor, m: int, k: int, dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The activations (m x k) that a packed buffer stands for, rounded to the result's type."""
+    if _binding is not None and _lib is not None:
+        done = _binding.unpack_q8(packed, m, k, dtype, out)
+        if done is not None:
+            return _answer(done, "tcec_unpack_q8")
     _require_bytes(packed, q8_bytes(m, k), "packed activations of this size")
     if out is None:
         out = torch.empty((m, k), dtype=dtype, device=packed.device)
@@ -689,6 +713,10 @@ def wgrad_q8(dy: torch.Tensor, packed: torch.Tensor, k: int, c: Optional[torch.T
 
     The result is of dY's type, or of ``dtype`` (dY's or float32).
     """
+    if _binding is not None and _lib is not None:
+        done = _binding.wgrad_q8(dy, packed, k, c, alpha, beta, dtype)
+        if done is not None:
+            return _answer(done, "tcec_wgrad_q8")
     kind = _dense_type(dy, "dy")
     m, n = dy.shape
     _require_bytes(packed, q8_bytes(m, k), "packed activations of this size")
