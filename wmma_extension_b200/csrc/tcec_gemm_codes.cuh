@@ -73,6 +73,7 @@ struct GemmCodesCfg {
   static constexpr bool PAIR = BN == 256;                     // 256 x 256 tiles on two SMs
   static constexpr int GROUPS = Q8 ? 1 : kSpans;
   static constexpr int CONVERTERS = 8, FOLDERS = 8;           // warps
+  static constexpr int TEAMS = BN == 64 && !Q8 ? 4 : PAIR && kSpans != 1 ? 1 : 2, TEAM = CONVERTERS / TEAMS;  // of converters: each takes a block in turn, with TEAM warps
   static constexpr int THREADS = 32 * (4 + CONVERTERS + FOLDERS);
   static constexpr int CODE_BYTES = Q8 ? kQ8CodeBytes : kQ4CodeBytes;
   static constexpr int BLOCK_BYTES = CODE_BYTES + kEntryBytes * GROUPS;
@@ -80,18 +81,19 @@ struct GemmCodesCfg {
   // multiple of 128, so that lanes with rows g, g + 1 of four chunks write to all banks at once.
   static constexpr int CHUNK_BYTES = 128 * 16 + 32;
   static constexpr int A_BYTES = 16 * CHUNK_BYTES;
-  static constexpr int A_STAGES = 3;
+  static constexpr int A_STAGES = BN == 64 ? 4 : 3;
   static constexpr int BC = PAIR ? 128 : BN;                  // columns of the dense operand that a CTA brings in
   static constexpr int B_HALF = BC * 128;                     // 64 of the sum, one part
-  static constexpr int B_STAGES = BN == 64 || (PAIR && kSpans == 1) ? 3 : 2;  // of two halves, which are filled and given back one by one
-  static constexpr int CODE_STAGES = PAIR && kSpans == 1 ? 2 : 3;
+  static constexpr int B_STAGES = (BN == 64 && kSpans < 4) || (PAIR && kSpans == 1) ? 3 : 2;  // of two halves, which are filled and given back one by one
+  static constexpr int CODE_STAGES = PAIR ? (kSpans == 1 ? 2 : 3) : Q8 ? 2 : 4;
   static constexpr int ACCS = BN == 256 ? 2 : 4;              // accumulators
-  static constexpr int SCALE_SLOTS = ACCS + 5;                // blocks; see the converters
+  static constexpr int SCALE_SLOTS = ACCS + A_STAGES + 1;     // blocks; see the converters
   static constexpr int B_OFFSET = 0;
   static constexpr int A_OFFSET = B_STAGES * 2 * B_HALF;
   static constexpr int CODE_OFFSET = A_OFFSET + A_STAGES * A_BYTES;
   static constexpr int SCALE_OFFSET = CODE_OFFSET + CODE_STAGES * BLOCK_BYTES;
   static constexpr int SMEM_BYTES = SCALE_OFFSET + SCALE_SLOTS * GROUPS * 512 + 1024;
+  static_assert(TEAMS <= A_STAGES && CODE_STAGES % TEAMS == 0, "a team may not wait for a phase that is two ahead");
   static_assert(SMEM_BYTES <= 232448 - 512, "dynamic + static shared memory exceed an SM");
   static_assert(PAIR || A_OFFSET >= 128 * BN * 4, "partial results go where the dense operand was");
   static constexpr int TMEM_COLS = ACCS * BN;
@@ -141,39 +143,48 @@ __device__ __forceinline__ bool mbar_wait_lanes(uint32_t bar, uint32_t parity, v
   return __all_sync(0xffffffffu, ok);
 }
 
-// Expands the codes of one block (shared memory) to 16-bit operands: an eighth of it, warp by warp.
-template <bool kF16, int kSpans>
-struct Converter {  // 4 bits: a strip of 16 rows a warp, lane 4 g + t has rows g and g + 8
-  static __device__ __forceinline__ void expand(const uint8_t* block, uint8_t* out, int warp, int lane) {
-    constexpr int kChunk = GemmCodesCfg<128, kSpans>::CHUNK_BYTES;
-    const uint8_t* codes = block + warp * q4_strip_bytes(128 / kSpans) + lane * 16;
-    const uint32_t* entries = reinterpret_cast<const uint32_t*>(block + warp * q4_strip_bytes(128 / kSpans) + kStripCodeBytes) + (lane >> 2);
-    uint8_t* to = out + (lane & 3) * kChunk + warp * 256 + (lane >> 2) * 16;
-    const uint4 w[2] = {*reinterpret_cast<const uint4*>(codes), *reinterpret_cast<const uint4*>(codes + 512)};
+// Expands a part of the codes of one block (shared memory) to 16-bit operands: part `index` of kParts, a warp.
+template <bool kF16, int kSpans, int kParts>
+struct Converter {  // 4 bits: strips of 16 rows, lane 4 g + t has rows g and g + 8
+  static __device__ __forceinline__ void expand(const uint8_t* block, uint8_t* out, int index, int lane) {
+    constexpr int kChunk = GemmCodesCfg<128, kSpans>::CHUNK_BYTES, kStrips = 8 / kParts, kStripBytes = q4_strip_bytes(128 / kSpans);
+    const uint8_t* codes = block + index * kStrips * kStripBytes + lane * 16;
+    const uint32_t* entries = reinterpret_cast<const uint32_t*>(block + index * kStrips * kStripBytes + kStripCodeBytes) + (lane >> 2);
+    uint8_t* to = out + (lane & 3) * kChunk + index * kStrips * 256 + (lane >> 2) * 16;
 #pragma unroll
-    for (int q = 0; q < kSpans; ++q) {
-      const uint32_t zero0 = q4_zero<kF16>(entries[q * 16] & 15u), zero1 = q4_zero<kF16>(entries[q * 16 + 8] & 15u);
+    for (int s = 0; s < kStrips; ++s) {
+      const uint4 w[2] = {*reinterpret_cast<const uint4*>(codes + s * kStripBytes), *reinterpret_cast<const uint4*>(codes + s * kStripBytes + 512)};
 #pragma unroll
-      for (int panel = q * 4 / kSpans; panel < (q + 1) * 4 / kSpans; ++panel) {
-        const uint4 pair = w[panel >> 1];
-        uint8_t* at = to + panel * 4 * kChunk;
-        *reinterpret_cast<uint4*>(at) = q4_expand<kF16>(panel & 1 ? pair.z : pair.x, zero0);
-        *reinterpret_cast<uint4*>(at + 128) = q4_expand<kF16>(panel & 1 ? pair.w : pair.y, zero1);
+      for (int q = 0; q < kSpans; ++q) {
+        const uint32_t zero0 = q4_zero<kF16>(entries[s * (kStripBytes / 4) + q * 16] & 15u);
+        const uint32_t zero1 = q4_zero<kF16>(entries[s * (kStripBytes / 4) + q * 16 + 8] & 15u);
+#pragma unroll
+        for (int panel = q * 4 / kSpans; panel < (q + 1) * 4 / kSpans; ++panel) {
+          const uint4 pair = w[panel >> 1];
+          uint8_t* at = to + panel * 4 * kChunk + s * 256;
+          *reinterpret_cast<uint4*>(at) = q4_expand<kF16>(panel & 1 ? pair.z : pair.x, zero0);
+          *reinterpret_cast<uint4*>(at + 128) = q4_expand<kF16>(panel & 1 ? pair.w : pair.y, zero1);
+        }
       }
     }
   }
 };
-template <bool kF16>
-struct Converter<kF16, 0> {  // 8 bits: 32 rows, a lane each, and half of the sum a warp
-  static __device__ __forceinline__ void expand(const uint8_t* block, uint8_t* out, int warp, int lane) {
+template <bool kF16, int kParts>
+struct Converter<kF16, 0, kParts> {  // 8 bits: 32 rows at a time, a lane each; of eight warps two share them, half of the sum each
+  static __device__ __forceinline__ void expand(const uint8_t* block, uint8_t* out, int index, int lane) {
     constexpr int kChunk = GemmCodesCfg<128, 0>::CHUNK_BYTES;
-    const int at = ((warp & 3) * 32 + lane) * 16;  // of this row, among 16 tokens of codes and among 8 of operands
-    const int half = warp >> 2;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const uint4 v = *reinterpret_cast<const uint4*>(block + (half * 4 + c) * 2048 + at);
-      *reinterpret_cast<uint4*>(out + (half * 8 + 2 * c) * kChunk + at) = q8_expand<kF16>(v.x, v.y);
-      *reinterpret_cast<uint4*>(out + (half * 8 + 2 * c + 1) * kChunk + at) = q8_expand<kF16>(v.z, v.w);
+    for (int r = 0; r < (kParts < 4 ? 4 / kParts : 1); ++r) {
+      const int rows = kParts < 4 ? index * (4 / kParts) + r : index & 3, half = kParts == 8 ? index >> 2 : 0;
+      const int at = (rows * 32 + lane) * 16;  // of this row, among 16 tokens of codes and among 8 of operands
+#pragma unroll
+      for (int c = half * 4; c < half * 4 + (kParts == 8 ? 4 : 8); c += 2) {
+        const uint4 v = *reinterpret_cast<const uint4*>(block + c * 2048 + at), w = *reinterpret_cast<const uint4*>(block + (c + 1) * 2048 + at);
+        *reinterpret_cast<uint4*>(out + (2 * c) * kChunk + at) = q8_expand<kF16>(v.x, v.y);
+        *reinterpret_cast<uint4*>(out + (2 * c + 1) * kChunk + at) = q8_expand<kF16>(v.z, v.w);
+        *reinterpret_cast<uint4*>(out + (2 * c + 2) * kChunk + at) = q8_expand<kF16>(w.x, w.y);
+        *reinterpret_cast<uint4*>(out + (2 * c + 3) * kChunk + at) = q8_expand<kF16>(w.z, w.w);
+      }
     }
   }
 };
@@ -220,10 +231,10 @@ __global__ void __launch_bounds__(GemmCodesCfg<BN, kSpans>::THREADS, 1) tcec_gem
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::CODE_STAGES; ++s) {
       mbar_init(smem_u32(&bar_code_full[s]), 1);
-      mbar_init(smem_u32(&bar_code_empty[s]), Cfg::CONVERTERS);
+      mbar_init(smem_u32(&bar_code_empty[s]), Cfg::TEAM);
     }
     for (int s = 0; s < Cfg::A_STAGES; ++s) {
-      mbar_init(smem_u32(&bar_a_full[s]), Cfg::CONVERTERS + (kPair && leader));  // in a leader the peer's relay too
+      mbar_init(smem_u32(&bar_a_full[s]), Cfg::TEAM + (kPair && leader));  // in a leader the peer's relay too
       mbar_init(smem_u32(&bar_a_empty[s]), 1);
     }
     for (int s = 0; s < Cfg::B_STAGES; ++s) {
@@ -415,36 +426,39 @@ __global__ void __launch_bounds__(GemmCodesCfg<BN, kSpans>::THREADS, 1) tcec_gem
   } else if (warp < 4 + Cfg::CONVERTERS) {
     // ------------------------------------------------------------ codes to operands
     setmaxnreg_dec<Cfg::REGS_CONVERT>();
-    uint32_t cs = 0, cph = 0, as = 0, aph = 0, slot = 0;
-    const int t = threadIdx.x - 128;
+    // The teams take the blocks in turn, so that one waits and passes its block on while another expands.  A team that waits for a phase must
+    // know that the one before is over, as the next but one has the same parity.  A stage of codes is always the same team's, and of the stages of
+    // operands, whose MMAs come in order, there are no fewer than teams.
+    const int team = (warp - 4) / Cfg::TEAM, index = (warp - 4) % Cfg::TEAM;
+    const int total = first_tile < ntiles ? ((ntiles - first_tile + stride - 1) / stride) * nkb : 0;  // blocks, of all tiles
+    uint32_t cs = team, cph = 0, as = team, aph = 0, slot = team;
     bool ok = true;
-    for (int tile = first_tile; tile < ntiles && ok; tile += stride)
-      for (int kb = 0; kb < nkb; ++kb) {
-        if (!mbar_wait_lanes(smem_u32(&bar_code_full[cs]), cph, abortp) || !mbar_wait_lanes(smem_u32(&bar_a_empty[as]), aph ^ 1, abortp)) {
-          ok = false;
-          break;
-        }
-        const uint8_t* block = smem_gen + Cfg::CODE_OFFSET + cs * Cfg::BLOCK_BYTES;
-        // The scales, for those who come to them when the products are made.  The stage just waited for says that the MMAs of A_STAGES
-        // blocks before are done, for which all but the last ACCS accumulators had been folded: a slot is written again later than that.
-        if (warp < 8) {
-          float* scales = reinterpret_cast<float*>(smem_gen + Cfg::SCALE_OFFSET) + slot * (kGroups * 128) + t;
-#pragma unroll
-          for (int g = 0; g < kGroups; ++g)
-            if constexpr (Cfg::Q8) scales[0] = reinterpret_cast<const float*>(block + Cfg::CODE_BYTES)[t];
-            else scales[g * 128] = __uint_as_float(reinterpret_cast<const uint32_t*>(block)[q4_entry_word<128 / (Cfg::Q8 ? 1 : kSpans)>(t, g)] & ~15u);
-        }
-        Converter<kF16, kSpans>::expand(block, smem_gen + Cfg::A_OFFSET + as * Cfg::A_BYTES, warp - 4, lane);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(smem_u32(&bar_a_full[as]));
-          mbar_arrive(smem_u32(&bar_code_empty[cs]));
-        }
-        if (++cs == Cfg::CODE_STAGES) cs = 0, cph ^= 1;
-        if (++as == Cfg::A_STAGES) as = 0, aph ^= 1;
-        if (++slot == Cfg::SCALE_SLOTS) slot = 0;
+    for (int i = team; i < total; i += Cfg::TEAMS) {
+      if (!mbar_wait_lanes(smem_u32(&bar_code_full[cs]), cph, abortp) || !mbar_wait_lanes(smem_u32(&bar_a_empty[as]), aph ^ 1, abortp)) {
+        ok = false;
+        break;
       }
+      const uint8_t* block = smem_gen + Cfg::CODE_OFFSET + cs * Cfg::BLOCK_BYTES;
+      // The scales, for those who come to them when the products are made.  The stage just waited for says that the MMAs of A_STAGES
+      // blocks before are done, for which all but the last ACCS accumulators had been folded: a slot is written again later than that.
+      float* scales = reinterpret_cast<float*>(smem_gen + Cfg::SCALE_OFFSET) + slot * (kGroups * 128);
+#pragma unroll
+      for (int t = index * 32 + lane; t < 128; t += Cfg::TEAM * 32)
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+          if constexpr (Cfg::Q8) scales[t] = reinterpret_cast<const float*>(block + Cfg::CODE_BYTES)[t];
+          else scales[g * 128 + t] = __uint_as_float(reinterpret_cast<const uint32_t*>(block)[q4_entry_word<128 / (Cfg::Q8 ? 1 : kSpans)>(t, g)] & ~15u);
+      Converter<kF16, kSpans, Cfg::TEAM>::expand(block, smem_gen + Cfg::A_OFFSET + as * Cfg::A_BYTES, index, lane);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(smem_u32(&bar_a_full[as]));
+        mbar_arrive(smem_u32(&bar_code_empty[cs]));
+      }
+      if ((cs += Cfg::TEAMS) >= Cfg::CODE_STAGES) cs -= Cfg::CODE_STAGES, cph ^= 1;
+      if ((as += Cfg::TEAMS) >= Cfg::A_STAGES) as -= Cfg::A_STAGES, aph ^= 1;
+      if ((slot += Cfg::TEAMS) >= Cfg::SCALE_SLOTS) slot -= Cfg::SCALE_SLOTS;
+    }
     if (!ok && lane == 0) give_up(kErrOperandWait);
   } else {
     // ------------------------------------------------------------ scales
