@@ -189,6 +189,34 @@ struct Converter<kF16, 0, kParts> {  // 8 bits: 32 rows at a time, a lane each; 
   }
 };
 
+// Columns of one row of C, `step` bytes apart: alpha * acc + beta * C.  Each of these loops is gone through once a tile, and what it costs is to fetch
+// its instructions (element by element with the type, the stride and beta looked at each time, a tile of 64 columns took 1.7 us to store), so
+// the common one is kept short.
+template <int kType, int N>
+__device__ __forceinline__ void store_columns(const float (&acc)[N], uint8_t* at, long long step, int cols, float alpha, float beta) {
+  typedef typename Element<kType>::type T;
+  if (beta == 0.f && cols >= N) {
+#pragma unroll
+    for (int i = 0; i < N; ++i, at += step) *reinterpret_cast<T*>(at) = Element<kType>::put(__fmul_rn(alpha, acc[i]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i, at += step)
+      if (i < cols) {
+        float v = __fmul_rn(alpha, acc[i]);
+        if (beta != 0.f) v = __fmaf_rn(beta, Element<kType>::get(*reinterpret_cast<T*>(at)), v);
+        *reinterpret_cast<T*>(at) = Element<kType>::put(v);
+      }
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_columns_as(const GemmCodesParams& p, const float (&acc)[N], long long row, long long col, int cols) {
+  const int size = p.c_type == kTypeF32 ? 4 : 2;
+  uint8_t* const at = static_cast<uint8_t*>(p.c) + (row * p.c_row + col * p.c_col) * size;
+  if (p.c_type == kTypeF32) store_columns<kTypeF32>(acc, at, p.c_col * size, cols, p.alpha, p.beta);
+  else if (p.c_type == kTypeF16) store_columns<kTypeF16>(acc, at, p.c_col * size, cols, p.alpha, p.beta);
+  else store_columns<kTypeBf16>(acc, at, p.c_col * size, cols, p.alpha, p.beta);
+}
+
 // Which rows and columns a tile is.  Sixteen rows of tiles at a time go through all columns: what is on at a time shares its operands.
 struct CodeTile {
   int row, col;
@@ -228,26 +256,24 @@ __global__ void __launch_bounds__(GemmCodesCfg<BN, kSpans>::THREADS, 1) tcec_gem
   const int nkb = kb_end - kb_first;
   auto row_tile = [&](const CodeTile& t) { return kPair ? t.row * 2 + rank : t.row; };
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < Cfg::CODE_STAGES; ++s) {
-      mbar_init(smem_u32(&bar_code_full[s]), 1);
-      mbar_init(smem_u32(&bar_code_empty[s]), Cfg::TEAM);
+  if (warp == 0) {  // a barrier or two a lane
+    if (lane < Cfg::CODE_STAGES) {
+      mbar_init(smem_u32(&bar_code_full[lane]), 1);
+      mbar_init(smem_u32(&bar_code_empty[lane]), Cfg::TEAM);
+    } else if (lane >= 8 && lane < 8 + Cfg::A_STAGES) {
+      mbar_init(smem_u32(&bar_a_full[lane - 8]), Cfg::TEAM + (kPair && leader));  // in a leader the peer's relay too
+      mbar_init(smem_u32(&bar_a_empty[lane - 8]), 1);
+    } else if (lane >= 16 && lane < 16 + Cfg::B_STAGES) {
+      mbar_init(smem_u32(&bar_b_full[lane - 16]), 2 + (kPair && leader));
+      mbar_init(smem_u32(&bar_b_empty[2 * (lane - 16)]), 1);
+      mbar_init(smem_u32(&bar_b_empty[2 * (lane - 16) + 1]), 1);
+    } else if (lane >= 24 && lane < 24 + Cfg::ACCS) {
+      mbar_init(smem_u32(&bar_acc_full[lane - 24]), 1);
+      mbar_init(smem_u32(&bar_acc_free[lane - 24]), (kPair ? 2 : 1) * Cfg::FOLDERS);  // of a pair the leader's is used
+    } else if (lane == 31) {
+      mbar_init(smem_u32(&bar_drain[0]), 1);
+      abort_flag = 0;
     }
-    for (int s = 0; s < Cfg::A_STAGES; ++s) {
-      mbar_init(smem_u32(&bar_a_full[s]), Cfg::TEAM + (kPair && leader));  // in a leader the peer's relay too
-      mbar_init(smem_u32(&bar_a_empty[s]), 1);
-    }
-    for (int s = 0; s < Cfg::B_STAGES; ++s) {
-      mbar_init(smem_u32(&bar_b_full[s]), 2 + (kPair && leader));
-      mbar_init(smem_u32(&bar_b_empty[2 * s]), 1);
-      mbar_init(smem_u32(&bar_b_empty[2 * s + 1]), 1);
-    }
-    for (int i = 0; i < Cfg::ACCS; ++i) {
-      mbar_init(smem_u32(&bar_acc_full[i]), 1);
-      mbar_init(smem_u32(&bar_acc_free[i]), (kPair ? 2 : 1) * Cfg::FOLDERS);  // of a pair the leader's is used
-    }
-    mbar_init(smem_u32(&bar_drain[0]), 1);
-    abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -512,43 +538,38 @@ __global__ void __launch_bounds__(GemmCodesCfg<BN, kSpans>::THREADS, 1) tcec_gem
         if (++slot == Cfg::SCALE_SLOTS) slot = 0;
       }
       const int row = row_tile(ti) * 128 + r;
-      if (shares == 1 && ok && row < p.rows) {
-        const long long base = row * p.c_row + col0 * p.c_col;
-#pragma unroll
-        for (int i = 0; i < Cfg::NC; ++i)
-          if (i < cols) {
-            const long long at = base + i * p.c_col;
-            float v = __fmul_rn(p.alpha, acc[i]);
-            if (p.beta != 0.f) v = __fmaf_rn(p.beta, ld_element_as(p.c_type, p.c, at), v);
-            st_element_as(p.c_type, p.c, at, v);
-          }
-      }
+      if (shares == 1 && ok && row < p.rows && cols > 0) store_columns_as(p, acc, row, col0, cols);
     }
     if (!ok && lane == 0) give_up(kErrEpilogueWait);
     if constexpr (!kPair) {
       if (shares > 1) {  // then a cluster has one tile
         cluster_sync_all();  // nobody reads operands any more where the partial results go
         const CodeTile ti = code_tile(first_tile, tile_rows, p.col_tiles);
-        const int per = BN / shares;  // columns that a CTA adds up and stores
+        // The columns go to the CTAs in turn, four at a time: what a CTA adds up is the fours rank, rank + shares, ...
+        const uint32_t mine = smem_base + Cfg::B_OFFSET + r * 16;
 #pragma unroll
-        for (int i = 0; i < Cfg::NC; ++i) {
-          const int col = first_col + i, to = col / per;
-          const uint32_t at = smem_base + Cfg::B_OFFSET + ((rank * per + col - to * per) * 128 + r) * 4;
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(at, to)), "f"(acc[i]) : "memory");
+        for (int i = 0; i < Cfg::NC / 4; ++i) {
+          const uint32_t four = (first_col >> 2) + i;
+          const uint32_t at = mine + (rank * (BN / 4 / shares) + four / shares) * 2048;
+          st_cluster_v4(map_to_cta(at, four & (shares - 1)), acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
         }
         cluster_sync_all();
         const int row = ti.row * 128 + r;
         if (row < p.rows && !*abortp) {
-          const float* parts = reinterpret_cast<const float*>(smem_gen + Cfg::B_OFFSET) + r;
-          for (int i = fw >> 2; i < per; i += 2) {
-            const int col = ti.col * BN + rank * per + i;
+          const uint32_t fours = BN / 4 / shares;
+#pragma unroll 1
+          for (uint32_t f = fw >> 2; f < fours; f += 2) {
+            const int col = ti.col * BN + (f * shares + rank) * 4;
             if (col >= p.cols) break;
-            float v = parts[i * 128];
-            for (int s = 1; s < shares; ++s) v += parts[(s * per + i) * 128];
-            const long long at = row * p.c_row + col * p.c_col;
-            v = __fmul_rn(p.alpha, v);
-            if (p.beta != 0.f) v = __fmaf_rn(p.beta, ld_element_as(p.c_type, p.c, at), v);
-            st_element_as(p.c_type, p.c, at, v);
+            float4 v[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+              if (s < shares) v[s] = ld_shared_v4(mine + (s * fours + f) * 2048);
+            float sum[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+            for (int s = 1; s < 8; ++s)
+              if (s < shares) sum[0] += v[s].x, sum[1] += v[s].y, sum[2] += v[s].z, sum[3] += v[s].w;
+            store_columns_as(p, sum, row, col, p.cols - col);
           }
         }
       }
