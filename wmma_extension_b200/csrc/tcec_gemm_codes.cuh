@@ -151,7 +151,7 @@ struct Converter {  // 4 bits: strips of 16 rows, lane 4 g + t has rows g and g 
     const uint8_t* codes = block + index * kStrips * kStripBytes + lane * 16;
     const uint32_t* entries = reinterpret_cast<const uint32_t*>(block + index * kStrips * kStripBytes + kStripCodeBytes) + (lane >> 2);
     uint8_t* to = out + (lane & 3) * kChunk + index * kStrips * 256 + (lane >> 2) * 16;
-#pragma unroll
+#pragma unroll 1
     for (int s = 0; s < kStrips; ++s) {
       const uint4 w[2] = {*reinterpret_cast<const uint4*>(codes + s * kStripBytes), *reinterpret_cast<const uint4*>(codes + s * kStripBytes + 512)};
 #pragma unroll
@@ -177,7 +177,7 @@ struct Converter<kF16, 0, kParts> {  // 8 bits: 32 rows at a time, a lane each; 
     for (int r = 0; r < (kParts < 4 ? 4 / kParts : 1); ++r) {
       const int rows = kParts < 4 ? index * (4 / kParts) + r : index & 3, half = kParts == 8 ? index >> 2 : 0;
       const int at = (rows * 32 + lane) * 16;  // of this row, among 16 tokens of codes and among 8 of operands
-#pragma unroll
+#pragma unroll 1
       for (int c = half * 4; c < half * 4 + (kParts == 8 ? 4 : 8); c += 2) {
         const uint4 v = *reinterpret_cast<const uint4*>(block + c * 2048 + at), w = *reinterpret_cast<const uint4*>(block + (c + 1) * 2048 + at);
         *reinterpret_cast<uint4*>(out + (2 * c) * kChunk + at) = q8_expand<kF16>(v.x, v.y);
@@ -414,33 +414,47 @@ __global__ void __launch_bounds__(GemmCodesCfg<BN, kSpans>::THREADS, 1) tcec_gem
                   break;
                 }
                 tc_fence_after();
-                const uint32_t b_here = b16 + bs * (2 * Cfg::B_HALF >> 4);
-#pragma unroll
-                for (int step = 0; step < 8; ++step) {  // of 16 along the sum
-                  // an accumulator holds one group; where a block is one, all parts of it
-                  const bool first = step % (8 / kGroups) == 0 && (kGroups > 1 || part == 0);
-                  if (kGroups > 1 && step > 0 && first) {
-                    if (!mbar_wait(smem_u32(&bar_acc_free[x]), xph ^ 1, abortp, 0)) {
-                      ok = false;
-                      break;
+                // Short loops: the issuing thread shares its instruction cache with four warps that are busy elsewhere, and unrolled what it
+                // does for a block took longer than the MMAs.
+                uint32_t da = a_here, db = b16 + bs * (2 * Cfg::B_HALF >> 4);
+                uint32_t more = kGroups == 1 && part > 0;  // an accumulator holds one group; where a block is one, all parts of it
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll 1
+                  for (int j = 0; j < 2; ++j) {  // 32 of the sum
+                    if (kGroups == 4 && h + j > 0 || kGroups == 2 && h > 0 && j == 0) {
+                      if (!mbar_wait(smem_u32(&bar_acc_free[x]), xph ^ 1, abortp, 0)) {
+                        ok = false;
+                        break;
+                      }
+                      tc_fence_after();
+                      more = 0;
                     }
-                    tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                      if constexpr (kPair) umma_ss_pair<false>(tmem + x * BN, a_const | da, b_const | (db + i * 16), idesc, more);
+                      else umma_ss<false>(tmem + x * BN, a_const | da, b_const | (db + i * 16), idesc, more);
+                      da += 2 * Cfg::CHUNK_BYTES >> 4;
+                      more = 1;
+                    }
+                    db += Cfg::BC * 64 >> 4;
+                    if (kGroups == 4 || kGroups == 2 && j == 1) {
+                      commit(&bar_acc_full[x]);
+                      if (++x == Cfg::ACCS) x = 0, xph ^= 1;
+                    }
                   }
-                  const uint64_t da = a_const | (a_here + step * (2 * Cfg::CHUNK_BYTES >> 4));
-                  const uint64_t db = b_const | (b_here + (step >> 1) * (Cfg::BC * 64 >> 4) + (step & 1) * 16);
-                  if constexpr (kPair) umma_ss_pair<false>(tmem + x * BN, da, db, idesc, first ? 0u : 1u);
-                  else umma_ss<false>(tmem + x * BN, da, db, idesc, first ? 0u : 1u);
-                  if (step == 3) commit(&bar_b_empty[2 * bs]);
-                  if (step % (8 / kGroups) == 8 / kGroups - 1 && (kGroups > 1 || part == p.parts - 1)) {
-                    commit(&bar_acc_full[x]);
-                    if (++x == Cfg::ACCS) x = 0, xph ^= 1;
-                  }
+                  if (!ok) break;
+                  if (h == 0) commit(&bar_b_empty[2 * bs]);
                 }
                 if (!ok) break;
                 commit(&bar_b_empty[2 * bs + 1]);
                 if (++bs == Cfg::B_STAGES) bs = 0, bph ^= 1;
               }
               if (!ok) break;
+              if (kGroups == 1) {
+                commit(&bar_acc_full[x]);
+                if (++x == Cfg::ACCS) x = 0, xph ^= 1;
+              }
               commit(&bar_a_empty[as]);
               if (++as == Cfg::A_STAGES) as = 0, aph ^= 1;
             }

@@ -15,7 +15,7 @@ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 // follows from sizes.
 int warps_of(int ctas, int warps_of_sm, int least, int most) {
   const int warps = warps_of_sm / ceil_div(ctas, 148);
-  return warps < least ? least : warps > most ? most : warps;
+  return warps < least ? most / 2 > least ? most / 2 : most : warps > most ? most : warps;  // too many for one round: then not too few warps
 }
 // Launches for so many eights of columns and strips of rows a CTA, or (p null) allows the kernel its shared memory.
 template <int T, int G, int E, int S, bool One>
@@ -23,7 +23,7 @@ cudaError_t one_gemv(const GemvQ4Params* p, cudaStream_t stream) {
   using Cfg = GemvQ4Cfg<T, G, E, S, One>;
   constexpr int kMost = One ? 16 : 8;
   if (!p) return cudaFuncSetAttribute(gemv_q4_kernel<T, G, E, S, One>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem_bytes(kMost));
-  const int ctas = ceil_div(p->n, Cfg::ROWS), warps = warps_of(ctas, Cfg::WARPS_OF_SM, E == 1 ? 5 : 8, kMost);
+  const int ctas = ceil_div(p->n, Cfg::ROWS), warps = warps_of(ctas, Cfg::WARPS_OF_SM, 4, kMost);
   launch_early(gemv_q4_kernel<T, G, E, S, One>, ctas, 32 * warps, Cfg::smem_bytes(warps), stream, *p);
   return cudaSuccess;
 }
