@@ -173,12 +173,14 @@ __device__ __forceinline__ float ld_element_as(int type, const void* base, long 
 }
 
 // ---------------------------------------------------------------- arithmetic of the codes
-// rint(x / s) of the exact quotient, ties to even, for |x / s| below 2^8, without a branch: with values of few bits, as bf16 has, one in
-// some hundred quotients is a tie or next to one, so hardly a warp is without (8192 x 4096 bf16 to 8 bits 125 us with the exact way in a branch).
+// rint(x / s) of the exact quotient, ties to even, for |x / s| below 2^8, without a branch: of values of few bits, as bf16 has, one quotient in
+// some hundred is a tie or next to one, so hardly a warp would go without it (8192 x 4096 bf16 to 8 bits: 125 us with the exact way in a branch for
+// 16 values, 50 for four).
 //
-// q = x * (1 / s) + 1.5 * 2^23, whose last place is 1, is off by at most one.  The remainder r = x - q s is exact in FP32: x and q s are both
-// multiples of half the last place of s whenever |x| is at least s / 2, and |r| stays below 2 s; where |x| is smaller, q is 0 or +-1.  The sign of
-// 2 |r| - s decides; a tie (0) of an odd q does too, as the number whose bits are that one bit.
+// q = (x - s / 4) * (1 / s) + 1.5 * 2^23, whose last place is 1, is the number wanted or one below it.  The remainder r = x - q s is exact in FP32: x
+// and q s are both multiples of half the last place of s whenever |x| is at least s / 2, and |r| stays below 2 s; where |x| is smaller, q is 0 or -1.
+// The sign of 2 r - s decides; a tie (0) of an odd q does too, as the number whose bits are that one bit.  Logic and comparisons, which run at half the
+// rate of multiply-adds, are what packing is bound by: three of them here, five with a q to either side (42 us, PACKQ8 so).
 constexpr float kRintBase = 12582912.0f;
 struct Quotient {
   float s, inv;
@@ -186,21 +188,22 @@ struct Quotient {
     s = scale;
     inv = scale < 0x1p-126f ? 0.0f : __fdiv_rn(1.0f, scale);
   }
+  __device__ __forceinline__ Quotient(float scale, float inverse) {
+    s = scale;
+    inv = inverse;
+  }
   // A scale below the normal numbers, whose inverse may overflow, is not for nearest().
   __device__ __forceinline__ bool tiny() const { return inv == 0.0f; }
   // kRintBase + rint(x / s), as bits.
-  __device__ __forceinline__ int nearest(float x) const {
-    const float q = __fmaf_rn(x, inv, kRintBase), r = __fmaf_rn(kRintBase - q, s, x);
-    const int bits = __float_as_int(q);
-    const float past = __fmaf_rn(2.0f, fabsf(r), -s) + __int_as_float(bits & 1);
-    return past > 0.0f ? bits + ((__float_as_int(r) >> 31) | 1) : bits;
-  }
-  __device__ __forceinline__ int nearest_of_tiny(float x) const {
-    const float q = rintf(__fdiv_rn(x, s)), r = __fmaf_rn(-q, s, x), r2 = r + r;
-    int n = __float_as_int(q + kRintBase);
-    if (r2 > s || (r2 == s && (n & 1))) ++n;
-    else if (r2 < -s || (r2 == -s && (n & 1))) --n;
-    return n;
+  __device__ __forceinline__ int nearest(float x) const { return decide(__fmaf_rn(__fmaf_rn(s, -0.25f, x), inv, kRintBase), x); }
+  __device__ __forceinline__ int nearest_of_tiny(float x) const { return decide(floorf(__fdiv_rn(x, s)) + kRintBase, x); }
+
+ private:
+  __device__ __forceinline__ int decide(float q, float x) const {
+    const float r = __fmaf_rn(kRintBase - q, s, x);
+    int bits = __float_as_int(q);
+    if (__fmaf_rn(2.0f, r, -s) + __int_as_float(bits & 1) > 0.0f) ++bits;
+    return bits;
   }
 };
 __device__ __forceinline__ bool not_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
@@ -264,24 +267,24 @@ __global__ void __launch_bounds__(256) pack_q4_kernel(const PackQ4Params p) {
 #pragma unroll
     for (int q = 0; q < kSpans; ++q) {  // groups; 128 / kSpans = 16 * 8 / kSpans
       float lo = 0.f, hi = 0.f;
-      uint32_t most = 0;  // magnitude as bits, among which infinities and NaN come last
+      float none = 0.f;  // NaN if a value is not finite
 #pragma unroll
       for (int j = q * 8 / kSpans; j < (q + 1) * 8 / kSpans; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           lo = fminf(lo, v[j][i]);
           hi = fmaxf(hi, v[j][i]);
-          most = max(most, __float_as_uint(v[j][i]) & 0x7fffffffu);
+          none = __fmaf_rn(v[j][i], 0.0f, none);
         }
 #pragma unroll
       for (int d = 1; d <= 2; d <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+        none += __shfl_xor_sync(0xffffffffu, none, d);
       }
       const float want = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
       const float s = p.scale_bf16 ? __bfloat162float(__float2bfloat16_rn(want)) : __half2float(__float2half_rn(want));
-      const bool bad = most >= 0x7f800000u || not_finite(s), some = !bad && s > 0.f;
+      const bool bad = none != 0.f || not_finite(s), some = !bad && s > 0.f;
       const Quotient by(some ? s : 1.0f);
       const int base = __float_as_int(kRintBase), z = !some ? 0 : min((by.tiny() ? by.nearest_of_tiny(-lo) : by.nearest(-lo)) - base, 15);
       uint32_t code[8 / kSpans];
@@ -407,8 +410,8 @@ struct PackQ8Params {
 // One CTA a block of 128 tokens x 128 features: a warp takes 16 tokens, a lane four consecutive features of each, all of it in
 // registers; the warps' maxima meet in shared memory.
 template <int kType>
-__global__ void __launch_bounds__(256) pack_q8_kernel(const PackQ8Params p) {
-  __shared__ float4 most[8][32];
+__global__ void __launch_bounds__(256, 3) pack_q8_kernel(const PackQ8Params p) {
+  __shared__ float4 most[8][32], scales[32], inverses[32];
   wait_for_launch_before();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = (p.features + kCodeRows - 1) / kCodeRows, tile = blockIdx.x % tiles, tb = blockIdx.x / tiles;  // whole rows at a time
@@ -416,43 +419,51 @@ __global__ void __launch_bounds__(256) pack_q8_kernel(const PackQ8Params p) {
   float v[16][4];
   ld_lines4<kType, 16>(p.x, t0 * p.token_step + f0 * p.feature_step, p.token_step, p.feature_step, p.tokens - t0, p.features - f0, p.vec, v);
   let_next_launch_start();
-  float m[4] = {0.f, 0.f, 0.f, 0.f};  // the largest magnitude as bits, among which infinities and NaN come last
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) m[j] = __uint_as_float(max(__float_as_uint(m[j]), __float_as_uint(v[i][j]) & 0x7fffffffu));
-  most[warp][lane] = make_float4(m[0], m[1], m[2], m[3]);
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const float4 o = most[w][lane];
-    m[0] = __uint_as_float(max(__float_as_uint(m[0]), __float_as_uint(o.x)));
-    m[1] = __uint_as_float(max(__float_as_uint(m[1]), __float_as_uint(o.y)));
-    m[2] = __uint_as_float(max(__float_as_uint(m[2]), __float_as_uint(o.z)));
-    m[3] = __uint_as_float(max(__float_as_uint(m[3]), __float_as_uint(o.w)));
-  }
-  uint8_t* block = p.packed + (static_cast<size_t>(tile) * p.token_blocks + tb) * kQ8BlockBytes;
-  float scale[4];
+  float m[4];  // the largest magnitude, or NaN if a value is not finite
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const bool bad = not_finite(m[j]);
-    const float s = bad ? 1.0f : fmaxf(__fdiv_rn(m[j], 127.0f), 0x1p-120f);
-    scale[j] = bad ? nan32() : s;
-    const Quotient by(s);
-    uint32_t q[16];  // magnitudes, in the low bytes
+    float none = 0.f;
+    m[j] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) q[i] = by.nearest(fabsf(v[i][j]));
+    for (int i = 0; i < 16; ++i) {
+      m[j] = fmaxf(m[j], fabsf(v[i][j]));
+      none = __fmaf_rn(v[i][j], 0.0f, none);
+    }
+    if (none != 0.f) m[j] = nan32();
+  }
+  most[warp][lane] = make_float4(m[0], m[1], m[2], m[3]);
+  __syncthreads();
+  uint8_t* block = p.packed + (static_cast<size_t>(tile) * p.token_blocks + tb) * kQ8BlockBytes;
+  if (threadIdx.x < 128) {  // a feature each: divisions are long
+    uint32_t top = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) top = max(top, __float_as_uint(reinterpret_cast<const float*>(most[w])[threadIdx.x]));
+    const bool bad = top >= 0x7f800000u;
+    const Quotient by(bad ? 1.0f : fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), 0x1p-120f));
+    reinterpret_cast<float*>(scales)[threadIdx.x] = by.s;
+    reinterpret_cast<float*>(inverses)[threadIdx.x] = bad ? nan32() : by.inv;
+    reinterpret_cast<float*>(block + kQ8CodeBytes)[threadIdx.x] = bad ? nan32() : by.s;
+  }
+  __syncthreads();
+  const float4 s4 = scales[lane], i4 = inverses[lane];
+  const float scale[4] = {s4.x, s4.y, s4.z, s4.w}, inverse[4] = {i4.x, i4.y, i4.z, i4.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const bool bad = inverse[j] != inverse[j];
+    const Quotient by(scale[j], inverse[j]);
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // tokens 0 2 1 3 of each four, and their signs
-      const uint32_t size = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 2], 0x0040), __byte_perm(q[4 * i + 1], q[4 * i + 3], 0x0040), 0x5410);
+      int q[4];  // magnitudes, in the low bytes
+#pragma unroll
+      for (int t = 0; t < 4; ++t) q[t] = by.nearest(fabsf(v[4 * i + t][j]));
+      const uint32_t size = __byte_perm(__byte_perm(q[0], q[2], 0x0040), __byte_perm(q[1], q[3], 0x0040), 0x5410);
       const uint32_t sign = __byte_perm(__byte_perm(__float_as_uint(v[4 * i][j]), __float_as_uint(v[4 * i + 2][j]), 0x0073),
                                         __byte_perm(__float_as_uint(v[4 * i + 1][j]), __float_as_uint(v[4 * i + 3][j]), 0x0073), 0x5410);
       w[i] = bad ? 0 : (size & 0x7f7f7f7fu) | (sign & 0x80808080u);
     }
     *reinterpret_cast<uint4*>(block + warp * 2048 + (lane * 4 + j) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  if (warp == 0) reinterpret_cast<float4*>(block + kQ8CodeBytes)[lane] = make_float4(scale[0], scale[1], scale[2], scale[3]);
 }
 
 // A lane takes four features of 16 tokens.
