@@ -130,7 +130,7 @@ struct StageColumns {
 };
 template <int T>
 struct StagePanels {
-  static void go(int grid, cudaStream_t stream, const StagePanelsParams& p) { launch_early(stage_panels_kernel<T>, grid, 256, 0, stream, p); }
+  static void go(int grid, cudaStream_t stream, const StagePanelsParams& p) { launch_early(stage_panels_kernel<T>, dim3(grid, 2), 256, 0, stream, p); }
 };
 // D[row][col] of tcec_gemm_codes.cuh for an operand of codes (spans: groups of 4-bit codes in a block, 0: 8-bit codes) and a dense one whose columns and sum lie at the given steps.
 int gemm_codes(const void* codes, int spans, int rows, int cols, int sum, const void* dense, long long col_step, long long sum_step,

@@ -291,7 +291,8 @@ __global__ void __launch_bounds__(GemmCodesCfg<BN, kSpans>::THREADS, 1) tcec_gem
   tc_fence_after();
   const uint32_t tmem = tmem_base_s;
   volatile uint32_t* abortp = &abort_flag;
-  wait_for_launch_before();
+  // Only what touches the dense operand or C waits for the kernel before, which stages the dense operand: that was through its own wait when
+  // this one could start, so whatever the codes come from has ended, and they are fetched and expanded meanwhile.
   auto give_up = [&](int code) {
     if constexpr (kPair) raise_abort_pair(&abort_flag);
     else abort_flag = 1;
@@ -302,6 +303,7 @@ __global__ void __launch_bounds__(GemmCodesCfg<BN, kSpans>::THREADS, 1) tcec_gem
     setmaxnreg_dec<Cfg::REGS_CONTROL>();
     if (warp == 0) {
       // ---------------------------------------------------------- copies of the dense operand
+      wait_for_launch_before();
       if (elect_one()) {
         uint32_t half = 0, ph = 0, armed = 0, armed_parity = 0;  // halves of stages
         bool ok = true;
@@ -309,7 +311,7 @@ __global__ void __launch_bounds__(GemmCodesCfg<BN, kSpans>::THREADS, 1) tcec_gem
           const CodeTile ti = code_tile(tile, tile_rows, p.col_tiles);
           const int col = ti.col * BN + (kPair ? rank * 128 : 0);
           const uint32_t bytes = max(0, min(Cfg::BC, (p.cols - col + 15) & ~15)) * 64;  // a pair's second half may have no columns
-          const uint8_t* src = p.panels + (static_cast<size_t>(col >> 7) * p.blocks + kb_first) * p.parts * kSpanBytes + (col & 127) * 64;
+          const uint8_t* src = after_wait(p.panels) + (static_cast<size_t>(col >> 7) * p.blocks + kb_first) * p.parts * kSpanBytes + (col & 127) * 64;
           for (int left = nkb * p.parts * 2; left > 0; --left) {  // a half of a block and part
             if (!mbar_wait(smem_u32(&bar_b_empty[half]), ph ^ 1, abortp)) {
               ok = false;
@@ -503,6 +505,7 @@ __global__ void __launch_bounds__(GemmCodesCfg<BN, kSpans>::THREADS, 1) tcec_gem
   } else {
     // ------------------------------------------------------------ scales
     setmaxnreg_inc<Cfg::REGS_FOLD>();
+    wait_for_launch_before();
     const int fw = warp - 4 - Cfg::CONVERTERS, q = warp & 3, r = q * 32 + lane, first_col = fw >= 4 ? Cfg::NC : 0;
     const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + first_col;
     const float* scales = reinterpret_cast<const float*>(smem_gen + Cfg::SCALE_OFFSET) + r;

@@ -42,12 +42,13 @@ __device__ __forceinline__ void put_split(const Put& put, int it, const float (&
   for (int q = 0; q < 3; ++q) put(it, q, make_uint4(part[2 - q][0], part[2 - q][1], part[2 - q][2], part[2 - q][3]));
 }
 
-// One CTA a block of 128 columns x 128 of the sum; an item is 16 bytes of a panel, eight consecutive values of one column.  Addresses stay
+// Two CTAs a block of 128 columns x 128 of the sum; an item is 16 bytes of a panel, eight consecutive values of one column.  Addresses stay
 // among the elements that exist, so that all loads of some items go out before the first is waited for.
 template <int kType>
 __global__ void __launch_bounds__(256) stage_panels_kernel(const StagePanelsParams p) {
   constexpr int kParts = kType == kTypeF32 ? 3 : 1;
   wait_for_launch_before();
+  let_next_launch_start();  // the product: its CTAs take whole SMs, and fetch and expand codes
   const int kb = blockIdx.x % p.blocks, cb = blockIdx.x / p.blocks;
   uint8_t* out = p.panels + static_cast<size_t>(blockIdx.x) * kParts * kSpanBytes;
   const int cols = min(kCodeRows, (p.cols - cb * kCodeRows + 15) & ~15);  // columns that an MMA may read
@@ -67,7 +68,7 @@ __global__ void __launch_bounds__(256) stage_panels_kernel(const StagePanelsPara
   const int cols_here = p.cols - cb * kCodeRows, sum_here = p.sum - kb * kCodeSpan;
   const long long origin = static_cast<long long>(cb) * kCodeRows * p.col_step + static_cast<long long>(kb) * kCodeSpan * p.sum_step;
 #pragma unroll 1
-  for (int it0 = 0; it0 < 8; it0 += kAtOnce) {
+  for (int it0 = blockIdx.y * 4; it0 < blockIdx.y * 4 + 4; it0 += kAtOnce) {
     if (p.vec && sum_here >= kCodeSpan) {
       uint4 raw[kAtOnce][kType == kTypeF32 ? 2 : 1];
 #pragma unroll
@@ -115,7 +116,6 @@ __global__ void __launch_bounds__(256) stage_panels_kernel(const StagePanelsPara
       }
     }
   }
-  let_next_launch_start();
 }
 
 // Codes that are operands as they are, in the lowest bits of 16 (tcec_gemv_q4.cuh): bf16 operands come times kUpX, so that their products stay
