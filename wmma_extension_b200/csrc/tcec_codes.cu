@@ -147,6 +147,7 @@ int gemm_codes(const void* codes, int spans, int rows, int cols, int sum, const 
     sp.blocks = blocks;
     sp.panels = static_cast<uint8_t*>(workspace);
     sp.vec = vec;
+    sp.pairs = type != TCEC_TYPE_F32 && col_step == 1 && !vec && cols % 2 == 0 && sum_step % 2 == 0 && aligned(dense, 4);
     by_type<StagePanels>(type, static_cast<int>(ceil_div(cols, kCodeRows) * blocks), stream, sp);
   }
   GemmCodesParams gp{};

@@ -17,6 +17,7 @@ struct StagePanelsParams {
   int blocks;                 // along the sum
   uint8_t* panels;            // [128 columns][block][part][panel]
   int vec;                    // sum_step 1 and aligned for 16 bytes
+  int pairs;                  // 16 bits, col_step 1, an even number of columns, aligned for two
 };
 // x = hi + mid + lo, 8 bits each, two values at a time.  Exactly so unless lo falls below the smallest bf16 number; what is not finite
 // stays in hi alone.
@@ -67,6 +68,33 @@ __global__ void __launch_bounds__(256) stage_panels_kernel(const StagePanelsPara
   constexpr int kAtOnce = kType == kTypeF32 ? 2 : 4;  // items whose loads are under way together
   const int cols_here = p.cols - cb * kCodeRows, sum_here = p.sum - kb * kCodeSpan;
   const long long origin = static_cast<long long>(cb) * kCodeRows * p.col_step + static_cast<long long>(kb) * kCodeSpan * p.sum_step;
+  if constexpr (kType != kTypeF32) {
+    if (p.pairs) {  // two columns at a time, eight of the sum, of two panels
+      const int r = (first & 63) * 2, c = first >> 6, col = min(r, cols_here - 2);
+      const bool none = r >= cols_here;
+      uint32_t w[2][8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          w[h][j] = ld_operand32(static_cast<const uint16_t*>(p.src) + origin + col + min((blockIdx.y * 2 + h) * 32 + c * 8 + j, sum_here - 1) * p.sum_step);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int panel = blockIdx.y * 2 + h;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (none || panel * 32 + c * 8 + j >= sum_here) w[h][j] = 0;
+        if (r < cols) {  // which is a multiple of 16
+          uint4* const to = reinterpret_cast<uint4*>(out + panel * kPanelBytes + (r >> 3) * 512 + c * 128 + (r & 7) * 16);
+          to[0] = make_uint4(__byte_perm(w[h][0], w[h][1], 0x5410), __byte_perm(w[h][2], w[h][3], 0x5410), __byte_perm(w[h][4], w[h][5], 0x5410),
+                             __byte_perm(w[h][6], w[h][7], 0x5410));
+          to[1] = make_uint4(__byte_perm(w[h][0], w[h][1], 0x7632), __byte_perm(w[h][2], w[h][3], 0x7632), __byte_perm(w[h][4], w[h][5], 0x7632),
+                             __byte_perm(w[h][6], w[h][7], 0x7632));
+        }
+      }
+      return;
+    }
+  }
 #pragma unroll 1
   for (int it0 = blockIdx.y * 4; it0 < blockIdx.y * 4 + 4; it0 += kAtOnce) {
     if (p.vec && sum_here >= kCodeSpan) {
