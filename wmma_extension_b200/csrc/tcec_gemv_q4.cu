@@ -21,7 +21,7 @@ int warps_of(int ctas, int warps_of_sm, int least, int most) {
 template <int T, int G, int E, int S, bool One>
 cudaError_t one_gemv(const GemvQ4Params* p, cudaStream_t stream) {
   using Cfg = GemvQ4Cfg<T, G, E, S, One>;
-  constexpr int kMost = One ? 16 : 8;
+  constexpr int kMost = Cfg::MOST_WARPS;
   if (!p) return cudaFuncSetAttribute(gemv_q4_kernel<T, G, E, S, One>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem_bytes(kMost));
   const int ctas = ceil_div(p->n, Cfg::ROWS), warps = warps_of(ctas, Cfg::WARPS_OF_SM, 4, kMost);
   launch_early(gemv_q4_kernel<T, G, E, S, One>, ctas, 32 * warps, Cfg::smem_bytes(warps), stream, *p);
@@ -30,9 +30,10 @@ cudaError_t one_gemv(const GemvQ4Params* p, cudaStream_t stream) {
 template <int T, int G>
 cudaError_t gemv_of(int eights, const GemvQ4Params& p, cudaStream_t stream) {
   if (!p.staged && p.n <= 8192) return one_gemv<T, G, 1, 1, true>(&p, stream);
-  if (!p.staged) return one_gemv<T, G, 1, 2, true>(&p, stream);
+  const bool long_k = p.blocks >= 32;  // a CTA of four strips does for x what four of one do, but its warps need blocks to divide
+  if (!p.staged) return long_k ? one_gemv<T, G, 1, 4, true>(&p, stream) : one_gemv<T, G, 1, 2, true>(&p, stream);
   if (eights == 1 && p.n <= 8192) return one_gemv<T, G, 1, 1, false>(&p, stream);
-  if (eights == 1) return one_gemv<T, G, 1, 2, false>(&p, stream);
+  if (eights == 1) return long_k ? one_gemv<T, G, 1, 4, false>(&p, stream) : one_gemv<T, G, 1, 2, false>(&p, stream);
   // An SM runs one of these CTAs at a time.  What it does for its columns is about two thirds of the work of a strip, and CTAs of two strips do
   // it half as often; those of one strip leave fewer SMs idle at the end.
   const bool two = ceil_div(ceil_div(p.n, 32), 148) * (2 * 3 + 2) <= ceil_div(ceil_div(p.n, 16), 148) * (3 + 2);
@@ -43,8 +44,10 @@ template <int T, int G>
 cudaError_t set_attrs() {
   cudaError_t e = one_gemv<T, G, 1, 1, true>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 1, 2, true>(nullptr, nullptr);
+  if (e == cudaSuccess) e = one_gemv<T, G, 1, 4, true>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 1, 1, false>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 1, 2, false>(nullptr, nullptr);
+  if (e == cudaSuccess) e = one_gemv<T, G, 1, 4, false>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 2, 2, false>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 4, 2, false>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 2, 1, false>(nullptr, nullptr);
