@@ -165,13 +165,19 @@ int gemm_codes(const void* codes, int spans, int rows, int cols, int sum, const 
   gp.c_col = c_col;
   gp.c_type = c_type;
   gp.status = here.status;
+  // Pairs of SMs with 256 columns make the most of each converted weight, but are half as many: they are taken where tiles of 128 columns would be
+  // more than the SMs (4096 x 4096: 512 tokens, 128 such tiles, 25.8 us, in pairs 36.0; 768 tokens, 192 tiles, 43.4 and 35.7; 1000 45.2 and 38.9).
   int bn = cols <= 64 ? 64 : 128;
-  if (cols > 128 && ceil_div(gp.row_tiles, 2) * ceil_div(cols, 256) >= 50) bn = 256;
+  if (cols > 128 && gp.row_tiles * ceil_div(cols, 128) > 148) bn = 256;
   gp.col_tiles = static_cast<int>(ceil_div(cols, bn));
   const long long tiles = (bn == 256 ? ceil_div(gp.row_tiles, 2) : gp.row_tiles) * static_cast<long long>(gp.col_tiles);
   if (tiles > kMostBlocks) return TCEC_ERR_UNSUPPORTED;
   int ctas = bn == 256 ? 2 : 1;  // of a cluster
-  while (bn < 256 && ctas < 8 && tiles * ctas * 2 <= 148 && blocks >= 4 * ctas) ctas *= 2;
+  // Tiles too few for the SMs divide the sum among the CTAs of clusters.  Only as many clusters as surely run at a time: SMs that a GPC has over stay idle, and
+  // 16 clusters of eight took two rounds where 15 took one (64 columns of 4096: 2048 rows 17.5 us, 1920 rows 9.8; with clusters of four 11.0);
+  // of four, 35 did and 33 did not (4480 rows 22.1, 4224 rows 12.8).  Constants, as the order of the sums is to follow from sizes alone.
+  constexpr long long kMostClusters[4] = {0, 74, 32, 14};  // of 2, 4 and 8 CTAs
+  while (bn < 256 && ctas < 8 && tiles <= kMostClusters[ctas == 1 ? 1 : ctas == 2 ? 2 : 3] && blocks >= 4 * ctas) ctas *= 2;
   // One cluster a tile where the sum is divided; else as many as run at a time.
   const long long most = bn == 256 ? here.sm_count / 2 : ctas > 1 ? tiles : here.sm_count;
   const int grid = static_cast<int>(tiles < most ? tiles : most) * ctas;
@@ -182,7 +188,7 @@ int gemm_codes(const void* codes, int spans, int rows, int cols, int sum, const 
 // Columns of the tensor-core operand that this many tokens take, and whether they are so few that the weights are streamed through
 // registers (tcec_gemv_q4.cuh).
 long long columns_of(int m, int type) { return static_cast<long long>(m) * (type == TCEC_TYPE_F32 ? 3 : 1); }
-bool streamed(int m, int type) { return columns_of(m, type) <= 32; }
+bool streamed(int m, int n, int type) { return columns_of(m, type) <= (n <= 8192 || type == TCEC_TYPE_F32 ? 32 : 16); }
 int eights_of(int m, int type) { return columns_of(m, type) <= 8 ? 1 : columns_of(m, type) <= 16 ? 2 : 4; }
 
 }  // namespace
@@ -283,7 +289,7 @@ int tcec_unpack_q4(int layout_w, int n, int k, const void* packed, int group, vo
 
 size_t tcec_gemm_q4_workspace_bytes(int m, int n, int k, int type_x) {
   if (m < 0 || n < 0 || k < 0 || bad_type(type_x) || m <= 1) return 0;
-  if (streamed(m, type_x)) return static_cast<size_t>(staged_bytes(ceil_div(k, kCodeSpan), eights_of(m, type_x)));
+  if (streamed(m, n, type_x)) return static_cast<size_t>(staged_bytes(ceil_div(k, kCodeSpan), eights_of(m, type_x)));
   return panel_bytes(m, k, type_x);
 }
 
@@ -308,12 +314,12 @@ int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, c
     Here here;
     const int rc = get_here(&here);
     if (rc != TCEC_OK) return rc;
-    if (!streamed(m, type_x))
+    if (!streamed(m, n, type_x) || (m > 1 && !sum))  // without a sum there is no workspace to stage tokens in
       return gemm_codes(packed, kCodeSpan / group, n, m, sum, x, dx.row_step(), dx.col_step(), type_x, layout_x == TCEC_ROW_MAJOR && dx.wide(16), alpha,
                         beta, c, dc.col_step(), dc.row_step(), type_c, workspace, here, static_cast<cudaStream_t>(stream));
     const cudaStream_t on = static_cast<cudaStream_t>(stream);
     const int blocks = static_cast<int>(ceil_div(sum, kCodeSpan)), eights = eights_of(m, type_x);
-    if (m > 1 && blocks) {
+    if (m > 1) {
       StageColumnsParams sp{};
       sp.src = x;
       sp.col_step = dx.row_step();
@@ -329,7 +335,7 @@ int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, c
     }
     GemvQ4Params p{};
     p.codes = static_cast<const uint8_t*>(packed);
-    p.staged = m > 1 && blocks ? static_cast<const uint8_t*>(workspace) : nullptr;
+    p.staged = m > 1 ? static_cast<const uint8_t*>(workspace) : nullptr;
     p.x = x;
     p.x_k = dx.col_step();
     p.n = n;

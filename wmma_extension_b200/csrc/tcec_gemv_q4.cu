@@ -34,9 +34,11 @@ cudaError_t gemv_of(int eights, const GemvQ4Params& p, cudaStream_t stream) {
   if (!p.staged) return long_k ? one_gemv<T, G, 1, 4, true>(&p, stream) : one_gemv<T, G, 1, 2, true>(&p, stream);
   if (eights == 1 && p.n <= 8192) return one_gemv<T, G, 1, 1, false>(&p, stream);
   if (eights == 1) return long_k ? one_gemv<T, G, 1, 4, false>(&p, stream) : one_gemv<T, G, 1, 2, false>(&p, stream);
-  // An SM runs one of these CTAs at a time.  What it does for its columns is about two thirds of the work of a strip, and CTAs of two strips do
-  // it half as often; those of one strip leave fewer SMs idle at the end.
-  const bool two = ceil_div(ceil_div(p.n, 32), 148) * (2 * 3 + 2) <= ceil_div(ceil_div(p.n, 16), 148) * (3 + 2);
+  // A CTA of two strips does for its columns once what two of one strip do twice, but its SMs may stay idle at the end.  The work of a strip grows
+  // with its groups, and a strip of two groups costs about what the columns do (12 tokens, groups of 128: 2048 rows of 4096 5.4 us with one strip,
+  // 6.5 with two; 5000 rows of 7001 13.6 and 12.4; in groups of 32 15.9 and 17.8).
+  constexpr int kSpans = kCodeSpan / G;
+  const bool two = ceil_div(ceil_div(p.n, 32), 148) * (2 * kSpans + 2) <= ceil_div(ceil_div(p.n, 16), 148) * (kSpans + 2);
   if (eights == 2) return two ? one_gemv<T, G, 2, 2, false>(&p, stream) : one_gemv<T, G, 2, 1, false>(&p, stream);
   return two ? one_gemv<T, G, 4, 2, false>(&p, stream) : one_gemv<T, G, 4, 1, false>(&p, stream);
 }

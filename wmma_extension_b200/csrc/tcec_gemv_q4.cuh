@@ -44,7 +44,7 @@ template <int kType, int kGroup, int kEights, int kStrips, bool kOne>
 struct GemvQ4Cfg {
   static constexpr int PARTS = kType == kTypeF32 ? 3 : 1;
   static constexpr int ROWS = 16 * kStrips;
-  static constexpr int MOST_WARPS = kOne && kStrips < 4 ? 16 : 8;
+  static constexpr int MOST_WARPS = (kOne && kStrips < 4) || kEights == 2 ? 16 : 8;
   static constexpr int STAGE_BYTES = kStrips * q4_strip_bytes(kGroup);
   static constexpr int STAGES = 2;                            // blocks of codes under way, of each warp
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
@@ -55,7 +55,7 @@ struct GemvQ4Cfg {
   static constexpr int WARP_BYTES = RING_BYTES + X_BYTES > SUM_BYTES ? RING_BYTES + X_BYTES : SUM_BYTES;
   static constexpr int smem_bytes(int warps) { return warps * WARP_BYTES + 128; }
   // Registers a thread, and with them the warps of an SM: 64 (32 warps) for one token, else what the operands of the columns need.
-  static constexpr int WARPS_OF_SM = kEights == 1 ? (kStrips == 4 ? 16 : kOne ? 32 : 20) : kEights == 2 ? 12 : 8;
+  static constexpr int WARPS_OF_SM = kEights == 1 ? (kStrips == 4 ? 16 : kOne ? 32 : 20) : kEights == 2 ? 16 : 8;
 };
 
 template <bool kF16>
@@ -64,10 +64,10 @@ __device__ __forceinline__ void mma16816_zero(float (&d)[4], uint32_t a0, uint32
   mma16816<kF16>(d, a0, a1, a2, a3, b0, b1);
 }
 
-// One strip and eight columns: operands b of the four panels, `sums` of x over the groups and `unit` for this lane's two columns.
-template <int kType, int kGroup>
-__device__ __forceinline__ void multiply_strip(float (&acc)[4], const uint8_t* strip, int lane, const uint4 (&b)[4], const float (&sums)[kCodeSpan / kGroup][2],
-                                               const float (&unit)[2]) {
+// One strip: operands b of the four panels, `sums` of x over the groups and `unit` for this lane's two columns of each eight.
+template <int kType, int kGroup, int kEights>
+__device__ __forceinline__ void multiply_strip(float (&acc)[kEights][4], const uint8_t* strip, int lane, const uint4 (&b)[4][kEights],
+                                               const float2 (&sums)[kCodeSpan / kGroup][kEights], const float2 (&unit)[kEights]) {
   constexpr bool kF16 = kType == kTypeF16;
   constexpr int kSpans = kCodeSpan / kGroup;
   constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
@@ -75,25 +75,31 @@ __device__ __forceinline__ void multiply_strip(float (&acc)[4], const uint8_t* s
   const uint32_t* e = reinterpret_cast<const uint32_t*>(strip + kStripCodeBytes) + (lane >> 2);
 #pragma unroll
   for (int q = 0; q < kSpans; ++q) {
-    float d[2][4];  // of codes, and of 16 times codes
+    float d[kEights][2][4];  // of codes, and of 16 times codes
 #pragma unroll
     for (int panel = q * 4 / kSpans; panel < (q + 1) * 4 / kSpans; ++panel) {
       const bool first = panel == q * 4 / kSpans;
       const uint4 pair = w[panel >> 1];
       const uint32_t w0 = panel & 1 ? pair.z : pair.x, w1 = panel & 1 ? pair.w : pair.y;  // of rows g and g + 8
       const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
-      mma16816_zero<kF16>(d[0], w0 & kLow, w1 & kLow, v0 & kLow, v1 & kLow, b[panel].x, b[panel].z, first);
-      mma16816_zero<kF16>(d[1], w0 & kHigh, w1 & kHigh, v0 & kHigh, v1 & kHigh, b[panel].y, b[panel].w, first);
+#pragma unroll
+      for (int c = 0; c < kEights; ++c) {
+        mma16816_zero<kF16>(d[c][0], w0 & kLow, w1 & kLow, v0 & kLow, v1 & kLow, b[panel][c].x, b[panel][c].z, first);
+        mma16816_zero<kF16>(d[c][1], w0 & kHigh, w1 & kHigh, v0 & kHigh, v1 & kHigh, b[panel][c].y, b[panel][c].w, first);
+      }
     }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const uint32_t entry = e[q * 16 + r * 8];
       const float scale = __uint_as_float(entry & ~15u), z = 8388608.0f - __uint_as_float(0x4b000000u | (entry & 15u));  // minus the zero point
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float sum = __fmaf_rn(0.0625f * unit[j], d[1][r * 2 + j], unit[j] * d[0][r * 2 + j]);
-        acc[r * 2 + j] = __fmaf_rn(scale, __fmaf_rn(z, sums[q][j], sum), acc[r * 2 + j]);
-      }
+      for (int c = 0; c < kEights; ++c)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float u = j ? unit[c].y : unit[c].x, x = j ? sums[q][c].y : sums[q][c].x;
+          const float sum = __fmaf_rn(0.0625f * u, d[c][1][r * 2 + j], u * d[c][0][r * 2 + j]);
+          acc[c][r * 2 + j] = __fmaf_rn(scale, __fmaf_rn(z, x, sum), acc[c][r * 2 + j]);
+        }
     }
   }
 }
@@ -151,7 +157,7 @@ __device__ __forceinline__ void multiply_block(float (&acc)[kStrips][kEights][4]
 }
 
 template <int kType, int kGroup, int kEights, int kStrips, bool kOne>
-__global__ void __launch_bounds__(32 * (kOne && kStrips < 4 ? 16 : 8), kEights == 1 ? 2 : 1) gemv_q4_kernel(const GemvQ4Params p) {
+__global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips, kOne>::MOST_WARPS, kEights == 1 ? 2 : 1) gemv_q4_kernel(const GemvQ4Params p) {
   using Cfg = GemvQ4Cfg<kType, kGroup, kEights, kStrips, kOne>;
   static_assert(!kOne || kEights == 1, "one token has at most three columns");
   constexpr int kSpans = kCodeSpan / kGroup;
@@ -240,7 +246,7 @@ __global__ void __launch_bounds__(32 * (kOne && kStrips < 4 ? 16 : 8), kEights =
   if (warp < p.blocks) {
     if constexpr (kOne) {
       load_four(warp);
-    } else {
+    } else if constexpr (kEights != 2) {
       load_sums(warp);
 #pragma unroll
       for (int panel = 0; panel < 4; ++panel) load_operands(warp, panel);
@@ -279,42 +285,54 @@ __global__ void __launch_bounds__(32 * (kOne && kStrips < 4 ? 16 : 8), kEights =
       }
       if (next < p.blocks) load_four(next);
     }
+    if constexpr (kEights == 2) {  // more warps instead of operands ahead
+      load_sums(kb);
+#pragma unroll
+      for (int panel = 0; panel < 4; ++panel) load_operands(kb, panel);
+    }
     ok = mbar_wait_lanes(smem_u32(&bars[warp][stage]), parity, &abort_flag);  // brings the lanes together, too
     if (!ok) break;
     const uint8_t* const here = ring + stage * Cfg::STAGE_BYTES;
     if constexpr (kOne) {
       // sums of x: the same products with codes that are all one
-      uint4 b[4];
-      float ones[kSpans][4], sums[kSpans][2];
+      uint4 b[4][1];
+      float ones[kSpans][4];
+      float2 sums[kSpans][1];
 #pragma unroll
       for (int panel = 0; panel < 4; ++panel) {
-        b[panel] = *reinterpret_cast<const uint4*>(x_shared + (lane >> 2) * Cfg::X_PITCH + panel * 64 + (lane & 3) * 16);
+        b[panel][0] = *reinterpret_cast<const uint4*>(x_shared + (lane >> 2) * Cfg::X_PITCH + panel * 64 + (lane & 3) * 16);
         const int q = panel * kSpans / 4;
-        mma16816_zero<kF16>(ones[q], kOnes, kOnes, kOnes, kOnes, b[panel].x, b[panel].z, panel == q * 4 / kSpans);
-        mma16816<kF16>(ones[q], kOnes, kOnes, kOnes, kOnes, b[panel].y, b[panel].w);
+        mma16816_zero<kF16>(ones[q], kOnes, kOnes, kOnes, kOnes, b[panel][0].x, b[panel][0].z, panel == q * 4 / kSpans);
+        mma16816<kF16>(ones[q], kOnes, kOnes, kOnes, kOnes, b[panel][0].y, b[panel][0].w);
       }
 #pragma unroll
-      for (int q = 0; q < kSpans; ++q)
+      for (int q = 0; q < kSpans; ++q) sums[q][0] = make_float2(ones[q][0] * unit, ones[q][1] * unit);
+      const float2 units[1] = {make_float2(unit, unit)};
 #pragma unroll
-        for (int j = 0; j < 2; ++j) sums[q][j] = ones[q][j] * unit;
-      const float units[2] = {unit, unit};
+      for (int s = 0; s < kStrips; ++s) multiply_strip<kType, kGroup, 1>(acc[s], here + s * q4_strip_bytes(kGroup), lane, b, sums, units);
+    } else if constexpr (kEights == 2) {
+      if constexpr (kF16) units_ahead[0] = units_ahead[1] = make_float2(StagedUnit<kType>::UNIT, StagedUnit<kType>::UNIT);
 #pragma unroll
-      for (int s = 0; s < kStrips; ++s) multiply_strip<kType, kGroup>(acc[s][0], here + s * q4_strip_bytes(kGroup), lane, b, sums, units);
+      for (int s = 0; s < kStrips; ++s)
+        multiply_strip<kType, kGroup, kEights>(acc[s], here + s * q4_strip_bytes(kGroup), lane, b_ahead, sums_ahead, units_ahead);
     } else if constexpr (kEights == 1) {
-      uint4 b[4];
-      float sums[kSpans][2];
+      uint4 b[4][kEights];
+      float2 sums[kSpans][kEights], units[kEights];
 #pragma unroll
-      for (int panel = 0; panel < 4; ++panel) b[panel] = b_ahead[panel][0];
+      for (int c = 0; c < kEights; ++c) {
+        units[c] = kF16 ? make_float2(StagedUnit<kType>::UNIT, StagedUnit<kType>::UNIT) : units_ahead[c];
 #pragma unroll
-      for (int q = 0; q < kSpans; ++q) sums[q][0] = sums_ahead[q][0].x, sums[q][1] = sums_ahead[q][0].y;
-      const float units[2] = {kF16 ? StagedUnit<kType>::UNIT : units_ahead[0].x, kF16 ? StagedUnit<kType>::UNIT : units_ahead[0].y};
+        for (int panel = 0; panel < 4; ++panel) b[panel][c] = b_ahead[panel][c];
+#pragma unroll
+        for (int q = 0; q < kSpans; ++q) sums[q][c] = sums_ahead[q][c];
+      }
       if (next < p.blocks) {
         load_sums(next);
 #pragma unroll
         for (int panel = 0; panel < 4; ++panel) load_operands(next, panel);
       }
 #pragma unroll
-      for (int s = 0; s < kStrips; ++s) multiply_strip<kType, kGroup>(acc[s][0], here + s * q4_strip_bytes(kGroup), lane, b, sums, units);
+      for (int s = 0; s < kStrips; ++s) multiply_strip<kType, kGroup, kEights>(acc[s], here + s * q4_strip_bytes(kGroup), lane, b, sums, units);
     } else {
       float2 sums[kSpans][kEights], units[kEights];
 #pragma unroll
