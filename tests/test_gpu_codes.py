@@ -453,3 +453,132 @@ def test_python_refuses():
     with pytest.raises(tcec.TcecError) as e:  # the result over its own operand
         tcec.gemm_q4(x[:, :32], packed, 32, x[:, :32], group=32)
     assert e.value.status == tcec.ERR_INVALID_ARGUMENT
+
+
+# ---------------------------------------------------------------- every form of the kernels
+@pytest.mark.parametrize("n,k", [(2400, 200), (4810, 130), (8200, 100), (8200, 4100), (9000, 4000)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_few_tokens_of_wide_layers(n, k, group, dtype):
+    for m in (1, 2, 5, 8, 10, 12, 16, 24, 32):
+        x, packed, exact, tol = product_case(m, n, k, group, dtype, m + n)
+        check(tcec.gemm_q4(x, packed, n, group=group), exact, tol)
+    tcec.device_status()
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 1792, 4096), (40, 1921, 4096), (70, 4096, 2050), (40, 4224, 1100), (70, 9400, 1030), (200, 700, 5000),
+                                   (600, 4500, 260)])
+@pytest.mark.parametrize("dtype,group", [(F32, 32), (F16, 64), (BF16, 128)])
+def test_products_divided_among_clusters(m, n, k, dtype, group):
+    x, packed, exact, tol = product_case(m, n, k, group, dtype, m + n)
+    check(tcec.gemm_q4(x, packed, n, group=group), exact, tol)
+    tcec.device_status()
+
+
+@pytest.mark.parametrize("m", [1, 2, 12, 20, 40])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_without_a_sum_c_is_scaled(m, dtype):
+    x, packed, _, _ = product_case(m, 300, 4096, 128, dtype, 31)
+    c = randn(m, 300, seed=32, dtype=dtype)
+    half = (0.5 * c.double()).to(dtype)
+    assert torch.equal(tcec.gemm_q4(x * float("nan"), packed, 300, c.clone(), alpha=0.0, beta=0.5), half)
+    assert torch.equal(tcec.gemm_q4(x[:, :0], packed[:0], 300, c.clone(), beta=0.5), half)
+    assert (tcec.gemm_q4(x, packed, 300, c.fill_(float("nan")), alpha=0.0) == 0).all()
+
+
+@pytest.mark.parametrize("m", [1, 2, 5, 9, 10, 24, 60])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_tokens_of_any_magnitude(m, dtype):
+    """Relative to the largest magnitudes of a token, whatever they are: from 2^-110 (few tokens; more: 2^-90) to 2^100, in a block or in all.
+
+    bound() has an absolute part of 1e-30, so tokens are compared after their results are scaled back, by a power of two.  With one large value
+    the rounding of few tokens is relative to scale * (code + zero) * |x|, not to scale * |code - zero| * |x|: the sums of code * x and of x over a
+    group are made apart, each rounded to 2^-24 of itself, and the zero point times the second is taken off the first.  Where the code of a value
+    2^90 is its zero point the exact term is 0, and 2^-24 * scale * 2 * zero * 2^90 is left of it.
+    """
+    n, k = 70, 500
+    byte, s, z, w = with_codes(n, k, 64, 33)
+    packed = tcec.pack_q4_codes(byte, s, z, k=k, group=64)
+    base = randn(m, k, seed=m, dtype=dtype)
+    for exponent in (-110 if m * (3 if dtype == F32 else 1) <= 32 else -90, -61, -59, 26, 28, 100):
+        x = (base.double() * 2.0**exponent).to(dtype)
+        exact = base.double() @ w.T
+        got = tcec.gemm_q4(x, packed, n, group=64, dtype=F32).double() * 2.0**-exponent
+        check(got, exact, bound(base.double().abs() @ w.abs().T, exact, F32, k, 3 if dtype == F32 else 1))
+    # a large value in one block of some tokens: these lose what lies far below it, the others nothing
+    x = base.clone()
+    x[::2, 200] *= 2.0**90
+    got = tcec.gemm_q4(x, packed, n, group=64, dtype=F32)
+    exact = x.double() @ w.T
+    each = torch.arange(k, device=DEV) // 64
+    sizes = (torch.stack([byte & 15, byte >> 4], 2).reshape(n, -1)[:, :k].double() + z.double()[:, each]) * s.double()[:, each]
+    check(got, exact, bound(x.double().abs() @ sizes.T, exact, F32, k, 3 if dtype == F32 else 1))
+    assert torch.equal(got[1::2], tcec.gemm_q4(base, packed, n, group=64, dtype=F32)[1::2])
+
+
+def test_one_token_that_is_not_finite():
+    for dtype in (F32, F16, BF16):
+        x, packed, _, _ = product_case(1, 64, 256, 128, dtype, 35)
+        x[0, 130] = float("nan")
+        assert tcec.gemm_q4(x, packed, 64).isnan().all()
+        x[0, 130] = -float("inf")
+        assert not tcec.gemm_q4(x, packed, 64).isfinite().any()
+
+
+@pytest.mark.parametrize("m", [1, 12])
+def test_replays_see_new_tokens_and_new_weights(m):
+    n, k = 200, 700
+    x, packed, _, _ = product_case(m, n, k, 128, BF16, 37)
+    c = torch.zeros(m, n, device=DEV, dtype=BF16)
+    tcec.gemm_q4(x, packed, n, c)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tcec.gemm_q4(x, packed, n, c)
+    for seed in (41, 43, 45):
+        x2, packed2, exact, tol = product_case(m, n, k, 128, BF16, seed)
+        x.copy_(x2), packed.copy_(packed2)
+        graph.replay()
+        check(c, exact, tol)
+
+
+def test_calls_of_several_threads_at_once():
+    import threading
+
+    cases = [product_case(m, 300, 900, 64, dtype, m) for m, dtype in ((1, F32), (7, BF16), (30, F16), (100, BF16))]
+    torch.cuda.synchronize()
+    got, streams = [None] * 4, [torch.cuda.Stream() for _ in range(4)]
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(50):
+                got[i] = tcec.gemm_q4(cases[i][0], cases[i][1], 300, group=64)
+        streams[i].synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for c, (_, _, exact, tol) in zip(got, cases):
+        check(c, exact, tol)
+    tcec.device_status()
+
+
+def test_packing_and_product_one_after_the_other_without_a_wait():
+    """Each call may start before the one before has ended; what it reads has been written all the same."""
+    n, k = 1000, 2000
+    for i in range(20):
+        w = randn(n, k, seed=i, dtype=BF16)
+        x = randn(3 + i, k, seed=i + 50, dtype=BF16)
+        packed = torch.empty(tcec.q4_bytes(n, k, 128), dtype=torch.uint8, device=DEV)
+        kept = torch.empty(tcec.q8_bytes(3 + i, k), dtype=torch.uint8, device=DEV)
+        torch.cuda.synchronize()
+        y = tcec.gemm_q4(x, tcec.pack_q4(w, out=packed), n)
+        g = tcec.wgrad_q8(y, tcec.pack_q8(x, out=kept), k, dtype=F32)
+        q, s = quantise8(x)
+        wq = values(w, 128, F16)
+        exact = x.double() @ wq.T
+        check(y, exact, bound(x.double().abs() @ wq.abs().T, exact, BF16, k, 1))
+        exact = y.double().T @ (q * s)
+        check(g, exact, bound(y.double().abs().T @ (q * s).abs(), exact, F32, 3 + i, 1))

@@ -185,8 +185,10 @@ int gemm_codes(const void* codes, int spans, int rows, int cols, int sum, const 
   return launched();
 }
 
-// Columns of the tensor-core operand that this many tokens take, and whether they are so few that the weights are streamed through
-// registers (tcec_gemv_q4.cuh).
+// Columns of the tensor-core operand that this many tokens take, and whether they are so few that the weights are streamed through registers
+// (tcec_gemv_q4.cuh).  Up to 16 columns always: 16 tokens times 16384 x 16384 46 us, 17 74.  Up to 32 while the rows are few, as tiles of 128 rows then
+// leave SMs idle: 24 tokens times 4096 x 4096 10.7 us, in tiles 12.7; 8192 x 4096 15.8 and 16.9; but 16384 x 1024 15.8 and 10.8.  FP32 in
+// tiles has three parts to bring in: 10 tokens times 16384 x 16384 94 us, 11 160.
 long long columns_of(int m, int type) { return static_cast<long long>(m) * (type == TCEC_TYPE_F32 ? 3 : 1); }
 bool streamed(int m, int n, int type) { return columns_of(m, type) <= (n <= 8192 || type == TCEC_TYPE_F32 ? 32 : 16); }
 int eights_of(int m, int type) { return columns_of(m, type) <= 8 ? 1 : columns_of(m, type) <= 16 ? 2 : 4; }

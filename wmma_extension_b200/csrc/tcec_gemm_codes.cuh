@@ -41,20 +41,12 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
-// A constant that stays in a register.
-__device__ __forceinline__ uint32_t held(uint32_t v) {
-  asm volatile("mov.b32 %0, %0;" : "+r"(v));
-  return v;
-}
 // Eight 4-bit codes to code - zero point, in order.
 template <bool kF16>
-__device__ __forceinline__ uint4 q4_expand(uint32_t w, uint32_t zero, uint32_t mask, uint32_t magic) {
+__device__ __forceinline__ uint4 q4_expand(uint32_t w, uint32_t zero) {
+  constexpr uint32_t mask = 0x000f000fu, magic = kF16 ? 0x64006400u : 0x43004300u;
   return make_uint4(sub16x2(and_or(w, mask, magic), zero, kF16), sub16x2(and_or(w >> 4, mask, magic), zero, kF16),
                     sub16x2(and_or(w >> 8, mask, magic), zero, kF16), sub16x2(and_or(w >> 12, mask, magic), zero, kF16));
-}
-template <bool kF16>
-__device__ __forceinline__ uint4 q4_expand(uint32_t w, uint32_t zero) {
-  return q4_expand<kF16>(w, zero, 0x000f000fu, kF16 ? 0x64006400u : 0x43004300u);
 }
 // Eight 8-bit codes (sign and magnitude) in the bytes 0 2, 1 3 of two words, to operands in order: +-(magic + magnitude) -+ magic.
 template <bool kF16>

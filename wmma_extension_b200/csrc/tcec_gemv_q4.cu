@@ -10,9 +10,9 @@ namespace tcec_host {
 namespace {
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
-// As many warps divide the k of a CTA's rows as let all CTAs run at a time: a second round of them would leave SMs idle at its end, and as
-// every CTA goes through all of k it is long (16384 x 16384 with one token: ROUNDS).  So many SMs are assumed whatever the device has, so that the order of the sums
-// follows from sizes.
+// As many warps divide the k of a CTA's rows as let all CTAs run at a time: a second round of them would leave SMs idle at its end, and as every CTA
+// goes through all of k it is long (13 tokens times 5000 x 7001: 16.7 us, 19.8 with eight warps whatever the rows).  So many SMs are assumed whatever
+// the device has, so that the order of the sums follows from sizes.
 int warps_of(int ctas, int warps_of_sm, int least, int most) {
   const int warps = warps_of_sm / ceil_div(ctas, 148);
   return warps < least ? most / 2 > least ? most / 2 : most : warps > most ? most : warps;  // too many for one round: then not too few warps
@@ -29,8 +29,10 @@ cudaError_t one_gemv(const GemvQ4Params* p, cudaStream_t stream) {
 }
 template <int T, int G>
 cudaError_t gemv_of(int eights, const GemvQ4Params& p, cudaStream_t stream) {
+  // Wide layers have CTAs enough with more strips, which share what is done for x: four where k is long enough for their warps (one FP32 token
+  // times 16384 x 16384, groups of 64: 35 us, with two strips 42, with one 45), else two; 4096 x 4096 has 128 CTAs of two, and takes 5.2 us with one.
   if (!p.staged && p.n <= 8192) return one_gemv<T, G, 1, 1, true>(&p, stream);
-  const bool long_k = p.blocks >= 32;  // a CTA of four strips does for x what four of one do, but its warps need blocks to divide
+  const bool long_k = p.blocks >= 32;
   if (!p.staged) return long_k ? one_gemv<T, G, 1, 4, true>(&p, stream) : one_gemv<T, G, 1, 2, true>(&p, stream);
   if (eights == 1 && p.n <= 8192) return one_gemv<T, G, 1, 1, false>(&p, stream);
   if (eights == 1) return long_k ? one_gemv<T, G, 1, 4, false>(&p, stream) : one_gemv<T, G, 1, 2, false>(&p, stream);

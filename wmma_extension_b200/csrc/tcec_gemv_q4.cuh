@@ -1,20 +1,23 @@
 // Few tokens times 4-bit weights: C[token][row] = alpha * sum_g s[row, g] sum_{i in g} (q[row][i] - z[row, g]) x[token][i] + beta C.
 //
-// Bound by the bytes of the weights and by the instructions that make operands of them.  Codes go from global memory through a ring of bulk
-// copies into the registers of mma.m16n8k16, in whose order they are stored (tcec_codes.cuh).  Five logic instructions make operands of a
-// word of eight codes: a 4-bit code in the low 8 bits of a 16-bit number that is otherwise zero is that code (or 16 times it, in the upper
-// half) times the smallest number there is, 2^-24 in f16 and 2^-133 in bf16, subnormal or not; nothing is added or taken off.  The upper ones
-// have an accumulator of their own.  What the zero points take off is z times the sum of x over the group, and the power of two goes
-// into the last factor.  (Codes made to numbers first, by a magic number and a subtraction: seven logic instructions and four
-// subtractions; 16384 x 16384 37.0 us instead of WITHSUB.)  To stay among the normal FP32 numbers with such small factors, bf16 operands come times 2^100,
-// unless a token has a value of 2^27 or more among the 128 k: then times 2^6, and what is lost lies 2^-49 below the largest.  (Values
-// of 2^122 and more count as infinite.)
+// Bound by the bytes of the weights and, as these come from memory at two thirds of its rate, by the instructions that make operands of them.  Codes go
+// from global memory through a ring of bulk copies for each warp into the registers of mma.m16n8k16, in whose order they are stored (tcec_codes.cuh).
+// (tcgen05 takes operands from shared memory or TMEM: expanded codes would be written there and read again, and its tiles have no use for eight columns.)
+// A few logic instructions make operands of a word of eight codes: a 4-bit code in the low bits of a 16-bit number that is otherwise zero is that code
+// (or 16 times it, in the next four bits) times a power of two, subnormal or not; nothing is added or taken off.  The upper ones have an accumulator of
+// their own.  What the zero points take off is z times the sum of x over the group, and the power of two goes into the last factor.  (Codes made to
+// numbers first, by a magic number and a subtraction: an FP32 token times 16384 x 16384 in groups of 64 49 us instead of 45 at the time.)  How bf16
+// operands are kept from products below FP32: tcec_stage.cuh.  Values of 2^122 and more count as infinite.
 //
-// Columns are tokens; an FP32 token takes three, its bf16 parts of 8 bits each, which together are exactly it.  Every product
-// of a code and a part is exact; a group's sum is made in the MMA's FP32 accumulator, then multiplied by its scale and added in
-// FP32, rounded to nearest.
+// Columns are tokens; an FP32 token takes three, its bf16 parts of 8 bits each, which together are exactly it.  Every product of a code and a part is
+// exact; a group's sum is made in the MMA's FP32 accumulator, then multiplied by its scale and added in FP32, rounded to nearest.  As code and zero
+// point are multiplied apart, what is rounded off is relative to scale * (code + zero) * |x|.
 //
-// A CTA takes 16 kStrips rows; its warps divide k block by block and add up through shared memory in a fixed order.
+// A CTA takes 16 kStrips rows; its warps divide k block by block and add up through shared memory in a fixed order.  One strip after the other, the
+// operands of the columns stay in registers: 16384 x 16384 with 16 tokens 45.6 us, strips side by side 53.8, with one FP32 token (groups of 64) 35 and 42.
+//
+// Measured, from memory: one bf16 token times 4096 x 4096 5.2 us (1.7 TB/s: 32 rows of blocks an SM are over before the copies are up to speed), times
+// 16384 x 16384 30.5 (4.6 TB/s), FP32 in groups of 64 35.5 (4.2 TB/s); 8 tokens 29 us, 16 45.6, 32 (10 of FP32) 94.
 #pragma once
 #include "tcec_gemm_codes.cuh"
 
@@ -54,7 +57,7 @@ struct GemvQ4Cfg {
   static constexpr int SUM_BYTES = ROWS * SUM_PITCH * 4;      // of a warp
   static constexpr int WARP_BYTES = RING_BYTES + X_BYTES > SUM_BYTES ? RING_BYTES + X_BYTES : SUM_BYTES;
   static constexpr int smem_bytes(int warps) { return warps * WARP_BYTES + 128; }
-  // Registers a thread, and with them the warps of an SM: 64 (32 warps) for one token, else what the operands of the columns need.
+  // Warps that an SM's registers hold: 64 registers a thread for one token, else what the operands of the columns need.
   static constexpr int WARPS_OF_SM = kEights == 1 ? (kStrips == 4 ? 16 : kOne ? 32 : 20) : kEights == 2 ? 16 : 8;
 };
 
@@ -70,7 +73,10 @@ __device__ __forceinline__ void multiply_strip(float (&acc)[kEights][4], const u
                                                const float2 (&sums)[kCodeSpan / kGroup][kEights], const float2 (&unit)[kEights]) {
   constexpr bool kF16 = kType == kTypeF16;
   constexpr int kSpans = kCodeSpan / kGroup;
-  constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+  // In f16 the codes lie three bits higher, which with bit 10, the exponent's last, are as high as numbers grow evenly: the tensor core aligns
+  // products by their operands' exponents, and what lies low among the smallest keeps fewer bits.
+  constexpr int kUp = kF16 ? 3 : 0;
+  constexpr uint32_t kLow = 0x000f000fu << kUp, kHigh = 0x00f000f0u << kUp;
   const uint4 w[2] = {*reinterpret_cast<const uint4*>(strip + lane * 16), *reinterpret_cast<const uint4*>(strip + 512 + lane * 16)};
   const uint32_t* e = reinterpret_cast<const uint32_t*>(strip + kStripCodeBytes) + (lane >> 2);
 #pragma unroll
@@ -80,8 +86,8 @@ __device__ __forceinline__ void multiply_strip(float (&acc)[kEights][4], const u
     for (int panel = q * 4 / kSpans; panel < (q + 1) * 4 / kSpans; ++panel) {
       const bool first = panel == q * 4 / kSpans;
       const uint4 pair = w[panel >> 1];
-      const uint32_t w0 = panel & 1 ? pair.z : pair.x, w1 = panel & 1 ? pair.w : pair.y;  // of rows g and g + 8
-      const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
+      const uint32_t word0 = panel & 1 ? pair.z : pair.x, word1 = panel & 1 ? pair.w : pair.y;  // of rows g and g + 8
+      const uint32_t w0 = word0 << kUp, w1 = word1 << kUp, v0 = word0 >> (8 - kUp), v1 = word1 >> (8 - kUp);
 #pragma unroll
       for (int c = 0; c < kEights; ++c) {
         mma16816_zero<kF16>(d[c][0], w0 & kLow, w1 & kLow, v0 & kLow, v1 & kLow, b[panel][c].x, b[panel][c].z, first);
@@ -104,65 +110,13 @@ __device__ __forceinline__ void multiply_strip(float (&acc)[kEights][4], const u
   }
 }
 
-// The codes of a block, a strip at a time, times the operands that take(panel, b) gives; sums folded into acc.  sum_of(q, c, j) gives the sum of x
-// over group q for this lane's two columns (j) of eight c, unit_of(c, j) what makes their products values (StagedUnit).
-template <int kType, int kGroup, int kEights, int kStrips, class Take, class SumOf, class UnitOf>
-__device__ __forceinline__ void multiply_block(float (&acc)[kStrips][kEights][4], const uint8_t* stage, int lane, const Take& take,
-                                               const SumOf& sum_of, const UnitOf& unit_of) {
-  constexpr bool kF16 = kType == kTypeF16;
-  constexpr int kSpans = kCodeSpan / kGroup;
-  constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
-  uint4 w[kStrips][2];  // rows g and g + 8, of two panels each
-#pragma unroll
-  for (int s = 0; s < kStrips; ++s)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) w[s][h] = *reinterpret_cast<const uint4*>(stage + s * q4_strip_bytes(kGroup) + h * 512 + lane * 16);
-#pragma unroll
-  for (int q = 0; q < kSpans; ++q) {
-    float d[kStrips][kEights][2][4];  // of codes, and of 16 times codes
-#pragma unroll
-    for (int panel = q * 4 / kSpans; panel < (q + 1) * 4 / kSpans; ++panel) {
-      const bool first = panel == q * 4 / kSpans;
-      uint4 b[kEights];
-      take(panel, b);
-#pragma unroll
-      for (int s = 0; s < kStrips; ++s) {
-        const uint4 pair = w[s][panel >> 1];
-        const uint32_t w0 = panel & 1 ? pair.z : pair.x, w1 = panel & 1 ? pair.w : pair.y;  // of rows g and g + 8
-        const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
-#pragma unroll
-        for (int c = 0; c < kEights; ++c) {
-          mma16816_zero<kF16>(d[s][c][0], w0 & kLow, w1 & kLow, v0 & kLow, v1 & kLow, b[c].x, b[c].z, first);
-          mma16816_zero<kF16>(d[s][c][1], w0 & kHigh, w1 & kHigh, v0 & kHigh, v1 & kHigh, b[c].y, b[c].w, first);
-        }
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < kStrips; ++s) {
-      const uint32_t* e = reinterpret_cast<const uint32_t*>(stage + s * q4_strip_bytes(kGroup) + kStripCodeBytes) + q * 16 + (lane >> 2);
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint32_t entry = e[r * 8];
-        const float scale = __uint_as_float(entry & ~15u), z = 8388608.0f - __uint_as_float(0x4b000000u | (entry & 15u));  // minus the zero point
-#pragma unroll
-        for (int c = 0; c < kEights; ++c)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float unit = unit_of(c, j), sum = __fmaf_rn(0.0625f * unit, d[s][c][1][r * 2 + j], unit * d[s][c][0][r * 2 + j]);
-            acc[s][c][r * 2 + j] = __fmaf_rn(scale, __fmaf_rn(z, sum_of(q, c, j), sum), acc[s][c][r * 2 + j]);
-          }
-      }
-    }
-  }
-}
-
 template <int kType, int kGroup, int kEights, int kStrips, bool kOne>
 __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips, kOne>::MOST_WARPS, kEights == 1 ? 2 : 1) gemv_q4_kernel(const GemvQ4Params p) {
   using Cfg = GemvQ4Cfg<kType, kGroup, kEights, kStrips, kOne>;
   static_assert(!kOne || kEights == 1, "one token has at most three columns");
   constexpr int kSpans = kCodeSpan / kGroup;
   constexpr bool kF16 = kType == kTypeF16;
-  constexpr uint32_t kOnes = 0x00010001u;
+  constexpr uint32_t kOnes = kF16 ? 0x04000400u : 0x00800080u;  // 2^7 times a code's 1, the smallest normal number: no bits are lost
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bars[Cfg::MOST_WARPS][Cfg::STAGES];
   __shared__ uint32_t abort_flag;
@@ -246,7 +200,7 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
   if (warp < p.blocks) {
     if constexpr (kOne) {
       load_four(warp);
-    } else if constexpr (kEights != 2) {
+    } else if constexpr (kEights == 1) {
       load_sums(warp);
 #pragma unroll
       for (int panel = 0; panel < 4; ++panel) load_operands(warp, panel);
@@ -258,17 +212,19 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
   int kb = warp;
   for (; kb < p.blocks; kb += warps) {
     const int next = kb + warps;
-    [[maybe_unused]] float unit = StagedUnit<kType>::UNIT;
+    [[maybe_unused]] float unit = kUnitF16;
     if constexpr (kOne) {
       uint8_t* to = x_shared + lane * 8;
       float v[4];
       if constexpr (kType != kTypeF16) {
         four.get(v);
-        const bool large = __any_sync(0xffffffffu, fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))) >= kLargeX);
-        const float up = large ? kUpLarge : kUpX;
-        if (large) unit = kUnitLarge;
+        uint32_t most = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] *= up;
+        for (int j = 0; j < 4; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+        const UpX by = up_x(__reduce_max_sync(0xffffffffu, most));
+        unit = by.unit;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] *= by.up;
       }
       if constexpr (kType == kTypeF32) {
         uint2 hi, mid, lo;
@@ -285,7 +241,7 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
       }
       if (next < p.blocks) load_four(next);
     }
-    if constexpr (kEights == 2) {  // more warps instead of operands ahead
+    if constexpr (kEights > 1) {  // more warps instead of operands ahead (16 tokens times 16384 x 16384: 46 us, 54 so)
       load_sums(kb);
 #pragma unroll
       for (int panel = 0; panel < 4; ++panel) load_operands(kb, panel);
@@ -294,7 +250,7 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
     if (!ok) break;
     const uint8_t* const here = ring + stage * Cfg::STAGE_BYTES;
     if constexpr (kOne) {
-      // sums of x: the same products with codes that are all one
+      // sums of x: the same products with a constant for codes
       uint4 b[4][1];
       float ones[kSpans][4];
       float2 sums[kSpans][1];
@@ -306,21 +262,23 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
         mma16816<kF16>(ones[q], kOnes, kOnes, kOnes, kOnes, b[panel][0].y, b[panel][0].w);
       }
 #pragma unroll
-      for (int q = 0; q < kSpans; ++q) sums[q][0] = make_float2(ones[q][0] * unit, ones[q][1] * unit);
+      for (int q = 0; q < kSpans; ++q) sums[q][0] = make_float2(ones[q][0] * (unit * 0x1p-7f), ones[q][1] * (unit * 0x1p-7f));
       const float2 units[1] = {make_float2(unit, unit)};
 #pragma unroll
       for (int s = 0; s < kStrips; ++s) multiply_strip<kType, kGroup, 1>(acc[s], here + s * q4_strip_bytes(kGroup), lane, b, sums, units);
-    } else if constexpr (kEights == 2) {
-      if constexpr (kF16) units_ahead[0] = units_ahead[1] = make_float2(StagedUnit<kType>::UNIT, StagedUnit<kType>::UNIT);
+    } else if constexpr (kEights > 1) {
+#pragma unroll
+      for (int c = 0; c < kEights; ++c)
+        if constexpr (kF16) units_ahead[c] = make_float2(kUnitF16, kUnitF16);
 #pragma unroll
       for (int s = 0; s < kStrips; ++s)
         multiply_strip<kType, kGroup, kEights>(acc[s], here + s * q4_strip_bytes(kGroup), lane, b_ahead, sums_ahead, units_ahead);
-    } else if constexpr (kEights == 1) {
+    } else {
       uint4 b[4][kEights];
       float2 sums[kSpans][kEights], units[kEights];
 #pragma unroll
       for (int c = 0; c < kEights; ++c) {
-        units[c] = kF16 ? make_float2(StagedUnit<kType>::UNIT, StagedUnit<kType>::UNIT) : units_ahead[c];
+        units[c] = kF16 ? make_float2(kUnitF16, kUnitF16) : units_ahead[c];
 #pragma unroll
         for (int panel = 0; panel < 4; ++panel) b[panel][c] = b_ahead[panel][c];
 #pragma unroll
@@ -333,24 +291,6 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
       }
 #pragma unroll
       for (int s = 0; s < kStrips; ++s) multiply_strip<kType, kGroup, kEights>(acc[s], here + s * q4_strip_bytes(kGroup), lane, b, sums, units);
-    } else {
-      float2 sums[kSpans][kEights], units[kEights];
-#pragma unroll
-      for (int c = 0; c < kEights; ++c) {
-        units[c] = units_ahead[c];
-#pragma unroll
-        for (int q = 0; q < kSpans; ++q) sums[q][c] = sums_ahead[q][c];
-      }
-      if (next < p.blocks) load_sums(next);
-      multiply_block<kType, kGroup, kEights, kStrips>(
-          acc, here, lane,
-          [&](int panel, uint4(&now)[kEights]) {
-#pragma unroll
-            for (int c = 0; c < kEights; ++c) now[c] = b_ahead[panel][c];
-            if (next < p.blocks) load_operands(next, panel);
-          },
-          [&](int q, int c, int j) { return j ? sums[q][c].y : sums[q][c].x; },
-          [&](int c, int j) { return kF16 ? StagedUnit<kType>::UNIT : j ? units[c].y : units[c].x; });
     }
     __syncwarp();  // all have read the stage
     if (lane == 0 && kb + Cfg::STAGES * warps < p.blocks) fetch(kb + Cfg::STAGES * warps, stage);

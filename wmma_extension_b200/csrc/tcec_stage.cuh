@@ -146,14 +146,19 @@ __global__ void __launch_bounds__(256) stage_panels_kernel(const StagePanelsPara
   }
 }
 
-// Codes that are operands as they are, in the lowest bits of 16 (tcec_gemv_q4.cuh): bf16 operands come times kUpX, so that their products stay
-// normal numbers, or times kUpLarge where a token has a value of kLargeX or more among the 128 of a block.  The unit makes the product
-// of a code 1 and such an operand the operand's value.
-constexpr float kUpX = 0x1p100f, kLargeX = 0x1p27f, kUpLarge = 0x1p6f, kUnitLarge = 0x1p127f;
-template <int kType>
-struct StagedUnit {
-  static constexpr float UNIT = kType == kTypeF16 ? 0x1p24f : 0x1p33f;
+// Codes that are operands as they are, in the lowest bits of 16 (tcec_gemv_q4.cuh), are multiples of 2^-21 (f16) or 2^-133 (bf16).  f16 products are
+// normal FP32 numbers all the same.  bf16 operands come times a power of two, so that their products do not fall below what FP32 holds, 2^-149: 2^100,
+// or what suits the largest of a token's 128 values in a block: 2^6 from 2^27 on, 2^127 below 2^-60.  So what is lost lies below 2^-116, 2^-49 times the largest
+// value, or 2^-143.  The unit makes the product of a code 1 and such an operand the operand's value.
+constexpr float kUnitF16 = 0x1p21f;
+struct UpX {
+  float up, unit, down;  // down: 1 / up
 };
+__device__ __forceinline__ UpX up_x(uint32_t most) {  // the bits of the largest magnitude
+  if (most >= 0x4d000000u) return {0x1p6f, 0x1p127f, 0x1p-6f};  // 2^27
+  if (most < 0x21800000u) return {0x1p127f, 0x1p6f, 0x1p-127f};  // 2^-60
+  return {0x1p100f, 0x1p33f, 0x1p-100f};
+}
 
 // Columns of mma.m16n8k16: for each block of 128 of the sum, 32 of it and eight columns, lane 4 g + t has 8 values of column g from
 // 8 t on, 16 bytes.  A column is a token, or a part of one (FP32).  Behind the operands of all blocks, for each block: the columns'
@@ -219,17 +224,16 @@ __global__ void __launch_bounds__(512) stage_columns_kernel(const StageColumnsPa
       }
     }
   }
-  bool large = false;
+  UpX by = {1.f, kUnitF16, 1.f};
   if constexpr (kType != kTypeF16) {
-    float most = 0.f;
+    uint32_t most = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));
+    for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
 #pragma unroll
-    for (int d = 1; d < 16; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-    large = most >= kLargeX;
-    const float up = large ? kUpLarge : kUpX;
+    for (int d = 1; d < 16; d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+    by = up_x(most);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= up;
+    for (int j = 0; j < 8; ++j) v[j] *= by.up;
   }
   uint32_t part[kParts][4];
   if constexpr (kType == kTypeF32) {
@@ -266,8 +270,8 @@ __global__ void __launch_bounds__(512) stage_columns_kernel(const StageColumnsPa
     if (col < columns) {
       if ((chunk & (of_group - 1)) == 0)
         *reinterpret_cast<float*>(sums + ((1 + chunk / of_group) * columns + col) * 4) =
-            kType == kTypeF16 ? sum : sum * (large ? 1.0f / kUpLarge : 1.0f / kUpX);
-      if (chunk == 0) *reinterpret_cast<float*>(sums + col * 4) = large ? kUnitLarge : StagedUnit<kType>::UNIT;
+            sum * by.down;
+      if (chunk == 0) *reinterpret_cast<float*>(sums + col * 4) = by.unit;
     }
   }
 }
