@@ -456,7 +456,7 @@ def test_python_refuses():
 
 
 # ---------------------------------------------------------------- every form of the kernels
-@pytest.mark.parametrize("n,k", [(2400, 200), (4810, 130), (8200, 100), (8200, 4100), (9000, 4000)])
+@pytest.mark.parametrize("n,k", [(2400, 200), (4810, 130), (8200, 100), (8200, 4100), (9000, 4000), (9600, 300), (9600, 4100)])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_few_tokens_of_wide_layers(n, k, group, dtype):

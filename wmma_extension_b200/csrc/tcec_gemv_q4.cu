@@ -29,13 +29,13 @@ cudaError_t one_gemv(const GemvQ4Params* p, cudaStream_t stream) {
 }
 template <int T, int G>
 cudaError_t gemv_of(int eights, const GemvQ4Params& p, cudaStream_t stream) {
-  // Wide layers have CTAs enough with more strips, which share what is done for x: four where k is long enough for their warps (one FP32 token
-  // times 16384 x 16384, groups of 64: 35 us, with two strips 42, with one 45), else two; 4096 x 4096 has 128 CTAs of two, and takes 5.2 us with one.
-  if (!p.staged && p.n <= 8192) return one_gemv<T, G, 1, 1, true>(&p, stream);
-  const bool long_k = p.blocks >= 32;
-  if (!p.staged) return long_k ? one_gemv<T, G, 1, 4, true>(&p, stream) : one_gemv<T, G, 1, 2, true>(&p, stream);
-  if (eights == 1 && p.n <= 8192) return one_gemv<T, G, 1, 1, false>(&p, stream);
-  if (eights == 1) return long_k ? one_gemv<T, G, 1, 4, false>(&p, stream) : one_gemv<T, G, 1, 2, false>(&p, stream);
+  // What is done for x a CTA does once for all its strips.  One token: one strip while such CTAs fit the SMs, two likewise, then four, whose warps need
+  // blocks to divide, though (bf16, with one, two and four: 2048 x 4096 3.5, 4.1, 5.7 us; 4096 x 4096 5.3, 4.9, 6.1; 5120 x 5120 8.1, 7.8, 7.2;
+  // 8192 x 8192 14.3, 11.7, 10.6; 16384 x 16384 51, 37, 31; 12288 x 1024 4.8, 4.1, 4.2).
+  if (!p.staged && p.n <= 148 * 16) return one_gemv<T, G, 1, 1, true>(&p, stream);
+  if (!p.staged) return p.n <= 148 * 32 || p.blocks < 16 ? one_gemv<T, G, 1, 2, true>(&p, stream) : one_gemv<T, G, 1, 4, true>(&p, stream);
+  // Five tokens: 2048 x 4096 5.3, 5.1, 6.4 us; 8192 x 8192 13.8, 11.0, 15.4; 12288 x 1024 5.9, 6.2, 5.1; 16384 x 16384 36, 37, 29.
+  if (eights == 1) return p.n <= 148 * 64 ? one_gemv<T, G, 1, 2, false>(&p, stream) : one_gemv<T, G, 1, 4, false>(&p, stream);
   // A CTA of two strips does for its columns once what two of one strip do twice, but its SMs may stay idle at the end.  The work of a strip grows
   // with its groups, and a strip of two groups costs about what the columns do (12 tokens, groups of 128: 2048 rows of 4096 5.4 us with one strip,
   // 6.5 with two; 5000 rows of 7001 13.6 and 12.4; in groups of 32 15.9 and 17.8).
@@ -49,7 +49,6 @@ cudaError_t set_attrs() {
   cudaError_t e = one_gemv<T, G, 1, 1, true>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 1, 2, true>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 1, 4, true>(nullptr, nullptr);
-  if (e == cudaSuccess) e = one_gemv<T, G, 1, 1, false>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 1, 2, false>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 1, 4, false>(nullptr, nullptr);
   if (e == cudaSuccess) e = one_gemv<T, G, 2, 2, false>(nullptr, nullptr);
