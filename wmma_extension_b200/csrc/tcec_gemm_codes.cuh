@@ -73,11 +73,11 @@ struct GemmCodesCfg {
   // multiple of 128, so that lanes with rows g, g + 1 of four chunks write to all banks at once.
   static constexpr int CHUNK_BYTES = 128 * 16 + 32;
   static constexpr int A_BYTES = 16 * CHUNK_BYTES;
-  static constexpr int A_STAGES = BN == 64 ? 4 : 3;
+  static constexpr int A_STAGES = BN == 64 && !Q8 ? 4 : 3;
   static constexpr int BC = PAIR ? 128 : BN;                  // columns of the dense operand that a CTA brings in
   static constexpr int B_HALF = BC * 128;                     // 64 of the sum, one part
   static constexpr int B_STAGES = (BN == 64 && kSpans < 4) || (PAIR && kSpans == 1) ? 3 : 2;  // of two halves, which are filled and given back one by one
-  static constexpr int CODE_STAGES = PAIR ? (kSpans == 1 ? 2 : 3) : Q8 ? 2 : 4;
+  static constexpr int CODE_STAGES = PAIR ? (kSpans == 1 ? 2 : 3) : Q8 && BN == 128 ? 2 : 4;
   static constexpr int ACCS = BN == 256 ? 2 : 4;              // accumulators
   static constexpr int SCALE_SLOTS = ACCS + A_STAGES + 1;     // blocks; see the converters
   static constexpr int B_OFFSET = 0;
