@@ -13,6 +13,12 @@
 //
 // The dense operand is first laid out in panels (stage_panels_kernel), whatever its type, order and alignment: 128 columns x 32 of the
 // sum x 2 bytes in the core-matrix order that the MMA reads, so that the product brings them in with linear bulk copies.
+//
+// Bound by shared memory: a block of 128 x 128 codes and 128 columns moves 64 KB to the MMAs, 33 of expanded codes and 40 of copies in, and 8 out to
+// the converters, 1130 cycles at 128 bytes each; its MMAs take 520.  Tiles of 256 x 256 on two SMs do twice as many products with the same (1024
+// cycles of MMAs).  Measured: 512 tokens times 4096 x 4096, 128 tiles of 32 blocks, 25.5 us (670 TFLOP/s), 1000 tokens on pairs 38.8 (860), 8192 x 4096 x 4096
+// gradient 262 alone (1050).  Groups of 32 have four accumulators a block to fold, FP32 three times as many: 512 tokens 44 us, FP32 103, in groups of 128 56.
+// Few columns: by the codes' way from memory to operands; 8192 x 4096 gradient of rank 16 18.6 us (1.9 TB/s), 64 tokens times 4096 x 4096 12.9.
 #pragma once
 #include "tcec_codes.cuh"
 #include "tcec_codes_launch.h"
@@ -120,8 +126,8 @@ __device__ __forceinline__ bool mbar_wait_three(uint32_t a, uint32_t pa, uint32_
         : "=r"(ok)
         : "r"(a), "r"(pa), "r"(b), "r"(pb), "r"(c), "r"(pc)
         : "memory");
-    if (ok) return true;
-    if ((i & 0x3ff) == 0x3ff && *abortp) return false;
+    if (__all_sync(0xffffffffu, ok)) return true;
+    if ((i & 0x3ff) == 0x3ff && __any_sync(0xffffffffu, *abortp)) return false;
   }
   return false;
 }
@@ -361,100 +367,102 @@ __global__ void __launch_bounds__(GemmCodesCfg<BN, kSpans>::THREADS, 1) tcec_gem
         }
       }
     } else if (warp == 1) {
-      if (elect_one()) {
-        uint32_t as = 0, aph = 0, bs = 0, bph = 0;
-        bool ok = true;
-        if (!leader) {
-          // -------------------------------------------------------- peer: "my operands are there"
-          for (int tile = first_tile; tile < ntiles && ok; tile += stride)
-            for (int kb = 0; kb < nkb && ok; ++kb) {
-              if (!mbar_wait(smem_u32(&bar_a_full[as]), aph, abortp, 0)) {
+      const bool one = elect_one();  // which issues; all lanes go along, so that what it needs is the warp's
+      uint32_t as = 0, aph = 0, bs = 0, bph = 0;
+      bool ok = true;
+      if (!leader && one) {
+        // -------------------------------------------------------- peer: "my operands are there"
+        for (int tile = first_tile; tile < ntiles && ok; tile += stride)
+          for (int kb = 0; kb < nkb && ok; ++kb) {
+            if (!mbar_wait(smem_u32(&bar_a_full[as]), aph, abortp, 0)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_cluster(map_to_cta(smem_u32(&bar_a_full[as]), 0));
+            if (++as == Cfg::A_STAGES) as = 0, aph ^= 1;
+            for (int part = 0; part < p.parts; ++part) {
+              if (!mbar_wait(smem_u32(&bar_b_full[bs]), bph, abortp, 0)) {
                 ok = false;
                 break;
               }
-              mbar_arrive_cluster(map_to_cta(smem_u32(&bar_a_full[as]), 0));
-              if (++as == Cfg::A_STAGES) as = 0, aph ^= 1;
-              for (int part = 0; part < p.parts; ++part) {
-                if (!mbar_wait(smem_u32(&bar_b_full[bs]), bph, abortp, 0)) {
-                  ok = false;
-                  break;
-                }
-                mbar_arrive_cluster(map_to_cta(smem_u32(&bar_b_full[bs]), 0));
-                if (++bs == Cfg::B_STAGES) bs = 0, bph ^= 1;
-              }
-            }
-          if (!ok) give_up(kErrMmaWait);
-        } else {
-          // -------------------------------------------------------- MMAs
-          const uint64_t a_const = umma_desc_kmajor_noswizzle(0, Cfg::CHUNK_BYTES, 128), b_const = umma_desc_kmajor_noswizzle(0, 128, 512);
-          const uint32_t a16 = ((smem_base + Cfg::A_OFFSET) & 0x3ffff) >> 4, b16 = ((smem_base + Cfg::B_OFFSET) & 0x3ffff) >> 4;
-          uint32_t x = 0, xph = 0;  // the accumulator, and how often they all have been used
-          auto commit = [&](uint64_t* bar) {
-            if constexpr (kPair) umma_commit_pair(smem_u32(bar));
-            else umma_commit(smem_u32(bar));
-          };
-          for (int tile = first_tile; tile < ntiles && ok; tile += stride) {
-            const int cols = p.cols - code_tile(tile, tile_rows, p.col_tiles).col * BN;
-            const uint32_t idesc = umma_idesc(kF16 ? 0u : 1u, kPair ? 256 : 128, kPair ? 256 : min(BN, (cols + 15) & ~15));
-            for (int kb = 0; kb < nkb && ok; ++kb) {
-              const uint32_t a_here = a16 + as * (Cfg::A_BYTES >> 4);
-              for (int part = 0; part < p.parts; ++part) {
-                // the codes (waited for before), the dense operand, and the first accumulator if a new one begins
-                const uint32_t bfull = smem_u32(&bar_b_full[bs]);
-                const bool begins = kGroups > 1 || part == 0;
-                if (!mbar_wait_three(smem_u32(&bar_a_full[as]), aph, bfull, bph, begins ? smem_u32(&bar_acc_free[x]) : bfull,
-                                     begins ? xph ^ 1 : bph, abortp)) {
-                  ok = false;
-                  break;
-                }
-                tc_fence_after();
-                // Short loops: the issuing thread shares its instruction cache with four warps that are busy elsewhere, and unrolled what it
-                // does for a block took longer than the MMAs.
-                uint32_t da = a_here, db = b16 + bs * (2 * Cfg::B_HALF >> 4);
-                uint32_t more = kGroups == 1 && part > 0;  // an accumulator holds one group; where a block is one, all parts of it
-#pragma unroll 1
-                for (int h = 0; h < 2; ++h) {
-#pragma unroll 1
-                  for (int j = 0; j < 2; ++j) {  // 32 of the sum
-                    if (kGroups == 4 && h + j > 0 || kGroups == 2 && h > 0 && j == 0) {
-                      if (!mbar_wait(smem_u32(&bar_acc_free[x]), xph ^ 1, abortp, 0)) {
-                        ok = false;
-                        break;
-                      }
-                      tc_fence_after();
-                      more = 0;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                      if constexpr (kPair) umma_ss_pair<false>(tmem + x * BN, a_const | da, b_const | (db + i * 16), idesc, more);
-                      else umma_ss<false>(tmem + x * BN, a_const | da, b_const | (db + i * 16), idesc, more);
-                      da += 2 * Cfg::CHUNK_BYTES >> 4;
-                      more = 1;
-                    }
-                    db += Cfg::BC * 64 >> 4;
-                    if (kGroups == 4 || kGroups == 2 && j == 1) {
-                      commit(&bar_acc_full[x]);
-                      if (++x == Cfg::ACCS) x = 0, xph ^= 1;
-                    }
-                  }
-                  if (!ok) break;
-                  if (h == 0) commit(&bar_b_empty[2 * bs]);
-                }
-                if (!ok) break;
-                commit(&bar_b_empty[2 * bs + 1]);
-                if (++bs == Cfg::B_STAGES) bs = 0, bph ^= 1;
-              }
-              if (!ok) break;
-              if (kGroups == 1) {
-                commit(&bar_acc_full[x]);
-                if (++x == Cfg::ACCS) x = 0, xph ^= 1;
-              }
-              commit(&bar_a_empty[as]);
-              if (++as == Cfg::A_STAGES) as = 0, aph ^= 1;
+              mbar_arrive_cluster(map_to_cta(smem_u32(&bar_b_full[bs]), 0));
+              if (++bs == Cfg::B_STAGES) bs = 0, bph ^= 1;
             }
           }
-          if (!ok) mma_thread_gave_up<kPair>(&abort_flag, p.status, kErrMmaWait, &bar_drain[0]);
+        if (!ok) give_up(kErrMmaWait);
+      } else if (leader) {
+        // -------------------------------------------------------- MMAs
+        const uint64_t a_const = umma_desc_kmajor_noswizzle(0, Cfg::CHUNK_BYTES, 128), b_const = umma_desc_kmajor_noswizzle(0, 128, 512);
+        const uint32_t a16 = ((smem_base + Cfg::A_OFFSET) & 0x3ffff) >> 4, b16 = ((smem_base + Cfg::B_OFFSET) & 0x3ffff) >> 4;
+        uint32_t x = 0, xph = 0;  // the accumulator, and how often they all have been used
+        auto commit = [&](uint64_t* bar) {
+          if (!one) return;
+          if constexpr (kPair) umma_commit_pair(smem_u32(bar));
+          else umma_commit(smem_u32(bar));
+        };
+        for (int tile = first_tile; tile < ntiles && ok; tile += stride) {
+          const int cols = p.cols - code_tile(tile, tile_rows, p.col_tiles).col * BN;
+          const uint32_t idesc = umma_idesc(kF16 ? 0u : 1u, kPair ? 256 : 128, kPair ? 256 : min(BN, (cols + 15) & ~15));
+          for (int kb = 0; kb < nkb && ok; ++kb) {
+            const uint32_t a_here = a16 + as * (Cfg::A_BYTES >> 4);
+            for (int part = 0; part < p.parts; ++part) {
+              // the codes (waited for before), the dense operand, and the first accumulator if a new one begins
+              const uint32_t bfull = smem_u32(&bar_b_full[bs]);
+              const bool begins = kGroups > 1 || part == 0;
+              if (!mbar_wait_three(smem_u32(&bar_a_full[as]), aph, bfull, bph, begins ? smem_u32(&bar_acc_free[x]) : bfull,
+                                   begins ? xph ^ 1 : bph, abortp)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              // Short loops: the issuing thread shares its instruction cache with four warps that are busy elsewhere, and unrolled what it
+              // does for a block took longer than the MMAs.
+              uint32_t da = a_here, db = b16 + bs * (2 * Cfg::B_HALF >> 4);
+              uint32_t more = kGroups == 1 && part > 0;  // an accumulator holds one group; where a block is one, all parts of it
+#pragma unroll 1
+              for (int h = 0; h < 2; ++h) {
+#pragma unroll 1
+                for (int j = 0; j < 2; ++j) {  // 32 of the sum
+                  if (kGroups == 4 && h + j > 0 || kGroups == 2 && h > 0 && j == 0) {
+                    if (!mbar_wait_lanes(smem_u32(&bar_acc_free[x]), xph ^ 1, abortp)) {
+                      ok = false;
+                      break;
+                    }
+                    tc_fence_after();
+                    more = 0;
+                  }
+#pragma unroll
+                  for (int i = 0; i < 2; ++i) {
+                    if (one) {
+                      if constexpr (kPair) umma_ss_pair<false>(tmem + x * BN, a_const | da, b_const | (db + i * 16), idesc, more);
+                      else umma_ss<false>(tmem + x * BN, a_const | da, b_const | (db + i * 16), idesc, more);
+                    }
+                    da += 2 * Cfg::CHUNK_BYTES >> 4;
+                    more = 1;
+                  }
+                  db += Cfg::BC * 64 >> 4;
+                  if (kGroups == 4 || kGroups == 2 && j == 1) {
+                    commit(&bar_acc_full[x]);
+                    if (++x == Cfg::ACCS) x = 0, xph ^= 1;
+                  }
+                }
+                if (!ok) break;
+                if (h == 0) commit(&bar_b_empty[2 * bs]);
+              }
+              if (!ok) break;
+              commit(&bar_b_empty[2 * bs + 1]);
+              if (++bs == Cfg::B_STAGES) bs = 0, bph ^= 1;
+            }
+            if (!ok) break;
+            if (kGroups == 1) {
+              commit(&bar_acc_full[x]);
+              if (++x == Cfg::ACCS) x = 0, xph ^= 1;
+            }
+            commit(&bar_a_empty[as]);
+            if (++as == Cfg::A_STAGES) as = 0, aph ^= 1;
+          }
         }
+        if (!ok && one) mma_thread_gave_up<kPair>(&abort_flag, p.status, kErrMmaWait, &bar_drain[0]);
       }
     }
   } else if (warp < 4 + Cfg::CONVERTERS) {
