@@ -256,9 +256,10 @@ int tcec_split(const float* in, float* hi, float* lo, size_t count, int policy, 
  *
  * Packed buffers and workspaces are the caller's, in device memory and aligned to 16 bytes; the calls allocate nothing, so each captured
  * graph may have a workspace of its own.  A workspace may be used again as soon as the stream has passed the call.  Results must not overlap
- * operands or workspace (TCEC_ERR_INVALID_ARGUMENT), and nothing outside a result's rows and columns is written.  Sizes may be zero; a sum over
- * nothing, or alpha == 0, gives beta * C; beta == 0 never reads C.  The "path", tile and other options of the FP32 products have no
- * effect here, "reserve_sms" included.  A bounded wait that ran out is reported by tcec_device_status.
+ * operands or workspace (TCEC_ERR_INVALID_ARGUMENT; lines of one matrix between those of another are no overlap), and nothing outside a
+ * result's rows and columns is written.  Sizes may be zero; a sum over nothing, or alpha == 0, gives beta * C; beta == 0 never reads C.  Of the
+ * options "reserve_sms" holds for gradients and for more than few tokens, which are then not divided among SMs (the last bits may be others); the
+ * others have no effect here.  A bounded wait that ran out is reported by tcec_device_status.
  */
 #define TCEC_TYPE_F32 0
 #define TCEC_TYPE_F16 1
@@ -287,7 +288,9 @@ int tcec_unpack_q4(int layout_w, int n, int k, const void* packed, int group, vo
 /*
  * C (m x n) = alpha * X (m x k) * W^T + beta * C for weights packed as above: the product of a linear layer, from one token (a
  * matrix-vector product, bound by the 4-bit weights) to a whole prompt.  type_c is type_x or FP32.  `workspace` takes
- * tcec_gemm_q4_workspace_bytes(m, n, k, type_x) bytes, which is 0 for few tokens (it may then be NULL).
+ * tcec_gemm_q4_workspace_bytes(m, n, k, type_x) bytes, which is 0 up to one token (it may then be NULL).
+ * The sum over a group of codes times X has to fit FP32.  Up to 32 tokens (FP32: 10) code and zero point are multiplied apart: the error is then
+ * relative to the sum of |s| (q + z) |x| instead of |s| |q - z| |x|, and values of X of 2^122 and more count as infinite.
  */
 size_t tcec_gemm_q4_workspace_bytes(int m, int n, int k, int type_x);
 int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, const void* x, long long ldx, int type_x,

@@ -582,3 +582,44 @@ def test_packing_and_product_one_after_the_other_without_a_wait():
         check(y, exact, bound(x.double().abs() @ wq.abs().T, exact, BF16, k, 1))
         exact = y.double().T @ (q * s)
         check(g, exact, bound(y.double().abs().T @ (q * s).abs(), exact, F32, 3 + i, 1))
+
+
+def test_operands_and_result_side_by_side_in_one_matrix():
+    x, packed, exact, tol = product_case(6, 96, 160, 32, F32, 51)
+    whole = torch.full((6, 300), 7.0, device=DEV)
+    whole[:, 10:170] = x
+    check(tcec.gemm_q4(whole[:, 10:170], packed, 96, whole[:, 180:276], group=32), exact, tol)
+    assert (whole[:, 170:180] == 7.0).all() and (whole[:, 276:] == 7.0).all() and torch.equal(whole[:, 10:170], x)
+    for c in (whole[:, 169:265], whole[:, :96]):
+        with pytest.raises(tcec.TcecError):
+            tcec.gemm_q4(whole[:, 10:170], packed, 96, c, group=32)
+
+
+def test_with_sms_left_to_others():
+    lib = tcec.load()
+    x, packed, exact, tol = product_case(40, 300, 4096, 128, BF16, 53)
+    y, packed2, exact2, tol2 = product_case(1350, 2170, 300, 128, BF16, 55)
+    assert lib.tcec_set_option(b"reserve_sms", 20) == 0
+    try:
+        check(tcec.gemm_q4(x, packed, 300), exact, tol)
+        check(tcec.gemm_q4(y, packed2, 2170), exact2, tol2)
+    finally:
+        lib.tcec_set_option(b"reserve_sms", 0)
+
+
+def test_python_and_the_native_binding_agree(monkeypatch):
+    x, packed, _, _ = product_case(12, 130, 300, 64, BF16, 57)
+    w, dy = randn(130, 300, seed=1), randn(12, 50, seed=2)
+
+    def all_calls():
+        p, q = tcec.pack_q4(w, 64), tcec.pack_q8(w)
+        c, g = torch.ones(12, 130, device=DEV), torch.ones(300, 50, device=DEV).T
+        return [p, q, tcec.unpack_q4(p, 130, 300, 64, BF16), tcec.unpack_q8(q, 130, 300), tcec.gemm_q4(x, packed, 130, group=64),
+                tcec.gemm_q4(x, packed, 130, c, group=64, alpha=2.0, beta=-1.0), tcec.wgrad_q8(dy, tcec.pack_q8(w[:12]), 300),
+                tcec.wgrad_q8(dy, tcec.pack_q8(w[:12]), 300, g, beta=1.0), tcec.gemm_q4(x, packed, 130, group=64, dtype=F32)]
+
+    assert tcec._binding is not None
+    native = all_calls()
+    monkeypatch.setattr(tcec, "_binding", None)
+    for a, b in zip(native, all_calls()):
+        assert a.dtype == b.dtype and a.stride() == b.stride() and torch.equal(a, b)

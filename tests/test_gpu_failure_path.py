@@ -164,3 +164,59 @@ def test_waits_of_the_pair_kernel_run_out_the_same_way(long, policy):
         for name, value in ((b"debug_flags", 0), (b"cta_pair", -1), (b"half_tiles", 1)):
             lib.tcec_set_option(name, value)
         lib.tcec_destroy()
+
+
+# m, n, k (tokens, outputs, inputs): one token, tokens staged, tiles of 64 columns divided by eight, of 128 undivided, pairs
+@pytest.mark.parametrize("m,n,k", [(1, 300, 4096), (12, 300, 4096), (40, 300, 4096), (100, 300, 300), (1350, 2170, 700)])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_waits_of_the_products_of_codes_run_out_the_same_way(m, n, k, bits):
+    """For 8 bits n outputs are the tokens summed over and m the columns, so that the kernels and the division are the same."""
+    lib, i = _library(), ctypes.c_int
+    ll, f, p, sz = ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
+    lib.tcec_gemm_q4_workspace_bytes.argtypes = lib.tcec_wgrad_q8_workspace_bytes.argtypes = [i, i, i, i]
+    lib.tcec_gemm_q4_workspace_bytes.restype = lib.tcec_wgrad_q8_workspace_bytes.restype = sz
+    lib.tcec_q4_bytes.argtypes, lib.tcec_q8_bytes.argtypes = [i, i, i], [i, i]
+    lib.tcec_q4_bytes.restype = lib.tcec_q8_bytes.restype = sz
+    lib.tcec_pack_q4.argtypes = [i, i, i, p, ll, i, i, i, p, p]
+    lib.tcec_pack_q8.argtypes = [i, i, i, p, ll, i, p, p]
+    lib.tcec_gemm_q4.argtypes = [i, i, i, i, i, f, p, ll, i, p, i, f, p, ll, i, p, sz, p]
+    lib.tcec_wgrad_q8.argtypes = [i, i, i, i, i, f, p, ll, i, p, f, p, ll, i, p, sz, p]
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    detail = i(0)
+    if bits == 4:
+        w = torch.randn(n, k, device="cuda", generator=gen)
+        x = torch.randn(m, k, device="cuda", generator=gen).bfloat16()
+        packed = torch.empty(lib.tcec_q4_bytes(n, k, 128), dtype=torch.uint8, device="cuda")
+        assert lib.tcec_pack_q4(0, n, k, w.data_ptr(), k, 0, 128, 1, packed.data_ptr(), None) == 0
+        need = lib.tcec_gemm_q4_workspace_bytes(m, n, k, 2)
+        c = torch.full((m, n), 5.0, device="cuda")
+    else:
+        tokens, features = k, n
+        w = torch.randn(tokens, features, device="cuda", generator=gen)
+        x = torch.randn(tokens, m, device="cuda", generator=gen).bfloat16()
+        packed = torch.empty(lib.tcec_q8_bytes(tokens, features), dtype=torch.uint8, device="cuda")
+        assert lib.tcec_pack_q8(0, tokens, features, w.data_ptr(), features, 0, packed.data_ptr(), None) == 0
+        need = lib.tcec_wgrad_q8_workspace_bytes(tokens, m, features, 2)
+        c = torch.full((m, features), 5.0, device="cuda")
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+
+    def run():
+        if bits == 4:
+            st = lib.tcec_gemm_q4(0, 0, m, n, k, 1.0, x.data_ptr(), k, 2, packed.data_ptr(), 128, 0.0, c.data_ptr(), n, 0, ws.data_ptr(), need, None)
+        else:
+            st = lib.tcec_wgrad_q8(0, 0, k, m, n, 1.0, x.data_ptr(), m, 2, packed.data_ptr(), 0.0, c.data_ptr(), n, 0, ws.data_ptr(), need, None)
+        return st or lib.tcec_device_status(ctypes.byref(detail))
+
+    try:
+        assert run() == 0
+        want = c.clone()
+        assert not bool((want == 5.0).any())
+        assert lib.tcec_set_option(b"debug_flags", 128) == 0  # one block of codes never comes
+        c.fill_(5.0)
+        assert run() == ERR_TIMEOUT
+        assert bool((c == 5.0).any()) and bool(((c == 5.0) | (c == want)).all())  # whole, or untouched
+        assert lib.tcec_set_option(b"debug_flags", 0) == 0
+        assert run() == 0 and torch.equal(c, want)
+    finally:
+        lib.tcec_set_option(b"debug_flags", 0)
+        lib.tcec_destroy()

@@ -97,8 +97,9 @@ __device__ __forceinline__ bool mbar_wait_plain(uint32_t bar, uint32_t parity) {
 // ---------------------------------------------------------------- programmatic dependent launch
 // Splits and GEMM kernels are launched so that they may be set up while the kernel before them ends: their CTAs take SMs that are
 // done, initialise barriers, allocate TMEM.  None touches global memory before this wait, which returns when the kernel before has
-// ended and what it wrote is visible.  Every thread of every such kernel comes here, whatever it does afterwards: a kernel that
-// left without would let the next one start on the results of the one before.  Calls in a row, us, plain launches against this:
+// ended and what it wrote is visible, but for codes behind a kernel that has waited itself (tcec_gemm_codes.cuh).  Threads of every CTA of
+// every such kernel come here, whatever they do afterwards: a kernel that left without would let the next one start on the results of
+// the one before.  Calls in a row, us, plain launches against this:
 // 512^3 12.3, 8.8; 1024^3 20.3, 14.6; 1000 x 777 x 1111 20.5, 16.9; 1500 x 1400 x 300 14.4, 10.8.
 __device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // The next kernel of the stream may be set up as soon as every CTA of this one has come here (or ended).  The splits call it: the

@@ -50,6 +50,16 @@ bool overlap(const void* a, size_t na, const void* b, size_t nb) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
   return na && nb && x < y + nb && y < x + na;
 }
+// Lines of one matrix may lie between those of another, as parts of a wider one.
+bool overlap(const Dense& a, const Dense& b) {
+  if (!overlap(a.p, a.extent(), b.p, b.extent())) return false;
+  const size_t pitch = static_cast<size_t>(a.ld) * type_bytes(a.type);
+  if (pitch != static_cast<size_t>(b.ld) * type_bytes(b.type)) return true;
+  auto line = [](const Dense& d) { return static_cast<size_t>(d.layout == TCEC_ROW_MAJOR ? d.cols : d.rows) * type_bytes(d.type); };
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  const size_t off = x <= y ? (y - x) % pitch : (pitch - (x - y) % pitch) % pitch;  // of b's lines behind a's
+  return off < line(a) || off + line(b) > pitch;
+}
 
 size_t q4_bytes(int n, int k, int group) {
   return static_cast<size_t>(ceil_div(n, kCodeRows)) * ceil_div(k, kCodeSpan) * q4_block_bytes(group);
@@ -60,12 +70,14 @@ size_t panel_bytes(int cols, int sum, int type) {
   return static_cast<size_t>(ceil_div(cols, kCodeRows)) * ceil_div(sum, kCodeSpan) * (type == TCEC_TYPE_F32 ? 3 : 1) * kSpanBytes;
 }
 
-// What a launch needs to know of the current device.
+// What a launch needs to know of the current device, and of the options.
 struct Here {
   int* status;
   int sm_count;
+  int reserve_sms, debug_flags;
 };
 int get_here(Here* out) {
+  const Options opt = snapshot_options();
   std::lock_guard<std::mutex> lock(state_mutex());
   DeviceState* st = nullptr;
   const int rc = get_device_state(&st);
@@ -75,7 +87,7 @@ int get_here(Here* out) {
     TCEC_CUDA(set_gemv_q4_attrs());
     st->codes_attrs_done = true;
   }
-  *out = {st->status, st->sm_count};
+  *out = {st->status, st->sm_count, opt.reserve_sms, opt.debug_flags};
   return TCEC_OK;
 }
 
@@ -132,7 +144,9 @@ template <int T>
 struct StagePanels {
   static void go(int grid, cudaStream_t stream, const StagePanelsParams& p) { launch_early(stage_panels_kernel<T>, dim3(grid, 2), 256, 0, stream, p); }
 };
-// D[row][col] of tcec_gemm_codes.cuh for an operand of codes (spans: groups of 4-bit codes in a block, 0: 8-bit codes) and a dense one whose columns and sum lie at the given steps.
+
+// D[row][col] of tcec_gemm_codes.cuh for an operand of codes (spans: groups of 4-bit codes in a block, 0: 8-bit codes) and a dense one whose
+// columns and sum lie at the given steps.
 int gemm_codes(const void* codes, int spans, int rows, int cols, int sum, const void* dense, long long col_step, long long sum_step,
                int type, bool vec, float alpha, float beta, void* c, long long c_row, long long c_col, int c_type, void* workspace,
                const Here& here, cudaStream_t stream) {
@@ -165,6 +179,7 @@ int gemm_codes(const void* codes, int spans, int rows, int cols, int sum, const 
   gp.c_col = c_col;
   gp.c_type = c_type;
   gp.status = here.status;
+  gp.debug_flags = here.debug_flags;
   // Pairs of SMs with 256 columns make the most of each converted weight, but are half as many: they are taken where tiles of 128 columns would be
   // more than the SMs (4096 x 4096: 512 tokens, 128 such tiles, 25.8 us, in pairs 36.0; 768 tokens, 192 tiles, 43.4 and 35.7; 1000 45.2 and 38.9).
   int bn = cols <= 64 ? 64 : 128;
@@ -177,9 +192,10 @@ int gemm_codes(const void* codes, int spans, int rows, int cols, int sum, const 
   // 16 clusters of eight took two rounds where 15 took one (64 columns of 4096: 2048 rows 17.5 us, 1920 rows 9.8; with clusters of four 11.0);
   // of four, 35 did and 33 did not (4480 rows 22.1, 4224 rows 12.8).  Constants, as the order of the sums is to follow from sizes alone.
   constexpr long long kMostClusters[4] = {0, 74, 32, 14};  // of 2, 4 and 8 CTAs
-  while (bn < 256 && ctas < 8 && tiles <= kMostClusters[ctas == 1 ? 1 : ctas == 2 ? 2 : 3] && blocks >= 4 * ctas) ctas *= 2;
+  while (bn < 256 && ctas < 8 && !here.reserve_sms && tiles <= kMostClusters[ctas == 1 ? 1 : ctas == 2 ? 2 : 3] && blocks >= 4 * ctas) ctas *= 2;
   // One cluster a tile where the sum is divided; else as many as run at a time.
-  const long long most = bn == 256 ? here.sm_count / 2 : ctas > 1 ? tiles : here.sm_count;
+  const int sms = here.sm_count - here.reserve_sms;
+  const long long most = bn == 256 ? sms / 2 : ctas > 1 ? tiles : sms;
   const int grid = static_cast<int>(tiles < most ? tiles : most) * ctas;
   launch_gemm_codes(type == TCEC_TYPE_F16, spans, bn, gp, ctas, grid, stream);
   return launched();
@@ -307,7 +323,7 @@ int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, c
     if (sum) {
       if (dx.bad_memory() || !packed || !aligned(packed, 16) || workspace_bytes < scratch || (scratch && (!workspace || !aligned(workspace, 16))))
         return TCEC_ERR_INVALID_ARGUMENT;
-      if (overlap(c, dc.extent(), x, dx.extent()) || overlap(c, dc.extent(), packed, q4_bytes(n, k, group)) ||
+      if (overlap(dc, dx) || overlap(c, dc.extent(), packed, q4_bytes(n, k, group)) ||
           overlap(workspace, scratch, x, dx.extent()) || overlap(workspace, scratch, c, dc.extent()) ||
           overlap(workspace, scratch, packed, q4_bytes(n, k, group)))
         return TCEC_ERR_INVALID_ARGUMENT;
@@ -352,7 +368,7 @@ int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, c
     p.c_row = dc.col_step();
     p.c_type = type_c;
     p.status = here.status;
-    if (m > 1 && !blocks) return gemm_codes(packed, kCodeSpan / group, n, m, 0, x, 0, 0, type_x, false, alpha, beta, c, dc.col_step(), dc.row_step(), type_c, workspace, here, on);
+    p.debug_flags = here.debug_flags;
     launch_gemv_q4(type_x, group, eights, p, on);
     return launched();
   });
@@ -426,7 +442,7 @@ int tcec_wgrad_q8(int layout_dy, int layout_c, int m, int n, int k, float alpha,
     if (sum) {
       if (dd.bad_memory() || !packed || !aligned(packed, 16) || workspace_bytes < scratch || !workspace || !aligned(workspace, 16))
         return TCEC_ERR_INVALID_ARGUMENT;
-      if (overlap(c, dc.extent(), dy, dd.extent()) || overlap(c, dc.extent(), packed, q8_bytes(m, k)) ||
+      if (overlap(dc, dd) || overlap(c, dc.extent(), packed, q8_bytes(m, k)) ||
           overlap(workspace, scratch, dy, dd.extent()) || overlap(workspace, scratch, c, dc.extent()) ||
           overlap(workspace, scratch, packed, q8_bytes(m, k)))
         return TCEC_ERR_INVALID_ARGUMENT;

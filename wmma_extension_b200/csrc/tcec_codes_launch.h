@@ -17,6 +17,7 @@ struct GemmCodesParams {
   long long c_row, c_col;     // steps between elements of C along rows and columns of this product
   int c_type;
   int* status;
+  int debug_flags;            // develop builds only: bit 7 = a block of codes is never filled, in the last CTA of the first cluster
 };
 
 struct GemvQ4Params {
@@ -31,6 +32,7 @@ struct GemvQ4Params {
   long long c_token, c_row;
   int c_type;
   int* status;
+  int debug_flags;            // develop builds only: bit 7 = the first block of codes is never filled, in the first CTA
 };
 
 }  // namespace tcec_sm100

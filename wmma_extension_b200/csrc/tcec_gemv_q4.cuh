@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
   constexpr size_t kBlockBytes = q4_block_bytes(kGroup);
   const uint8_t* codes = p.codes + static_cast<size_t>(row0 / kCodeRows) * p.blocks * kBlockBytes + row0 % kCodeRows / 16 * q4_strip_bytes(kGroup);
   auto fetch = [&](int kb, int stage) {  // lane 0
+    if (dev_flag(p.debug_flags, 128) && blockIdx.x == 0 && kb == 0) return;
     const uint32_t bar = smem_u32(&bars[warp][stage]);
     mbar_arrive_expect_tx(bar, Cfg::STAGE_BYTES);
     bulk_load(smem_u32(ring + stage * Cfg::STAGE_BYTES), codes + kb * kBlockBytes, Cfg::STAGE_BYTES, bar);
