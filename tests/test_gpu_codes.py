@@ -69,7 +69,7 @@ def values(w, group, scale):
 SIZES = [(1, 1), (1, 128), (7, 33), (16, 96), (128, 128), (129, 257), (300, 1000)]
 
 
-@pytest.mark.parametrize("n,k", SIZES)
+@pytest.mark.parametrize("n,k", SIZES + [(2500, 4001)])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("dtype,scale", [(F32, F16), (F16, BF16), (BF16, F16)])
 def test_weights_go_to_the_nearest_of_16_steps(n, k, group, dtype, scale):

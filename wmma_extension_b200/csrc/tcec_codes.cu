@@ -111,10 +111,15 @@ void by_type(int type, const Args&... args) {
 
 template <int T>
 struct PackQ4 {
+  template <int G>
+  static void of(int grid, cudaStream_t stream, const PackQ4Params& p) {
+    if (grid <= 148 * 4) launch_early(pack_q4_kernel<T, G, 1>, grid, 512, 0, stream, p);
+    else launch_early(pack_q4_kernel<T, G, 2>, grid, 256, 0, stream, p);
+  }
   static void go(int group, int grid, cudaStream_t stream, const PackQ4Params& p) {
-    if (group == 32) launch_early(pack_q4_kernel<T, 32>, grid, 256, 0, stream, p);
-    else if (group == 64) launch_early(pack_q4_kernel<T, 64>, grid, 256, 0, stream, p);
-    else launch_early(pack_q4_kernel<T, 128>, grid, 256, 0, stream, p);
+    if (group == 32) of<32>(grid, stream, p);
+    else if (group == 64) of<64>(grid, stream, p);
+    else of<128>(grid, stream, p);
   }
 };
 template <int T>

@@ -224,17 +224,19 @@ struct PackQ4Params {
 __device__ __forceinline__ uint32_t q4_entry(float s, int z) { return (__float_as_uint(s) & ~15u) | static_cast<uint32_t>(z); }
 
 // One CTA a block.  A warp takes eight rows at a time, four lanes a row: lane 4 g + t has k = 16 j + 4 t .. + 3 of row g for j < 8, so a
-// group is two exchanges away at most.  Words gather in shared memory and leave together.
-template <int kType, int kGroup>
-__global__ void __launch_bounds__(256) pack_q4_kernel(const PackQ4Params p) {
+// group is two exchanges away at most.  Words gather in shared memory and leave together.  Of few blocks a warp takes eight rows, of many (up to 592 are
+// under way at a time) two times eight, in CTAs of which more fit an SM: 1000 x 1024 in groups of 32 4.2 us, 5.5 with sixteen rows a warp, 2048 x 2048 6.9 and 8.0,
+// 4096 x 4096 in groups of 128 27 and 24.5.
+template <int kType, int kGroup, int kHalves>
+__global__ void __launch_bounds__(512 / kHalves) pack_q4_kernel(const PackQ4Params p) {
   constexpr int kSpans = kCodeSpan / kGroup;
   __shared__ __align__(16) uint32_t words[2048 + 128 * kSpans];
   wait_for_launch_before();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int kb = blockIdx.x % p.blocks, tile = blockIdx.x / p.blocks;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = warp * 16 + half * 8 + g, row = tile * kCodeRows + r, k0 = kb * kCodeSpan + t * 4;
+  for (int half = 0; half < kHalves; ++half) {
+    const int r = warp * 8 * kHalves + half * 8 + g, row = tile * kCodeRows + r, k0 = kb * kCodeSpan + t * 4;
     float v[8][4];
     const int left = row < p.n ? p.k - k0 : 0;
     if (p.vec && left >= 7 * 16 + 4) {
@@ -257,7 +259,7 @@ __global__ void __launch_bounds__(256) pack_q4_kernel(const PackQ4Params p) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j][0] = v[j][1] = v[j][2] = v[j][3] = 0.f;
     }
-    if (half == 1) let_next_launch_start();
+    if (half == kHalves - 1) let_next_launch_start();
 #pragma unroll
     for (int q = 0; q < kSpans; ++q) {  // groups; 128 / kSpans = 16 * 8 / kSpans
       float lo = 0.f, hi = 0.f;
@@ -303,7 +305,7 @@ __global__ void __launch_bounds__(256) pack_q4_kernel(const PackQ4Params p) {
   }
   __syncthreads();
   uint4* out = reinterpret_cast<uint4*>(p.packed + (static_cast<size_t>(tile) * p.blocks + kb) * q4_block_bytes(kGroup));
-  for (int i = threadIdx.x; i < q4_block_bytes(kGroup) / 16; i += 256) out[i] = reinterpret_cast<const uint4*>(words)[i];
+  for (int i = threadIdx.x; i < q4_block_bytes(kGroup) / 16; i += 512 / kHalves) out[i] = reinterpret_cast<const uint4*>(words)[i];
 }
 
 // Lays out codes that the caller has.
