@@ -623,3 +623,31 @@ def test_python_and_the_native_binding_agree(monkeypatch):
     monkeypatch.setattr(tcec, "_binding", None)
     for a, b in zip(native, all_calls()):
         assert a.dtype == b.dtype and a.stride() == b.stride() and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("m,k", [(1, 2400), (130, 2369), (3000, 1000), (4100, 2700), (700, 9000)])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_gradients_of_few_columns(m, k, dtype):
+    for n in (1, 2, 3, 5, 8, 10, 11, 16, 17, 32, 33):
+        dy, packed, exact, tol = gradient_case(m, n, k, dtype, m + n)
+        check(tcec.wgrad_q8(dy, packed, k), exact, tol)
+        c = randn(n, k, seed=n)
+        want = exact - 2.0 * c.double()
+        check(tcec.wgrad_q8(dy.T.contiguous().T, packed, k, c, beta=-2.0), want, tol + want.abs() * 2.0**-22 + exact.abs() * 2.0**-22)
+    tcec.device_status()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradients_of_any_magnitude(dtype):
+    """As tokens of any magnitude: a column's power of two is of its largest value in a block."""
+    m, n, k = 300, 6, 200
+    dy, packed, exact, tol = gradient_case(m, n, k, dtype, 61, F32)
+    for exponent in (-110 if dtype == BF16 else -90, -61, -59, 26, 28, 100):
+        got = tcec.wgrad_q8((dy.double() * 2.0**exponent).to(dtype), packed, k, dtype=F32).double() * 2.0**-exponent
+        check(got, exact, tol)
+    bad = dy.clone()
+    bad[5, 2], bad[200, 4] = float("nan"), float("inf")
+    got = tcec.wgrad_q8(bad, packed, k, dtype=F32)
+    clean = tcec.wgrad_q8(dy, packed, k, dtype=F32)
+    keep = [0, 1, 3, 5]
+    assert got[2].isnan().all() and not got[4].isfinite().any() and torch.equal(got[keep], clean[keep])

@@ -85,6 +85,7 @@ int get_here(Here* out) {
   if (!st->codes_attrs_done) {
     TCEC_CUDA(set_gemm_codes_attrs());
     TCEC_CUDA(set_gemv_q4_attrs());
+    TCEC_CUDA(set_gemv_q8_attrs());
     st->codes_attrs_done = true;
   }
   *out = {st->status, st->sm_count, opt.reserve_sms, opt.debug_flags};
@@ -212,6 +213,9 @@ int gemm_codes(const void* codes, int spans, int rows, int cols, int sum, const 
 // tiles has three parts to bring in: 10 tokens times 16384 x 16384 94 us, 11 160.
 long long columns_of(int m, int type) { return static_cast<long long>(m) * (type == TCEC_TYPE_F32 ? 3 : 1); }
 bool streamed(int m, int n, int type) { return columns_of(m, type) <= (n <= 8192 || type == TCEC_TYPE_F32 ? 32 : 16); }
+// Whether a gradient has so few columns that the activations are streamed (tcec_gemv_q8.cuh), by the same reasons: 8192 x 4096 of rank 16 12.8 us, in
+// tiles 18.3; of rank 32 20.5 and 18.6, 8192 x 1024 13.2 and 13.1, 1024 x 1024 5.4 and 7.8; FP32 of rank 10 18.8 and 29.3, 4096 x 16384 36 and 47.
+bool few_columns(int n, int k, int type) { return columns_of(n, type) <= (k <= 148 * 16 || type == TCEC_TYPE_F32 ? 32 : 16); }
 int eights_of(int m, int type) { return columns_of(m, type) <= 8 ? 1 : columns_of(m, type) <= 16 ? 2 : 4; }
 
 }  // namespace
@@ -432,7 +436,9 @@ int tcec_unpack_q8(int layout_x, int m, int k, const void* packed, void* x, long
 }
 
 size_t tcec_wgrad_q8_workspace_bytes(int m, int n, int k, int type_dy) {
-  return m < 0 || n < 0 || k < 0 || bad_type(type_dy) ? 0 : panel_bytes(n, m, type_dy);
+  if (m < 0 || n < 0 || k < 0 || bad_type(type_dy)) return 0;
+  if (few_columns(n, k, type_dy)) return static_cast<size_t>(staged_bytes(ceil_div(m, kCodeSpan), eights_of(n, type_dy)));
+  return panel_bytes(n, m, type_dy);
 }
 
 int tcec_wgrad_q8(int layout_dy, int layout_c, int m, int n, int k, float alpha, const void* dy, long long lddy, int type_dy, const void* packed,
@@ -457,6 +463,38 @@ int tcec_wgrad_q8(int layout_dy, int layout_c, int m, int n, int k, float alpha,
     const int rc = get_here(&here);
     if (rc != TCEC_OK) return rc;
     // columns: the outputs of the layer; the sum: tokens
+    if (sum && few_columns(n, k, type_dy)) {
+      const cudaStream_t on = static_cast<cudaStream_t>(stream);
+      const int blocks = static_cast<int>(ceil_div(sum, kCodeSpan)), eights = eights_of(n, type_dy);
+      StageColumnsParams sp{};
+      sp.src = dy;
+      sp.col_step = dd.col_step();
+      sp.sum_step = dd.row_step();
+      sp.tokens = n;
+      sp.sum = sum;
+      sp.blocks = blocks;
+      sp.eights = eights;
+      sp.group = kCodeSpan;
+      sp.out = static_cast<uint8_t*>(workspace);
+      sp.vec = layout_dy == TCEC_COL_MAJOR && dd.wide(16);
+      by_type<StageColumns>(type_dy, on, sp);
+      GemvQ8Params p{};
+      p.codes = static_cast<const uint8_t*>(packed);
+      p.staged = static_cast<const uint8_t*>(workspace);
+      p.rows = k;
+      p.cols = n;
+      p.blocks = blocks;
+      p.alpha = alpha;
+      p.beta = beta;
+      p.c = c;
+      p.c_row = dc.col_step();
+      p.c_col = dc.row_step();
+      p.c_type = type_c;
+      p.status = here.status;
+      p.debug_flags = here.debug_flags;
+      launch_gemv_q8(type_dy, eights, p, on);
+      return launched();
+    }
     return gemm_codes(packed, 0, k, n, sum, dy, dd.col_step(), dd.row_step(), type_dy, layout_dy == TCEC_COL_MAJOR && dd.wide(16), alpha,
                       beta, c, dc.col_step(), dc.row_step(), type_c, workspace, here, static_cast<cudaStream_t>(stream));
   });

@@ -10,13 +10,6 @@ namespace tcec_host {
 namespace {
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
-// As many warps divide the k of a CTA's rows as let all CTAs run at a time: a second round of them would leave SMs idle at its end, and as every CTA
-// goes through all of k it is long (13 tokens times 5000 x 7001: 16.7 us, 19.8 with eight warps whatever the rows).  So many SMs are assumed whatever
-// the device has, so that the order of the sums follows from sizes.
-int warps_of(int ctas, int warps_of_sm, int least, int most) {
-  const int warps = warps_of_sm / ceil_div(ctas, 148);
-  return warps < least ? most / 2 > least ? most / 2 : most : warps > most ? most : warps;  // too many for one round: then not too few warps
-}
 // Launches for so many eights of columns and strips of rows a CTA, or (p null) allows the kernel its shared memory.
 template <int T, int G, int E, int S, bool One>
 cudaError_t one_gemv(const GemvQ4Params* p, cudaStream_t stream) {

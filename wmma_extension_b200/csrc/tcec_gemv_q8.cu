@@ -1,0 +1,54 @@
+// Launches of gradients of few columns from activations in 8 bits (tcec_gemv_q8.cuh).
+#include "tcec_gemv_q8.cuh"
+
+#include "tcec_codes_launch.h"
+#include "tcec_launch.h"
+
+using namespace tcec_sm100;
+
+namespace tcec_host {
+namespace {
+
+// Launches, or (p null) allows the kernel its shared memory.
+template <int T, int E, int S>
+cudaError_t one_gemv(const GemvQ8Params* p, cudaStream_t stream) {
+  using Cfg = GemvQ8Cfg<E, S>;
+  if (!p) return cudaFuncSetAttribute(gemv_q8_kernel<T, E, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem_bytes(Cfg::MOST_WARPS));
+  const int ctas = (p->rows + Cfg::ROWS - 1) / Cfg::ROWS, warps = warps_of(ctas, Cfg::WARPS_OF_SM, 4, Cfg::MOST_WARPS);
+  launch_early(gemv_q8_kernel<T, E, S>, ctas, 32 * warps, Cfg::smem_bytes(warps), stream, *p);
+  return cudaSuccess;
+}
+template <int T, int S>
+cudaError_t of_strips(int eights, const GemvQ8Params* p, cudaStream_t stream) {
+  return eights == 1 ? one_gemv<T, 1, S>(p, stream) : eights == 2 ? one_gemv<T, 2, S>(p, stream) : one_gemv<T, 4, S>(p, stream);
+}
+template <int T>
+void of_type(int eights, const GemvQ8Params& p, cudaStream_t stream) {
+  if (p.rows <= 148 * 16) of_strips<T, 1>(eights, &p, stream);
+  else of_strips<T, 2>(eights, &p, stream);
+}
+template <int T>
+cudaError_t set_type() {
+  cudaError_t e = cudaSuccess;
+  for (int eights = 1; eights <= 4 && e == cudaSuccess; eights *= 2) {
+    e = of_strips<T, 1>(eights, nullptr, nullptr);
+    if (e == cudaSuccess) e = of_strips<T, 2>(eights, nullptr, nullptr);
+  }
+  return e;
+}
+
+}  // namespace
+
+cudaError_t set_gemv_q8_attrs() {
+  cudaError_t e = set_type<kTypeF32>();
+  if (e == cudaSuccess) e = set_type<kTypeF16>();
+  if (e == cudaSuccess) e = set_type<kTypeBf16>();
+  return e;
+}
+void launch_gemv_q8(int type, int eights, const GemvQ8Params& p, cudaStream_t stream) {
+  if (type == kTypeF32) of_type<kTypeF32>(eights, p, stream);
+  else if (type == kTypeF16) of_type<kTypeF16>(eights, p, stream);
+  else of_type<kTypeBf16>(eights, p, stream);
+}
+
+}  // namespace tcec_host
