@@ -47,7 +47,7 @@ template <int kType, int kGroup, int kEights, int kStrips, bool kOne>
 struct GemvQ4Cfg {
   static constexpr int PARTS = kType == kTypeF32 ? 3 : 1;
   static constexpr int ROWS = 16 * kStrips;
-  static constexpr int MOST_WARPS = (kOne && kStrips < 4) || kEights == 2 ? 16 : 8;
+  static constexpr int MOST_WARPS = kStrips == 4 || kEights == 4 ? 8 : 16;
   static constexpr int STAGE_BYTES = kStrips * q4_strip_bytes(kGroup);
   static constexpr int STAGES = 2;                            // blocks of codes under way, of each warp
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
@@ -58,7 +58,7 @@ struct GemvQ4Cfg {
   static constexpr int WARP_BYTES = RING_BYTES + X_BYTES > SUM_BYTES ? RING_BYTES + X_BYTES : SUM_BYTES;
   static constexpr int smem_bytes(int warps) { return warps * WARP_BYTES + 128; }
   // Warps that an SM's registers hold: 64 registers a thread for one token, else what the operands of the columns need.
-  static constexpr int WARPS_OF_SM = kEights == 1 ? (kStrips == 4 ? 16 : kOne ? 32 : 20) : kEights == 2 ? 16 : 8;
+  static constexpr int WARPS_OF_SM = kOne && kStrips < 4 ? 32 : kEights == 4 ? 8 : 16;
 };
 
 template <bool kF16>
@@ -111,7 +111,7 @@ __device__ __forceinline__ void multiply_strip(float (&acc)[kEights][4], const u
 }
 
 template <int kType, int kGroup, int kEights, int kStrips, bool kOne>
-__global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips, kOne>::MOST_WARPS, kEights == 1 ? 2 : 1) gemv_q4_kernel(const GemvQ4Params p) {
+__global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips, kOne>::MOST_WARPS, kOne || kStrips == 4 ? 2 : 1) gemv_q4_kernel(const GemvQ4Params p) {
   using Cfg = GemvQ4Cfg<kType, kGroup, kEights, kStrips, kOne>;
   static_assert(!kOne || kEights == 1, "one token has at most three columns");
   constexpr int kSpans = kCodeSpan / kGroup;
