@@ -310,7 +310,8 @@ int tcec_unpack_q8(int layout_x, int m, int k, const void* packed, void* x, long
 /*
  * C (n x k) = alpha * dY^T (n x m) * X (m x k) + beta * C for activations kept as above: the gradient of a layer's weights from the
  * gradient dY (m x n) of its outputs; beta = 1 adds up over several batches.  type_c is type_dy or FP32.
- * `workspace` takes tcec_wgrad_q8_workspace_bytes(m, n, k, type_dy) bytes.
+ * `workspace` takes tcec_wgrad_q8_workspace_bytes(m, n, k, type_dy) bytes.  The sum over a group of codes times dY has to fit FP32; up to 32 columns
+ * of dY (FP32: 10) values of 2^122 and more count as infinite.
  */
 size_t tcec_wgrad_q8_workspace_bytes(int m, int n, int k, int type_dy);
 int tcec_wgrad_q8(int layout_dy, int layout_c, int m, int n, int k, float alpha, const void* dy, long long lddy, int type_dy,

@@ -18,7 +18,7 @@
 // the converters, 1130 cycles at 128 bytes each; its MMAs take 520.  Tiles of 256 x 256 on two SMs do twice as many products with the same (1024
 // cycles of MMAs).  Measured: 512 tokens times 4096 x 4096, 128 tiles of 32 blocks, 25.5 us (670 TFLOP/s), 1000 tokens on pairs 38.8 (860), 8192 x 4096 x 4096
 // gradient 262 alone (1050).  Groups of 32 have four accumulators a block to fold, FP32 three times as many: 512 tokens 44 us, FP32 103, in groups of 128 56.
-// Few columns: by the codes' way from memory to operands; 8192 x 4096 gradient of rank 16 18.6 us (1.9 TB/s), 64 tokens times 4096 x 4096 12.9.
+// Few columns: by the codes' way from memory to operands; 8192 x 4096 gradient of rank 48 18.7 us (1.8 TB/s), 64 tokens times 4096 x 4096 12.9.
 #pragma once
 #include "tcec_codes.cuh"
 #include "tcec_codes_launch.h"

@@ -27,7 +27,7 @@ cudaError_t gemv_of(int eights, const GemvQ4Params& p, cudaStream_t stream) {
   // 8192 x 8192 14.3, 11.7, 10.6; 16384 x 16384 51, 37, 31; 12288 x 1024 4.8, 4.1, 4.2).
   if (!p.staged && p.n <= 148 * 16) return one_gemv<T, G, 1, 1, true>(&p, stream);
   if (!p.staged) return p.n <= 148 * 32 || p.blocks < 16 ? one_gemv<T, G, 1, 2, true>(&p, stream) : one_gemv<T, G, 1, 4, true>(&p, stream);
-  // Five tokens: 2048 x 4096 5.3, 5.1, 6.4 us; 8192 x 8192 13.8, 11.0, 15.4; 12288 x 1024 5.9, 6.2, 5.1; 16384 x 16384 36, 37, 29.
+  // Five tokens, likewise: 2048 x 4096 5.3, 5.1, 6.4 us; 8192 x 8192 13.8, 11.0, 15.4; 12288 x 1024 5.9, 6.2, 5.1; 16384 x 16384 36, 37, 29.
   if (eights == 1) return p.n <= 148 * 64 ? one_gemv<T, G, 1, 2, false>(&p, stream) : one_gemv<T, G, 1, 4, false>(&p, stream);
   // A CTA of two strips does for its columns once what two of one strip do twice, but its SMs may stay idle at the end.  The work of a strip grows
   // with its groups, and a strip of two groups costs about what the columns do (12 tokens, groups of 128: 2048 rows of 4096 5.4 us with one strip,

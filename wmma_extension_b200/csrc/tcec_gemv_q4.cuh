@@ -17,7 +17,7 @@
 // operands of the columns stay in registers: 16384 x 16384 with 16 tokens 45.6 us, strips side by side 53.8, with one FP32 token (groups of 64) 35 and 42.
 //
 // Measured, from memory: one bf16 token times 4096 x 4096 4.9 us (1.8 TB/s: 32 rows of blocks an SM are over before the copies are up to speed), times
-// 16384 x 16384 30.5 (4.6 TB/s), FP32 in groups of 64 35.5 (4.2 TB/s); 8 tokens 29 us, 16 45.6, 32 (10 of FP32) 94.
+// 16384 x 16384 30.5 (4.6 TB/s), FP32 in groups of 64 35.5 (4.2 TB/s); 8 tokens 29 us, 16 46, 10 of FP32 94.
 #pragma once
 #include "tcec_gemm_codes.cuh"
 
@@ -57,7 +57,8 @@ struct GemvQ4Cfg {
   static constexpr int SUM_BYTES = ROWS * SUM_PITCH * 4;      // of a warp
   static constexpr int WARP_BYTES = RING_BYTES + X_BYTES > SUM_BYTES ? RING_BYTES + X_BYTES : SUM_BYTES;
   static constexpr int smem_bytes(int warps) { return warps * WARP_BYTES + 128; }
-  // Warps that an SM's registers hold: 64 registers a thread for one token, else what the operands of the columns need.
+  // Warps that an SM's registers hold: 64 registers a thread for one token, else what the operands of the columns need.  All of an SM in one CTA where CTAs
+  // are no more than SMs (five tokens times 4096 x 16384 11.2 us, with at most eight warps a CTA 17.1).
   static constexpr int WARPS_OF_SM = kOne && kStrips < 4 ? 32 : kEights == 4 ? 8 : 16;
 };
 

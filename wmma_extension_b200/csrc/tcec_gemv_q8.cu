@@ -24,6 +24,8 @@ cudaError_t of_strips(int eights, const GemvQ8Params* p, cudaStream_t stream) {
 }
 template <int T>
 void of_type(int eights, const GemvQ8Params& p, cudaStream_t stream) {
+  // One strip a CTA while such CTAs fit the SMs, else two, which share what is done for the columns (rank 16, 8192 tokens: 2368 features 8.7 us with one,
+  // 10.5 with two; 3000 12.6 and 11.2; 8192 26.9 and 19.6).
   if (p.rows <= 148 * 16) of_strips<T, 1>(eights, &p, stream);
   else of_strips<T, 2>(eights, &p, stream);
 }
