@@ -33,7 +33,10 @@ def test_workspaces():
     assert lib.tcec_gemm_q4_workspace_bytes(1000, 4096, 4096, BF16) == 8 * 32 * 32768
     assert lib.tcec_gemm_q4_workspace_bytes(1000, 4096, 4096, F32) == 3 * 8 * 32 * 32768
     assert lib.tcec_gemm_q4_workspace_bytes(1000, 4096, 4096, 3) == 0
-    assert lib.tcec_wgrad_q8_workspace_bytes(300, 16, 4096, F16) == 3 * 32768
+    assert lib.tcec_wgrad_q8_workspace_bytes(300, 40, 4096, F16) == 3 * 32768
+    # few: 2 KB for every eight columns of a block, their units and the sums of up to four groups
+    assert lib.tcec_wgrad_q8_workspace_bytes(300, 16, 4096, F16) == 3 * 2 * (2048 + 5 * 32)
+    assert lib.tcec_gemm_q4_workspace_bytes(3, 4096, 4096, F32) == 32 * 2 * (2048 + 5 * 32)
     assert lib.tcec_wgrad_q8_workspace_bytes(300, 129, 4096, F32) == 3 * 2 * 3 * 32768
 
 
