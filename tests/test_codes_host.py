@@ -81,7 +81,7 @@ def test_gemm_q4_refuses(change):
 
 @pytest.mark.parametrize("change", [
     dict(ly=2), dict(lc=9), dict(m=-1), dict(n=-1), dict(k=-1), dict(ty=-1), dict(tc=3), dict(ty=BF16, tc=F16), dict(ldy=7),
-    dict(ly=1, ldy=15), dict(ldc=3), dict(y=None), dict(c=None), dict(x=None), dict(ws=None), dict(wsb=3 * 32768 - 1), "y unaligned",
+    dict(ly=1, ldy=15), dict(ldc=3), dict(y=None), dict(c=None), dict(x=None), dict(ws=None), dict(wsb=4 * (2048 + 5 * 32) - 1), "y unaligned",
     "x unaligned", "c over y", "c over x", "ws over y",
 ])
 def test_wgrad_q8_refuses(change):
