@@ -26,6 +26,7 @@ struct GemvQ4Params {
   const void* x;              // one token: element i at i * x_k
   long long x_k;
   int n, k, tokens, blocks;
+  int strips, more;           // strips of 16 rows of a CTA, and how many CTAs, the first ones, have one more (set by the launch)
   int vec;                    // x_k 1 and x aligned for four values at a time
   float alpha, beta;
   void* c;                    // element (token, row) at token * c_token + row * c_row

@@ -16,8 +16,16 @@ cudaError_t one_gemv(const GemvQ4Params* p, cudaStream_t stream) {
   using Cfg = GemvQ4Cfg<T, G, E, S, One>;
   constexpr int kMost = Cfg::MOST_WARPS;
   if (!p) return cudaFuncSetAttribute(gemv_q4_kernel<T, G, E, S, One>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem_bytes(kMost));
-  const int ctas = ceil_div(p->n, Cfg::ROWS), warps = warps_of(ctas, Cfg::WARPS_OF_SM, 4, kMost);
-  launch_early(gemv_q4_kernel<T, G, E, S, One>, ctas, 32 * warps, Cfg::smem_bytes(warps), stream, *p);
+  // CTAs that are more than the SMs are made as many for each of these, with a strip more or less: 16384 rows are 256 times four strips, eight for some
+  // SMs and four for others, or 136 times four and 160 times three, seven for an SM (one FP32 token, groups of 64: 33.9 us, 36.7 so; 10000 x 10000 20.4
+  // and 23.6; 5 bf16 tokens times 5000 x 7001 8.0 and 9.4).
+  GemvQ4Params q = *p;
+  const int strips = ceil_div(p->n, 16), least = ceil_div(strips, S), per_sm = Cfg::SHARED_OUT ? ceil_div(least, 148) : 1;
+  const int ctas = per_sm == 1 ? least : 148 * per_sm < strips ? 148 * per_sm : strips;
+  q.strips = per_sm == 1 ? S : strips / ctas;
+  q.more = per_sm == 1 ? 0 : strips % ctas;
+  const int warps = warps_of(ctas, Cfg::WARPS_OF_SM, 4, kMost);
+  launch_early(gemv_q4_kernel<T, G, E, S, One>, ctas, 32 * warps, Cfg::smem_bytes(warps), stream, q);
   return cudaSuccess;
 }
 template <int T, int G>

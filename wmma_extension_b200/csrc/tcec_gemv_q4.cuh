@@ -13,11 +13,11 @@
 // exact; a group's sum is made in the MMA's FP32 accumulator, then multiplied by its scale and added in FP32, rounded to nearest.  As code and zero
 // point are multiplied apart, what is rounded off is relative to scale * (code + zero) * |x|.
 //
-// A CTA takes 16 kStrips rows; its warps divide k block by block and add up through shared memory in a fixed order.  One strip after the other, the
+// A CTA takes up to kStrips strips of 16 rows; its warps divide k block by block and add up through shared memory in a fixed order.  One strip after the other, the
 // operands of the columns stay in registers: 16384 x 16384 with 16 tokens 45.6 us, strips side by side 53.8, with one FP32 token (groups of 64) 35 and 42.
 //
 // Measured, from memory: one bf16 token times 4096 x 4096 4.9 us (1.8 TB/s: 32 rows of blocks an SM are over before the copies are up to speed), times
-// 16384 x 16384 30.5 (4.6 TB/s), FP32 in groups of 64 35.5 (4.2 TB/s); 8 tokens 29 us, 16 46, 10 of FP32 94.
+// 16384 x 16384 29.3 (4.9 TB/s), FP32 in groups of 64 33.8 (4.5 TB/s); 8 tokens 28 us, 16 46, 10 of FP32 94.
 #pragma once
 #include "tcec_gemm_codes.cuh"
 
@@ -49,6 +49,9 @@ struct GemvQ4Cfg {
   static constexpr int ROWS = 16 * kStrips;
   static constexpr int MOST_WARPS = kStrips == 4 || kEights == 4 ? 8 : 16;
   static constexpr int STAGE_BYTES = kStrips * q4_strip_bytes(kGroup);
+  // Whether CTAs may have a strip less (one_gemv).  Where nothing comes of it the test costs 3 % (two strips of one token, 4096 x 4096), and in groups of 32 with
+  // 9 to 16 columns 8 % (8192 x 8192).
+  static constexpr bool SHARED_OUT = kOne ? kStrips == 4 : kEights == 1 || (kEights == 2 && kGroup > 32);
   static constexpr int STAGES = 2;                            // blocks of codes under way, of each warp
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int X_PITCH = 320;                         // of a column in shared memory: two columns' lanes read from all banks
@@ -133,14 +136,21 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
   if constexpr (kOne)  // columns that no part of the token has
     for (int i = lane; i < Cfg::X_BYTES / 16; i += 32) reinterpret_cast<uint4*>(x_shared)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
-  const int row0 = blockIdx.x * Cfg::ROWS;
+  const int cta = blockIdx.x, strip0 = Cfg::SHARED_OUT ? cta * p.strips + min(cta, p.more) : cta * kStrips, row0 = strip0 * 16;
+  const int strips = Cfg::SHARED_OUT ? min(p.strips + (cta < p.more), (p.n - row0 + 15) / 16) : kStrips;
   constexpr size_t kBlockBytes = q4_block_bytes(kGroup);
-  const uint8_t* codes = p.codes + static_cast<size_t>(row0 / kCodeRows) * p.blocks * kBlockBytes + row0 % kCodeRows / 16 * q4_strip_bytes(kGroup);
+  // strips of one tile of rows, or the last ones of one and the first ones of the next
+  const uint32_t bytes = Cfg::SHARED_OUT ? min(strips, 8 - strip0 % 8) * q4_strip_bytes(kGroup) : Cfg::STAGE_BYTES;
+  const uint32_t bytes_next = strips * q4_strip_bytes(kGroup) - bytes;
+  const uint8_t* codes_next = p.codes + static_cast<size_t>(strip0 / 8 + 1) * p.blocks * kBlockBytes;
+  const uint8_t* codes = p.codes + static_cast<size_t>(strip0 / 8) * p.blocks * kBlockBytes + strip0 % 8 * q4_strip_bytes(kGroup);
   auto fetch = [&](int kb, int stage) {  // lane 0
     if (dev_flag(p.debug_flags, 128) && blockIdx.x == 0 && kb == 0) return;
     const uint32_t bar = smem_u32(&bars[warp][stage]);
-    mbar_arrive_expect_tx(bar, Cfg::STAGE_BYTES);
-    bulk_load(smem_u32(ring + stage * Cfg::STAGE_BYTES), codes + kb * kBlockBytes, Cfg::STAGE_BYTES, bar);
+    const uint32_t to = smem_u32(ring + stage * Cfg::STAGE_BYTES);
+    mbar_arrive_expect_tx(bar, bytes + bytes_next);
+    bulk_load(to, codes + kb * kBlockBytes, bytes, bar);
+    if (Cfg::SHARED_OUT && bytes_next) bulk_load(to + bytes, codes_next + kb * kBlockBytes, bytes_next, bar);
   };
   // Staged x is written by the kernel before this one, which was through its own wait when this one could start: whatever the codes
   // come from has ended, and they are fetched without waiting for x.
@@ -267,14 +277,16 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
       for (int q = 0; q < kSpans; ++q) sums[q][0] = make_float2(ones[q][0] * (unit * 0x1p-7f), ones[q][1] * (unit * 0x1p-7f));
       const float2 units[1] = {make_float2(unit, unit)};
 #pragma unroll
-      for (int s = 0; s < kStrips; ++s) multiply_strip<kType, kGroup, 1>(acc[s], here + s * q4_strip_bytes(kGroup), lane, b, sums, units);
+      for (int s = 0; s < kStrips; ++s)
+        if (!Cfg::SHARED_OUT || s < kStrips - 1 || strips == kStrips) multiply_strip<kType, kGroup, 1>(acc[s], here + s * q4_strip_bytes(kGroup), lane, b, sums, units);
     } else if constexpr (kEights > 1) {
 #pragma unroll
       for (int c = 0; c < kEights; ++c)
         if constexpr (kF16) units_ahead[c] = make_float2(kUnitF16, kUnitF16);
 #pragma unroll
       for (int s = 0; s < kStrips; ++s)
-        multiply_strip<kType, kGroup, kEights>(acc[s], here + s * q4_strip_bytes(kGroup), lane, b_ahead, sums_ahead, units_ahead);
+        if (!Cfg::SHARED_OUT || s < kStrips - 1 || strips == kStrips)
+          multiply_strip<kType, kGroup, kEights>(acc[s], here + s * q4_strip_bytes(kGroup), lane, b_ahead, sums_ahead, units_ahead);
     } else {
       uint4 b[4][kEights];
       float2 sums[kSpans][kEights], units[kEights];
@@ -292,7 +304,8 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
         for (int panel = 0; panel < 4; ++panel) load_operands(next, panel);
       }
 #pragma unroll
-      for (int s = 0; s < kStrips; ++s) multiply_strip<kType, kGroup, kEights>(acc[s], here + s * q4_strip_bytes(kGroup), lane, b, sums, units);
+      for (int s = 0; s < kStrips; ++s)
+        if (!Cfg::SHARED_OUT || s < kStrips - 1 || strips == kStrips) multiply_strip<kType, kGroup, kEights>(acc[s], here + s * q4_strip_bytes(kGroup), lane, b, sums, units);
     }
     __syncwarp();  // all have read the stage
     if (lane == 0 && kb + Cfg::STAGES * warps < p.blocks) fetch(kb + Cfg::STAGES * warps, stage);
@@ -323,7 +336,7 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
   __syncthreads();
   for (int i = threadIdx.x; i < Cfg::ROWS * p.tokens; i += blockDim.x) {
     const int r = i % Cfg::ROWS, token = i / Cfg::ROWS, row = row0 + r;
-    if (row >= p.n) continue;
+    if (row >= p.n || r >= strips * 16) continue;
     float v = 0.f;
 #pragma unroll
     for (int part = Cfg::PARTS - 1; part >= 0; --part)  // the small ones first
