@@ -651,3 +651,48 @@ def test_gradients_of_any_magnitude(dtype):
     clean = tcec.wgrad_q8(dy, packed, k, dtype=F32)
     keep = [0, 1, 3, 5]
     assert got[2].isnan().all() and not got[4].isfinite().any() and torch.equal(got[keep], clean[keep])
+
+
+def test_offsets_beyond_32_bits():
+    """Packed weights of 4.6 GB (one tile of rows, repeated), and dense matrices whose lines lie 2^31 elements apart."""
+    k, tiles = 65536, 1024
+    tile = tcec.pack_q4(randn(128, k, seed=1, dtype=BF16))
+    w = tcec.unpack_q4(tile, 128, k).double()
+    packed = tile.repeat(tiles)
+    for m in (1, 4, 12, 40):
+        x = randn(m, k, seed=m, dtype=BF16)
+        exact = x.double() @ w.T
+        tol = bound(x.double().abs() @ w.abs().T, exact, F32, k, 1)
+        got = tcec.gemm_q4(x, packed, 128 * tiles, dtype=F32).reshape(m, tiles, 128)
+        for t in (0, 480, 1023):
+            check(got[:, t], exact, tol)
+        assert torch.equal(got[:, 5], got[:, 1000])
+    del packed, got
+    features = tcec.pack_q8(randn(40000, 128, seed=2))
+    kept = features.repeat(512)
+    w = tcec.unpack_q8(features, 40000, 128).double()
+    dy = randn(40000, 40, seed=3, dtype=BF16)
+    for n in (4, 16, 40):
+        exact = dy[:, :n].double().T @ w
+        got = tcec.wgrad_q8(dy[:, :n].contiguous(), kept, 128 * 512, dtype=F32).reshape(n, 512, 128)
+        check(got[:, 511], exact, bound(dy[:, :n].double().abs().T @ w.abs(), exact, F32, 40000, 1))
+        assert torch.equal(got[:, 3], got[:, 500])
+    del kept, got
+    ld = 2**31 + 8
+    store = torch.empty(2 * ld + 256, device=DEV, dtype=BF16)
+    far = store.as_strided((3, 256), (ld, 1))
+    near = randn(3, 256, seed=4, dtype=BF16)
+    far.copy_(near)
+    w = tcec.pack_q4(randn(256, 256, seed=5))
+    assert torch.equal(tcec.gemm_q4(far, w, 256), tcec.gemm_q4(near, w, 256))
+    assert torch.equal(tcec.gemm_q4(far[2:], w, 256), tcec.gemm_q4(near[2:], w, 256))
+    assert torch.equal(tcec.pack_q4(far), tcec.pack_q4(near)) and torch.equal(tcec.pack_q8(far), tcec.pack_q8(near))
+    q4, q8 = tcec.pack_q4(near), tcec.pack_q8(near)
+    assert torch.equal(tcec.unpack_q4(q4, 3, 256, out=far), tcec.unpack_q4(q4, 3, 256, dtype=BF16))
+    assert torch.equal(tcec.unpack_q8(q8, 3, 256, out=far), tcec.unpack_q8(q8, 3, 256, dtype=BF16))
+    assert torch.equal(tcec.gemm_q4(near, w, 256, far), tcec.gemm_q4(near, w, 256))
+    for n in (16, 256):
+        far.copy_(near)
+        kept = tcec.pack_q8(randn(3, 70, seed=6))
+        assert torch.equal(tcec.wgrad_q8(far[:, :n], kept, 70), tcec.wgrad_q8(near[:, :n], kept, 70))
+    tcec.device_status()
