@@ -263,14 +263,14 @@ __global__ void __launch_bounds__(512) stage_columns_kernel(const StageColumnsPa
       for (int j = 0; j < 8; ++j) sum += v[j];
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum += __uint_as_float(part[q][j] << 16) + __uint_as_float(part[q][j] & 0xffff0000u);
+      for (int j = 0; j < 4; ++j)  // the values themselves, as the sum of scaled ones may be 2^28 * 2^100; exact, as their parts are FP32 numbers
+        sum += by.down * __uint_as_float(part[q][j] << 16) + by.down * __uint_as_float(part[q][j] & 0xffff0000u);
     }
     for (int d = 1; d < p.group / 8; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     const int of_group = p.group / 8;  // threads
     if (col < columns) {
       if ((chunk & (of_group - 1)) == 0)
-        *reinterpret_cast<float*>(sums + ((1 + chunk / of_group) * columns + col) * 4) =
-            sum * by.down;
+        *reinterpret_cast<float*>(sums + ((1 + chunk / of_group) * columns + col) * 4) = sum;
       if (chunk == 0) *reinterpret_cast<float*>(sums + col * 4) = by.unit;
     }
   }
