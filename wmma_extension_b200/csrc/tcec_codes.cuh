@@ -232,6 +232,7 @@ __global__ void __launch_bounds__(512 / kHalves) pack_q4_kernel(const PackQ4Para
   constexpr int kSpans = kCodeSpan / kGroup;
   __shared__ __align__(16) uint32_t words[2048 + 128 * kSpans];
   wait_for_launch_before();
+  const void* const w = after_wait(p.w);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int kb = blockIdx.x % p.blocks, tile = blockIdx.x / p.blocks;
 #pragma unroll
@@ -242,14 +243,14 @@ __global__ void __launch_bounds__(512 / kHalves) pack_q4_kernel(const PackQ4Para
     if (p.vec && left >= 7 * 16 + 4) {
       Four<kType> f[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j].load(p.w, row * p.row_step + k0 + j * 16);
+      for (int j = 0; j < 8; ++j) f[j].load(w, row * p.row_step + k0 + j * 16);
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j].get(v[j]);
     } else if (left > 0) {  // unaligned, column-major or at the edge: addresses stay inside the row
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[j][i] = ld_element<kType>(p.w, row * p.row_step + (k0 + min(j * 16 + i, left - 1)) * p.k_step);
+        for (int i = 0; i < 4; ++i) v[j][i] = ld_element<kType>(w, row * p.row_step + (k0 + min(j * 16 + i, left - 1)) * p.k_step);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -313,6 +314,8 @@ template <int kGroup>
 __global__ void __launch_bounds__(256) pack_q4_codes_kernel(const PackQ4Params p) {
   __shared__ __align__(16) uint32_t words[2048 + 128 * (kCodeSpan / kGroup)];
   wait_for_launch_before();
+  const uint8_t *const codes = after_wait(p.codes), *const zeros = after_wait(p.zeros);
+  const void* const scales = after_wait(p.scales);
   const int kb = blockIdx.x % p.blocks, tile = blockIdx.x / p.blocks;
   constexpr int kSpans = kCodeSpan / kGroup;
   for (int i = threadIdx.x; i < 128 * kSpans; i += 256) {
@@ -320,8 +323,8 @@ __global__ void __launch_bounds__(256) pack_q4_codes_kernel(const PackQ4Params p
     uint32_t entry = 0;
     if (row < p.n && g < p.groups) {
       const long long at = static_cast<long long>(row) * p.groups + g;
-      const float s = p.scale_bf16 ? ld_element<kTypeBf16>(p.scales, at) : ld_element<kTypeF16>(p.scales, at);
-      entry = q4_entry(not_finite(s) ? nan32() : s, p.zeros ? (p.zeros[at] & 15) : 8);
+      const float s = p.scale_bf16 ? ld_element<kTypeBf16>(scales, at) : ld_element<kTypeF16>(scales, at);
+      entry = q4_entry(not_finite(s) ? nan32() : s, zeros ? (zeros[at] & 15) : 8);
     }
     words[q4_entry_word<kGroup>(r, i >> 7)] = entry;
   }
@@ -334,7 +337,7 @@ __global__ void __launch_bounds__(256) pack_q4_codes_kernel(const PackQ4Params p
     for (int j = 0; j < 4; ++j) {
       uint32_t lo = z, hi = z;
       if (row < p.n && k0 + 2 * j < p.k) {
-        const uint32_t b = p.codes[row * p.codes_ld + (k0 >> 1) + j];
+        const uint32_t b = codes[row * p.codes_ld + (k0 >> 1) + j];
         lo = b & 15u;
         if (k0 + 2 * j + 1 < p.k) hi = b >> 4;
       }
@@ -363,7 +366,7 @@ __global__ void __launch_bounds__(256) unpack_q4_kernel(const UnpackParams p) {
   __shared__ __align__(16) uint32_t words[2048 + 128 * (kCodeSpan / kGroup)];
   wait_for_launch_before();
   const int kb = blockIdx.x % p.blocks, tile = blockIdx.x / p.blocks;
-  const uint8_t* in = p.packed + (static_cast<size_t>(tile) * p.blocks + kb) * q4_block_bytes(kGroup);
+  const uint8_t* in = after_wait(p.packed) + (static_cast<size_t>(tile) * p.blocks + kb) * q4_block_bytes(kGroup);
   for (int i = threadIdx.x; i < q4_block_bytes(kGroup) / 16; i += 256) reinterpret_cast<uint4*>(words)[i] = ld_operand128(in + i * 16);
   let_next_launch_start();
   __syncthreads();
@@ -413,7 +416,7 @@ __global__ void __launch_bounds__(256, 3) pack_q8_kernel(const PackQ8Params p) {
   const int tiles = (p.features + kCodeRows - 1) / kCodeRows, tile = blockIdx.x % tiles, tb = blockIdx.x / tiles;  // whole rows at a time
   const int f0 = tile * kCodeRows + lane * 4, t0 = tb * kCodeSpan + warp * 16;
   float v[16][4];
-  ld_lines4<kType, 16>(p.x, t0 * p.token_step + f0 * p.feature_step, p.token_step, p.feature_step, p.tokens - t0, p.features - f0, p.vec, v);
+  ld_lines4<kType, 16>(after_wait(p.x), t0 * p.token_step + f0 * p.feature_step, p.token_step, p.feature_step, p.tokens - t0, p.features - f0, p.vec, v);
   let_next_launch_start();
   float m[4];  // the largest magnitude, or NaN if a value is not finite
 #pragma unroll
@@ -468,7 +471,7 @@ __global__ void __launch_bounds__(256) unpack_q8_kernel(const UnpackParams p) {
   wait_for_launch_before();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = (p.rows + kCodeRows - 1) / kCodeRows, tile = blockIdx.x % tiles, tb = blockIdx.x / tiles;
-  const uint8_t* block = p.packed + (static_cast<size_t>(tile) * p.blocks + tb) * kQ8BlockBytes;
+  const uint8_t* block = after_wait(p.packed) + (static_cast<size_t>(tile) * p.blocks + tb) * kQ8BlockBytes;
   const int f0 = tile * kCodeRows + lane * 4, t0 = tb * kCodeSpan + warp * 16;
   const uint4 sc = ld_operand128(block + kQ8CodeBytes + lane * 16);
   const float s[4] = {__uint_as_float(sc.x), __uint_as_float(sc.y), __uint_as_float(sc.z), __uint_as_float(sc.w)};

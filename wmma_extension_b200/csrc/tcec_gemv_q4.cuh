@@ -170,17 +170,18 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
   // x of the next block, on its way while this one is worked on: the token's four values of this lane, or whole operands
   [[maybe_unused]] Four<kType> four;
   [[maybe_unused]] uint4 b_ahead[4][kEights];
+  [[maybe_unused]] const void* const token_x = kOne ? after_wait(p.x) : nullptr;
   auto load_four = [&](int kb) {
     const int k0 = kb * kCodeSpan + lane * 4, left = p.k - k0;
     if (p.vec && left >= 4) {
-      four.load(p.x, k0);
+      four.load(token_x, k0);
     } else {
       uint32_t v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const long long at = min(k0 + j, p.k - 1) * p.x_k;
-        if constexpr (kType == kTypeF32) v[j] = ld_operand32(static_cast<const uint32_t*>(p.x) + at);
-        else v[j] = ld_operand16(static_cast<const uint16_t*>(p.x) + at);
+        if constexpr (kType == kTypeF32) v[j] = ld_operand32(static_cast<const uint32_t*>(token_x) + at);
+        else v[j] = ld_operand16(static_cast<const uint16_t*>(token_x) + at);
         if (j >= left) v[j] = 0;
       }
       if constexpr (kType == kTypeF32) four.raw = make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
@@ -334,6 +335,7 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
       for (int j = 0; j < 4; ++j)
         sums[(warp * Cfg::ROWS + s * 16 + (lane >> 2) + (j >> 1) * 8) * Cfg::SUM_PITCH + c * 8 + (lane & 3) * 2 + (j & 1)] = acc[s][c][j];
   __syncthreads();
+  void* const c = after_wait(p.c);
   for (int i = threadIdx.x; i < Cfg::ROWS * p.tokens; i += blockDim.x) {
     const int r = i % Cfg::ROWS, token = i / Cfg::ROWS, row = row0 + r;
     if (row >= p.n || r >= strips * 16) continue;
@@ -344,8 +346,8 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
       for (int w = 0; w < warps; ++w) v += sums[(w * Cfg::ROWS + r) * Cfg::SUM_PITCH + token * Cfg::PARTS + part];
     const long long at = token * p.c_token + row * p.c_row;
     v = __fmul_rn(p.alpha, v);
-    if (p.beta != 0.f) v = __fmaf_rn(p.beta, ld_element_as(p.c_type, p.c, at), v);
-    st_element_as(p.c_type, p.c, at, v);
+    if (p.beta != 0.f) v = __fmaf_rn(p.beta, ld_element_as(p.c_type, c, at), v);
+    st_element_as(p.c_type, c, at, v);
   }
 }
 

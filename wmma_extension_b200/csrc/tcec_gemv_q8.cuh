@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(32 * GemvQ8Cfg<kEights, kStrips>::MOST_WARPS, 
       for (int j = 0; j < 4; ++j)
         sums[(warp * Cfg::ROWS + s * 16 + (lane >> 2) + (j >> 1) * 8) * Cfg::SUM_PITCH + c * 8 + (lane & 3) * 2 + (j & 1)] = acc[s][c][j];
   __syncthreads();
+  void* const c = after_wait(p.c);
   for (int i = threadIdx.x; i < Cfg::ROWS * p.cols; i += blockDim.x) {
     const int r = i % Cfg::ROWS, col = i / Cfg::ROWS, row = row0 + r;
     if (row >= p.rows) continue;
@@ -162,8 +163,8 @@ __global__ void __launch_bounds__(32 * GemvQ8Cfg<kEights, kStrips>::MOST_WARPS, 
       for (int w = 0; w < warps; ++w) v += sums[(w * Cfg::ROWS + r) * Cfg::SUM_PITCH + col * kParts + part];
     const long long to = row * p.c_row + col * p.c_col;
     v = __fmul_rn(p.alpha, v);
-    if (p.beta != 0.f) v = __fmaf_rn(p.beta, ld_element_as(p.c_type, p.c, to), v);
-    st_element_as(p.c_type, p.c, to, v);
+    if (p.beta != 0.f) v = __fmaf_rn(p.beta, ld_element_as(p.c_type, c, to), v);
+    st_element_as(p.c_type, c, to, v);
   }
 }
 

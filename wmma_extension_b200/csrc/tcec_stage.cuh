@@ -49,6 +49,7 @@ template <int kType>
 __global__ void __launch_bounds__(256) stage_panels_kernel(const StagePanelsParams p) {
   constexpr int kParts = kType == kTypeF32 ? 3 : 1;
   wait_for_launch_before();
+  const void* const operand = after_wait(p.src);
   let_next_launch_start();  // the product: its CTAs take whole SMs, and fetch and expand codes
   const int kb = blockIdx.x % p.blocks, cb = blockIdx.x / p.blocks;
   uint8_t* out = p.panels + static_cast<size_t>(blockIdx.x) * kParts * kSpanBytes;
@@ -77,7 +78,7 @@ __global__ void __launch_bounds__(256) stage_panels_kernel(const StagePanelsPara
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          w[h][j] = ld_operand32(static_cast<const uint16_t*>(p.src) + origin + col + min((blockIdx.y * 2 + h) * 32 + c * 8 + j, sum_here - 1) * p.sum_step);
+          w[h][j] = ld_operand32(static_cast<const uint16_t*>(operand) + origin + col + min((blockIdx.y * 2 + h) * 32 + c * 8 + j, sum_here - 1) * p.sum_step);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int panel = blockIdx.y * 2 + h;
@@ -104,10 +105,10 @@ __global__ void __launch_bounds__(256) stage_panels_kernel(const StagePanelsPara
         const int it = it0 + i;
         const long long at = origin + min(column(it), cols_here - 1) * p.col_step + (it >> 1) * 32 + chunk(it) * 8;
         if constexpr (kType == kTypeF32) {
-          raw[i][0] = ld_operand128(static_cast<const float*>(p.src) + at);
-          raw[i][1] = ld_operand128(static_cast<const float*>(p.src) + at + 4);
+          raw[i][0] = ld_operand128(static_cast<const float*>(operand) + at);
+          raw[i][1] = ld_operand128(static_cast<const float*>(operand) + at + 4);
         } else {
-          raw[i][0] = ld_operand128(static_cast<const uint16_t*>(p.src) + at);
+          raw[i][0] = ld_operand128(static_cast<const uint16_t*>(operand) + at);
         }
       }
 #pragma unroll
@@ -129,8 +130,8 @@ __global__ void __launch_bounds__(256) stage_panels_kernel(const StagePanelsPara
         for (int j = 0; j < 8; ++j) {
           const int it = it0 + i, at_sum = (it >> 1) * 32 + chunk(it) * 8 + j;
           const long long at = origin + min(column(it), cols_here - 1) * p.col_step + min(at_sum, sum_here - 1) * p.sum_step;
-          if constexpr (kType == kTypeF32) w[i][j] = ld_operand(static_cast<const float*>(p.src) + at);
-          else w[i][j] = ld_operand16(static_cast<const uint16_t*>(p.src) + at);
+          if constexpr (kType == kTypeF32) w[i][j] = ld_operand(static_cast<const float*>(operand) + at);
+          else w[i][j] = ld_operand16(static_cast<const uint16_t*>(operand) + at);
         }
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
@@ -180,13 +181,14 @@ template <int kType>
 __global__ void __launch_bounds__(512) stage_columns_kernel(const StageColumnsParams p) {
   constexpr int kParts = kType == kTypeF32 ? 3 : 1;
   wait_for_launch_before();
+  const void* const operand = after_wait(p.src);
   let_next_launch_start();
   const int kb = blockIdx.x, chunk = threadIdx.x & 15, token = threadIdx.x >> 4, sum_here = p.sum - kb * kCodeSpan - chunk * 8;
   const long long at = token * p.col_step + (static_cast<long long>(kb) * kCodeSpan + chunk * 8) * p.sum_step;
   float v[8] = {};
   if (token < p.tokens && sum_here > 0) {
     if constexpr (kType == kTypeF32) {
-      const float* src = static_cast<const float*>(p.src) + at;
+      const float* src = static_cast<const float*>(operand) + at;
       if (p.vec && sum_here >= 8) {
         const float4 a = ld_operand(reinterpret_cast<const float4*>(src)), b = ld_operand(reinterpret_cast<const float4*>(src + 4));
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(512) stage_columns_kernel(const StageColumnsPa
           if (j >= sum_here) v[j] = 0.f;
       }
     } else {
-      const uint16_t* src = static_cast<const uint16_t*>(p.src) + at;
+      const uint16_t* src = static_cast<const uint16_t*>(operand) + at;
       uint32_t w[4];
       if (p.vec && sum_here >= 8) {
         const uint4 o = ld_operand128(src);
