@@ -36,3 +36,11 @@ def test_operands_are_read_through_pointers_that_are_known_after_the_wait(file, 
         for at in uses:
             assert body[:at].endswith("after_wait("), (field, body[at - 40:at + 40])
             assert at > wait, field
+
+
+def test_one_tokens_operands_are_handed_over_behind_a_warp_barrier():
+    """Lanes write their part of x to shared memory and read what others wrote; votes and the barrier of the codes' copies order neither."""
+    body = kernel("tcec_gemv_q4.cuh", "gemv_q4_kernel")
+    written = body.rindex("*reinterpret_cast<uint2*>(to")
+    read = body.index("*reinterpret_cast<const uint4*>(x_shared", written)
+    assert "__syncwarp();" in body[written:read]

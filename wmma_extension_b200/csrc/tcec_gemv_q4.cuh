@@ -253,13 +253,14 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
         *reinterpret_cast<uint2*>(to) = four.raw;
       }
       if (next < p.blocks) load_four(next);
+      __syncwarp();  // what all lanes have written, for all to read
     }
     if constexpr (kEights > 1) {  // more warps instead of operands ahead (16 tokens times 16384 x 16384: 46 us, 54 so)
       load_sums(kb);
 #pragma unroll
       for (int panel = 0; panel < 4; ++panel) load_operands(kb, panel);
     }
-    ok = mbar_wait_lanes(smem_u32(&bars[warp][stage]), parity, &abort_flag);  // brings the lanes together, too
+    ok = mbar_wait_lanes(smem_u32(&bars[warp][stage]), parity, &abort_flag);
     if (!ok) break;
     const uint8_t* const here = ring + stage * Cfg::STAGE_BYTES;
     if constexpr (kOne) {
