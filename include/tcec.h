@@ -258,8 +258,8 @@ int tcec_split(const float* in, float* hi, float* lo, size_t count, int policy, 
  * graph may have a workspace of its own.  A workspace may be used again as soon as the stream has passed the call.  Results must not overlap
  * operands or workspace (TCEC_ERR_INVALID_ARGUMENT; lines of one matrix between those of another are no overlap), and nothing outside a
  * result's rows and columns is written.  Sizes may be zero; a sum over nothing, or alpha == 0, gives beta * C; beta == 0 never reads C.  Of the
- * options "reserve_sms" holds for gradients and for more than few tokens, which are then not divided among SMs (the last bits may be others); the
- * others have no effect here.  A bounded wait that ran out is reported by tcec_device_status.
+ * options "reserve_sms" holds for the products of gradients and of more than few tokens: tiles are then not divided among SMs, and gradients of few
+ * columns come in several launches (the last bits may be others).  The others have no effect here.  A bounded wait that ran out is reported by tcec_device_status.
  */
 #define TCEC_TYPE_F32 0
 #define TCEC_TYPE_F16 1

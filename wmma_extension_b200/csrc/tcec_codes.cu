@@ -492,7 +492,7 @@ int tcec_wgrad_q8(int layout_dy, int layout_c, int m, int n, int k, float alpha,
       p.c_type = type_c;
       p.status = here.status;
       p.debug_flags = here.debug_flags;
-      launch_gemv_q8(type_dy, eights, p, on);
+      launch_gemv_q8(type_dy, eights, here.reserve_sms ? here.sm_count - here.reserve_sms : 0, p, on);
       return launched();
     }
     return gemm_codes(packed, 0, k, n, sum, dy, dd.col_step(), dd.row_step(), type_dy, layout_dy == TCEC_COL_MAJOR && dd.wide(16), alpha,

@@ -40,6 +40,7 @@ struct GemvQ8Params {
   const uint8_t* codes;       // [row tile][block]
   const uint8_t* staged;      // dY as operands of the MMAs (stage_columns_kernel)
   int rows, cols, blocks;     // features, outputs, blocks of tokens
+  int first;                  // CTAs of the launches before this one (set by the launch)
   float alpha, beta;
   void* c;
   long long c_row, c_col;
@@ -66,7 +67,8 @@ void launch_gemv_q4(int type, int group, int eights, const tcec_sm100::GemvQ4Par
 // spans: groups of 4-bit codes in a block, 0: 8-bit codes.  ctas: of a cluster.
 void launch_gemm_codes(bool f16, int spans, int bn, const tcec_sm100::GemmCodesParams& gp, int ctas, int grid, cudaStream_t stream);
 cudaError_t set_gemv_q4_attrs();
-void launch_gemv_q8(int type, int eights, const tcec_sm100::GemvQ8Params& p, cudaStream_t stream);
+// most_ctas > 0: no more than so many at a time.
+void launch_gemv_q8(int type, int eights, int most_ctas, const tcec_sm100::GemvQ8Params& p, cudaStream_t stream);
 cudaError_t set_gemv_q8_attrs();
 
 }  // namespace tcec_host

@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(32 * GemvQ8Cfg<kEights, kStrips>::MOST_WARPS, 
   }
   if (threadIdx.x == 0) abort_flag = 0;
   __syncthreads();
-  const int row0 = blockIdx.x * Cfg::ROWS;
+  const int row0 = (p.first + blockIdx.x) * Cfg::ROWS;
   const uint8_t* codes = p.codes + static_cast<size_t>(row0 / kCodeRows) * p.blocks * kQ8BlockBytes;
   auto fetch = [&](int kb, int stage) {  // a chunk a lane, and the scales
     if (dev_flag(p.debug_flags, 128) && blockIdx.x == 0 && kb == 0) return;

@@ -29,5 +29,10 @@ template <class... Params, class... Args>
 void launch_early(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
   launch_clusters(kernel, 0, grid, threads, smem, stream, args...);
 }
+// Launches a kernel that is not set up before the one in front of it has ended.
+template <class... Params, class... Args>
+void launch_late(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
+  kernel<<<grid, threads, smem, stream>>>(Params(args)...);
+}
 
 }  // namespace tcec_host
