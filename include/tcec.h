@@ -289,8 +289,10 @@ int tcec_unpack_q4(int layout_w, int n, int k, const void* packed, int group, vo
  * C (m x n) = alpha * X (m x k) * W^T + beta * C for weights packed as above: the product of a linear layer, from one token (a
  * matrix-vector product, bound by the 4-bit weights) to a whole prompt.  type_c is type_x or FP32.  `workspace` takes
  * tcec_gemm_q4_workspace_bytes(m, n, k, type_x) bytes, which is 0 up to one token (it may then be NULL).
- * The sum over a group of codes times X has to fit FP32.  Up to 32 tokens (FP32: 10) code and zero point are multiplied apart: the error is then
- * relative to the sum of |s| (q + z) |x| instead of |s| |q - z| |x|, and values of X of 2^122 and more count as infinite.
+ * The sums over a group of X, and of codes times X, have to fit FP32.  Up to 16 tokens, for n <= 8192 up to 32 (FP32: 10), code and zero point
+ * are multiplied apart: the error is then relative to the sum of |s| (q + z) |x| instead of |s| |q - z| |x|, values of X of 2^122 and more
+ * count as infinite, and a token with an infinite value is NaN throughout.  In products of more tokens it is infinite with the sign of
+ * s (q - z) x, and NaN where q = z.
  */
 size_t tcec_gemm_q4_workspace_bytes(int m, int n, int k, int type_x);
 int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, const void* x, long long ldx, int type_x,
@@ -310,8 +312,8 @@ int tcec_unpack_q8(int layout_x, int m, int k, const void* packed, void* x, long
 /*
  * C (n x k) = alpha * dY^T (n x m) * X (m x k) + beta * C for activations kept as above: the gradient of a layer's weights from the
  * gradient dY (m x n) of its outputs; beta = 1 adds up over several batches.  type_c is type_dy or FP32.
- * `workspace` takes tcec_wgrad_q8_workspace_bytes(m, n, k, type_dy) bytes.  The sum over a group of codes times dY has to fit FP32; up to 32 columns
- * of dY (FP32: 10) values of 2^122 and more count as infinite.
+ * `workspace` takes tcec_wgrad_q8_workspace_bytes(m, n, k, type_dy) bytes.  The sum over 128 tokens of codes times dY has to fit FP32.  Up to 16
+ * columns of dY, for k <= 2368 up to 32 (FP32: 10), values of 2^122 and more count as infinite.
  */
 size_t tcec_wgrad_q8_workspace_bytes(int m, int n, int k, int type_dy);
 int tcec_wgrad_q8(int layout_dy, int layout_c, int m, int n, int k, float alpha, const void* dy, long long lddy, int type_dy,

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_codes import BF16, DEV, F32, bound, check, randn, with_codes
+from test_gpu_codes import BF16, DEV, F16, F32, bound, check, randn, with_codes
 from wmma_extension_b200 import tcec
 
 pytestmark = pytest.mark.gpu
@@ -29,3 +29,52 @@ def test_tokens_up_to_2_27_and_beyond(m, dtype, group, alike):
         x = (base.double() * 2.0**exponent).to(dtype)
         exact = x.double() @ w.T
         check(tcec.gemm_q4(x, packed, n, group=group, dtype=F32), exact, bound(x.double().abs() @ sizes.T, exact, F32, k, 3 if dtype == F32 else 1))
+
+
+@pytest.mark.parametrize("m,dtype", [(1, F32), (1, F16), (1, BF16), (4, F32), (12, F16), (24, BF16)])
+def test_few_tokens_with_an_infinity_are_nan(m, dtype):
+    """As include/tcec.h says: code and zero point are multiplied apart, q * inf - z * inf; the other tokens keep their results."""
+    n, k = 40, 300
+    byte, s, z, w = with_codes(n, k, 64, 73)
+    z[5] = 0
+    packed = tcec.pack_q4_codes(byte, s, z, k=k, group=64)
+    x = randn(m, k, seed=m, dtype=dtype)
+    clean = tcec.gemm_q4(x, packed, n, group=64)
+    for value in (float("inf"), -float("inf")) if dtype == F16 else (float("inf"), -float("inf"), 2.0**122):
+        bad = x.clone()
+        bad[0, 70] = value
+        got = tcec.gemm_q4(bad, packed, n, group=64)
+        assert got[0].isnan().all() and torch.equal(got[1:], clean[1:])
+    if dtype != F16:  # the largest value below them counts
+        x[0, 70] = 2.0**122 * (1 - torch.finfo(dtype).eps)
+        assert tcec.gemm_q4(x, packed, n, group=64, dtype=F32)[0].isfinite().all()
+
+
+@pytest.mark.parametrize("m", [40, 300])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("group", [32, 128])
+def test_many_tokens_with_an_infinity_are_infinite(m, dtype, group):
+    n, k = 200, 300
+    byte, s, z, w = with_codes(n, k, group, 73)
+    packed = tcec.pack_q4_codes(byte, s, z, k=k, group=group)
+    x = randn(m, k, seed=m, dtype=dtype)
+    for value in (float("inf"), -float("inf")):
+        x[3, 70] = value
+        want = value * w[:, 70]  # NaN where the weight is 0
+        got = tcec.gemm_q4(x, packed, n, group=group)[3].double()
+        torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("n", [3, 9, 50])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_gradients_of_an_infinity_are_infinite(n, dtype):
+    m, k = 300, 200
+    x = randn(m, k, seed=n)
+    x[150, ::7] = 0.0
+    packed = tcec.pack_q8(x)
+    kept = tcec.unpack_q8(packed, m, k).double()
+    dy = randn(m, n, seed=n + 1, dtype=dtype)
+    for value in (float("inf"), -float("inf")):
+        dy[150, 2] = value
+        got = tcec.wgrad_q8(dy, packed, k)[2].double()
+        torch.testing.assert_close(got, value * kept[150], rtol=0, atol=0, equal_nan=True)

@@ -7,7 +7,8 @@
 // (or 16 times it, in the next four bits) times a power of two, subnormal or not; nothing is added or taken off.  The upper ones have an accumulator of
 // their own.  What the zero points take off is z times the sum of x over the group, and the power of two goes into the last factor.  (Codes made to
 // numbers first, by a magic number and a subtraction: an FP32 token times 16384 x 16384 in groups of 64 49 us instead of 45 at the time.)  How bf16
-// operands are kept from products below FP32: tcec_stage.cuh.  Values of 2^122 and more count as infinite.
+// operands are kept from products below FP32: tcec_stage.cuh.  Values of 2^122 and more count as infinite, and an infinite value makes NaN of its token's results
+// (q inf - z inf).
 //
 // Columns are tokens; an FP32 token takes three, its bf16 parts of 8 bits each, which together are exactly it.  Every product of a code and a part is
 // exact; a group's sum is made in the MMA's FP32 accumulator, then multiplied by its scale and added in FP32, rounded to nearest.  As code and zero
