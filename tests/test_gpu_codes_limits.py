@@ -78,3 +78,23 @@ def test_gradients_of_an_infinity_are_infinite(n, dtype):
         dy[150, 2] = value
         got = tcec.wgrad_q8(dy, packed, k)[2].double()
         torch.testing.assert_close(got, value * kept[150], rtol=0, atol=0, equal_nan=True)
+
+
+def test_sizes_that_are_no_extents_are_refused():
+    """Matrices without elements have such sizes too; 2^32 + 4 rows would be taken for four."""
+    many, none = 2**32 + 4, torch.empty(0, dtype=torch.uint8, device=DEV)
+    for call in (
+        lambda: tcec.gemm_q4(torch.empty(many, 0, dtype=BF16, device=DEV), none, 1),
+        lambda: tcec.gemm_q4(torch.empty(0, 4, dtype=BF16, device=DEV), none, many),
+        lambda: tcec.gemm_q4(torch.empty(0, 4, dtype=BF16, device=DEV), none, -1),
+        lambda: tcec.wgrad_q8(torch.empty(0, many, dtype=BF16, device=DEV), none, 1),
+        lambda: tcec.wgrad_q8(torch.empty(0, 4, dtype=BF16, device=DEV), none, many),
+        lambda: tcec.pack_q4(torch.empty(many, 0, device=DEV)),
+        lambda: tcec.pack_q8(torch.empty(0, many, device=DEV)),
+        lambda: tcec.pack_q4_codes(torch.empty(0, many // 2, dtype=torch.uint8, device=DEV), torch.empty(0, many // 128 + 1, dtype=F16, device=DEV), k=many),
+        lambda: tcec.unpack_q4(none, many, 0),
+        lambda: tcec.unpack_q8(none, 0, many),
+        lambda: tcec.unpack_q8(none, 4, -1),
+    ):
+        with pytest.raises(ValueError, match="2147483647"):
+            call()

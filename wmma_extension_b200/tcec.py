@@ -532,6 +532,12 @@ def _exact_result(c: Optional[torch.Tensor], shape, dtype: Optional[torch.dtype]
     return c
 
 
+def _require_extents(*sizes: int) -> None:
+    """The library counts rows and columns in 32 bits; ctypes would cut off the rest."""
+    if any(not 0 <= s <= 0x7FFFFFFF for s in sizes):
+        raise ValueError(f"sizes must be 0 to 2147483647, not {sizes}")
+
+
 def _require_bytes(t: torch.Tensor, need: int, what: str) -> None:
     if not t.is_cuda or not t.is_contiguous() or t.numel() * t.element_size() < need:
         raise ValueError(f"{what} takes {need} consecutive bytes on a GPU")
@@ -550,6 +556,7 @@ def q4_bytes(n: int, k: int, group: int = 128) -> int:
     """Bytes of weights (n x k) packed by pack_q4 or pack_q4_codes."""
     if group not in (32, 64, 128):
         raise ValueError("group must be 32, 64 or 128")
+    _require_extents(n, k)
     return int(load().tcec_q4_bytes(n, k, group))
 
 
@@ -644,6 +651,7 @@ def gemm_q4(x: torch.Tensor, packed: torch.Tensor, n: int, c: Optional[torch.Ten
             return _answer(done, "tcec_gemm_q4")
     kind = _dense_type(x, "x")
     m, k = x.shape
+    _require_extents(m)
     need = q4_bytes(n, k, group)
     _require_bytes(packed, need, "packed weights of this size")
     c = _exact_result(c, (m, n), dtype, x, beta)
@@ -663,6 +671,7 @@ def gemm_q4(x: torch.Tensor, packed: torch.Tensor, n: int, c: Optional[torch.Ten
 
 def q8_bytes(m: int, k: int) -> int:
     """Bytes of activations (m x k) packed by pack_q8."""
+    _require_extents(m, k)
     return int(load().tcec_q8_bytes(m, k))
 
 
@@ -719,6 +728,7 @@ def wgrad_q8(dy: torch.Tensor, packed: torch.Tensor, k: int, c: Optional[torch.T
             return _answer(done, "tcec_wgrad_q8")
     kind = _dense_type(dy, "dy")
     m, n = dy.shape
+    _require_extents(n)
     _require_bytes(packed, q8_bytes(m, k), "packed activations of this size")
     c = _exact_result(c, (n, k), dtype, dy, beta)
     kind_c = _result_type(c.dtype, dy)
