@@ -98,3 +98,15 @@ def test_sizes_that_are_no_extents_are_refused():
     ):
         with pytest.raises(ValueError, match="2147483647"):
             call()
+
+
+@pytest.mark.parametrize("alpha", [float("inf"), float("nan"), -3.0])
+@pytest.mark.parametrize("m", [1, 2, 12, 40])
+def test_a_sum_over_nothing_is_nothing_times_anything(alpha, m):
+    n = 150
+    c, none = randn(m, n, seed=m), torch.empty(0, dtype=torch.uint8, device=DEV)
+    want = 0.5 * c
+    assert torch.equal(tcec.gemm_q4(c[:, :0], none, n, c.clone(), alpha=alpha, beta=0.5), want)
+    assert torch.equal(tcec.gemm_q4(c[:, :0], none, n, alpha=alpha), torch.zeros(m, n, device=DEV))
+    assert torch.equal(tcec.wgrad_q8(c[:0, :m], none, n, c.clone(), alpha=alpha, beta=0.5), want)
+    assert torch.equal(tcec.wgrad_q8(c[:0, :m], none, n, alpha=alpha), torch.zeros(m, n, device=DEV))

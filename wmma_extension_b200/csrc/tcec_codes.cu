@@ -328,6 +328,7 @@ int tcec_gemm_q4(int layout_x, int layout_c, int m, int n, int k, float alpha, c
     if (dc.empty()) return TCEC_OK;
     if (dc.bad_memory()) return TCEC_ERR_INVALID_ARGUMENT;
     const int sum = alpha == 0.f ? 0 : k;  // as without a product, X and W are then not read
+    if (!sum) alpha = 0.f;                 // which may be no number, and times a sum over nothing is to be nothing
     const size_t scratch = sum ? tcec_gemm_q4_workspace_bytes(m, n, sum, type_x) : 0;
     if (sum) {
       if (dx.bad_memory() || !packed || !aligned(packed, 16) || workspace_bytes < scratch || (scratch && (!workspace || !aligned(workspace, 16))))
@@ -449,6 +450,7 @@ int tcec_wgrad_q8(int layout_dy, int layout_c, int m, int n, int k, float alpha,
     if (dc.empty()) return TCEC_OK;
     if (dc.bad_memory()) return TCEC_ERR_INVALID_ARGUMENT;
     const int sum = alpha == 0.f ? 0 : m;
+    if (!sum) alpha = 0.f;
     const size_t scratch = sum ? tcec_wgrad_q8_workspace_bytes(sum, n, k, type_dy) : 0;
     if (sum) {
       if (dd.bad_memory() || !packed || !aligned(packed, 16) || workspace_bytes < scratch || !workspace || !aligned(workspace, 16))
