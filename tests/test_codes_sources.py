@@ -44,3 +44,11 @@ def test_one_tokens_operands_are_handed_over_behind_a_warp_barrier():
     written = body.rindex("*reinterpret_cast<uint2*>(to")
     read = body.index("*reinterpret_cast<const uint4*>(x_shared", written)
     assert "__syncwarp();" in body[written:read]
+
+
+def test_indexes_at_the_largest_extents_stay_in_32_bits():
+    """With up to 2^31 - 1 rows or columns no sum of an extent or an index and something else may pass that: it would be negative, and taken for inside."""
+    bad = re.compile(r"\b[kf]0 \+ 4 <=|\+ kCodeRows - 1\) /|\(a \+ b - 1\) /|\+ Cfg::ROWS - 1\) /|- row0 \+ 15\)")
+    for file in ("tcec_codes.cuh", "tcec_gemv_q4.cu", "tcec_gemv_q4.cuh", "tcec_gemv_q8.cu", "tcec_gemv_q8.cuh"):
+        found = bad.findall(open(os.path.join(CSRC, file)).read())
+        assert not found, (file, found)

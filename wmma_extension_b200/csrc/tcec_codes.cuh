@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(256) unpack_q4_kernel(const UnpackParams p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = s * static_cast<float>(static_cast<int>((w >> ((j & 1) * 16 + (j >> 1) * 4)) & 15u) - z);
     const long long at = row * p.row_step + k0 * p.sum_step;
-    if (p.vec && k0 + 4 <= p.sum) {
+    if (p.vec && p.sum - k0 >= 4) {
       typename Element<kType>::type o[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = Element<kType>::put(v[j]);
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(256, 3) pack_q8_kernel(const PackQ8Params p) {
   __shared__ float4 most[8][32], scales[32], inverses[32];
   wait_for_launch_before();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tiles = (p.features + kCodeRows - 1) / kCodeRows, tile = blockIdx.x % tiles, tb = blockIdx.x / tiles;  // whole rows at a time
+  const int tiles = (p.features - 1) / kCodeRows + 1, tile = blockIdx.x % tiles, tb = blockIdx.x / tiles;  // whole rows at a time
   const int f0 = tile * kCodeRows + lane * 4, t0 = tb * kCodeSpan + warp * 16;
   float v[16][4];
   ld_lines4<kType, 16>(after_wait(p.x), t0 * p.token_step + f0 * p.feature_step, p.token_step, p.feature_step, p.tokens - t0, p.features - f0, p.vec, v);
@@ -470,7 +470,7 @@ template <int kType>
 __global__ void __launch_bounds__(256) unpack_q8_kernel(const UnpackParams p) {
   wait_for_launch_before();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tiles = (p.rows + kCodeRows - 1) / kCodeRows, tile = blockIdx.x % tiles, tb = blockIdx.x / tiles;
+  const int tiles = (p.rows - 1) / kCodeRows + 1, tile = blockIdx.x % tiles, tb = blockIdx.x / tiles;
   const uint8_t* block = after_wait(p.packed) + (static_cast<size_t>(tile) * p.blocks + tb) * kQ8BlockBytes;
   const int f0 = tile * kCodeRows + lane * 4, t0 = tb * kCodeSpan + warp * 16;
   const uint4 sc = ld_operand128(block + kQ8CodeBytes + lane * 16);
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(256) unpack_q8_kernel(const UnpackParams p) {
       v[j] = __fmaf_rn(s[j], code & 128u ? -q : q, 0.0f);  // no negative zeros
     }
     const long long at = f0 * p.row_step + token * p.sum_step;
-    if (p.vec && f0 + 4 <= p.rows) {
+    if (p.vec && p.rows - f0 >= 4) {
       typename Element<kType>::type o[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = Element<kType>::put(v[j]);

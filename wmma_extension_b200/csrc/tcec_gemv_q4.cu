@@ -9,7 +9,7 @@ using namespace tcec_sm100;
 namespace tcec_host {
 namespace {
 
-int ceil_div(int a, int b) { return (a + b - 1) / b; }
+int ceil_div(int a, int b) { return (a - 1) / b + 1; }  // a > 0
 // Launches for so many eights of columns and strips of rows a CTA, or (p null) allows the kernel its shared memory.
 template <int T, int G, int E, int S, bool One>
 cudaError_t one_gemv(const GemvQ4Params* p, cudaStream_t stream) {

@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(32 * GemvQ4Cfg<kType, kGroup, kEights, kStrips
     for (int i = lane; i < Cfg::X_BYTES / 16; i += 32) reinterpret_cast<uint4*>(x_shared)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   const int cta = blockIdx.x, strip0 = Cfg::SHARED_OUT ? cta * p.strips + min(cta, p.more) : cta * kStrips, row0 = strip0 * 16;
-  const int strips = Cfg::SHARED_OUT ? min(p.strips + (cta < p.more), (p.n - row0 + 15) / 16) : kStrips;
+  const int strips = Cfg::SHARED_OUT ? min(p.strips + (cta < p.more), (p.n - row0 - 1) / 16 + 1) : kStrips;
   constexpr size_t kBlockBytes = q4_block_bytes(kGroup);
   // strips of one tile of rows, or the last ones of one and the first ones of the next
   const uint32_t bytes = Cfg::SHARED_OUT ? min(strips, 8 - strip0 % 8) * q4_strip_bytes(kGroup) : Cfg::STAGE_BYTES;

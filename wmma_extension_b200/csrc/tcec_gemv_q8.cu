@@ -15,7 +15,7 @@ template <int T, int E, int S>
 cudaError_t one_gemv(const GemvQ8Params* p, int most_ctas, cudaStream_t stream) {
   using Cfg = GemvQ8Cfg<E, S>;
   if (!p) return cudaFuncSetAttribute(gemv_q8_kernel<T, E, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem_bytes(Cfg::MOST_WARPS));
-  const int ctas = (p->rows + Cfg::ROWS - 1) / Cfg::ROWS, most = most_ctas > 0 && most_ctas < ctas ? most_ctas : ctas;
+  const int ctas = (p->rows - 1) / Cfg::ROWS + 1, most = most_ctas > 0 && most_ctas < ctas ? most_ctas : ctas;
   const int warps = warps_of(most, Cfg::WARPS_OF_SM, 4, Cfg::MOST_WARPS);
   GemvQ8Params q = *p;
   for (q.first = 0; q.first < ctas; q.first += most) {
