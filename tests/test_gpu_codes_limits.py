@@ -110,3 +110,66 @@ def test_a_sum_over_nothing_is_nothing_times_anything(alpha, m):
     assert torch.equal(tcec.gemm_q4(c[:, :0], none, n, alpha=alpha), torch.zeros(m, n, device=DEV))
     assert torch.equal(tcec.wgrad_q8(c[:0, :m], none, n, c.clone(), alpha=alpha, beta=0.5), want)
     assert torch.equal(tcec.wgrad_q8(c[:0, :m], none, n, alpha=alpha), torch.zeros(m, n, device=DEV))
+
+
+def test_the_first_call_is_not_captured():
+    """It is refused, and the next one outside works.  In a process of its own, as others have called before."""
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from wmma_extension_b200 import tcec
+w = torch.full((128, 128), 15.0, device="cuda")  # a scale of 1
+torch.cuda.synchronize()
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        tcec.pack_q4(w)
+except (tcec.TcecError, RuntimeError) as e:
+    print("refused", type(e).__name__)
+for i in range(2):
+    try:
+        assert torch.equal(tcec.unpack_q4(tcec.pack_q4(w), 128, 128), w)
+        print("worked", i)
+    except Exception as e:
+        print("failed", i, repr(e))
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert "refused" in run.stdout and "worked 1" in run.stdout, (run.stdout, run.stderr)
+
+
+# The last of the three bf16 parts of an FP32 value holds up to 2^-16 of it.  Where all values have it in full, and all terms have one sign, a product without it is off
+# by nearly 2^-16 of their sum, and bound() allows 2^-17.2 at 256 terms.
+def last_part_in_full(*shape, seed):
+    return ((randn(*shape, seed=seed).abs() + 0.5).view(torch.int32) | 0x7F).view(F32)
+
+
+def without_last_part(t):
+    return (t.view(torch.int32) & ~0x7F).view(F32).double()
+
+
+@pytest.mark.parametrize("m", [1, 5, 10, 40, 300])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_products_have_all_parts_of_fp32_tokens(m, group):
+    n, k = 136, 256
+    byte, s, z, w = with_codes(n, k, group, 75)
+    z.zero_()
+    w = torch.stack([byte & 15, byte >> 4], 2).reshape(n, -1).double() * s.double()[:, torch.arange(k, device=DEV) // group]
+    packed = tcec.pack_q4_codes(byte, s, z, k=k, group=group)
+    x = last_part_in_full(m, k, seed=m)
+    exact = x.double() @ w.T
+    tol = bound(exact, exact, F32, k, 3)
+    assert ((without_last_part(x) @ w.T - exact).abs() > 1.5 * tol).all()  # this would be noticed
+    check(tcec.gemm_q4(x, packed, n, group=group), exact, tol)
+
+
+@pytest.mark.parametrize("n", [2, 10, 40, 300])
+def test_gradients_have_all_parts_of_fp32(n):
+    m, k = 256, 200
+    packed = tcec.pack_q8(randn(m, k, seed=n).abs())
+    kept = tcec.unpack_q8(packed, m, k).double()
+    dy = last_part_in_full(m, n, seed=n + 1)
+    exact = dy.double().T @ kept
+    tol = bound(exact, exact, F32, m, 3)
+    assert ((without_last_part(dy).T @ kept - exact).abs() > 1.5 * tol).all()
+    check(tcec.wgrad_q8(dy, packed, k), exact, tol)
