@@ -135,7 +135,7 @@ for i in range(2):
         print("failed", i, repr(e))
 """
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
-    assert "refused" in run.stdout and "worked 1" in run.stdout, (run.stdout, run.stderr)
+    assert "refused" in run.stdout and "worked 0" in run.stdout and "worked 1" in run.stdout, (run.stdout, run.stderr)
 
 
 # The last of the three bf16 parts of an FP32 value holds up to 2^-16 of it.  Where all values have it in full, and all terms have one sign, a product without it is off

@@ -5,7 +5,7 @@
 //            z = clamp(rint(-lo / s), 0, 15);  q = clamp(rint(w / s) + z, 0, 15);  w^ = s (q - z)
 //   8 bits:  s = max(RN32(max |x| / 127), 2^-120);  q = rint(x / s);  x^ = s q
 //
-// rint is of the exact quotient, ties to even (rint_quotient).  A group with a value that is not finite (or, with f16 scales,
+// rint is of the exact quotient, ties to even (Quotient).  A group with a value that is not finite (or, with f16 scales,
 // whose scale would not be) has the scale NaN, and so has all that is computed from it.
 //
 // Both are kept in blocks of 128 rows x 128 of the axis that the products sum over ("rows": n for weights, features for

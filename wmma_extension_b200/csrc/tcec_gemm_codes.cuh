@@ -14,10 +14,12 @@
 // The dense operand is first laid out in panels (stage_panels_kernel), whatever its type, order and alignment: 128 columns x 32 of the
 // sum x 2 bytes in the core-matrix order that the MMA reads, so that the product brings them in with linear bulk copies.
 //
-// Bound by shared memory: a block of 128 x 128 codes and 128 columns moves 64 KB to the MMAs, 33 of expanded codes and 40 of copies in, and 8 out to
-// the converters, 1130 cycles at 128 bytes each; its MMAs take 520.  Tiles of 256 x 256 on two SMs do twice as many products with the same (1024
-// cycles of MMAs).  Measured: 512 tokens times 4096 x 4096, 128 tiles of 32 blocks, 25.5 us (670 TFLOP/s), 1000 tokens on pairs 38.8 (860), 8192 x 4096 x 4096
-// gradient 262 alone (1050).  Groups of 32 have four accumulators a block to fold, FP32 three times as many: 512 tokens 44 us, FP32 103, in groups of 128 56.
+// A block of 128 x 128 codes and 128 columns moves 64 KB through shared memory to the MMAs, 33 of expanded codes and 40 of copies in, and 8 out to the
+// converters, 1130 cycles at 128 bytes each, while its MMAs take 520; tiles of 256 x 256 on two SMs do twice as many products with the same (1024 cycles of
+// MMAs).  That is not all that bounds the pairs: by counters the 8192 x 4096 x 4096 gradient keeps the tensor pipe busy for half of the time and no other unit for
+// longer, 1000 tokens times 4096 x 4096 for a third, so what is left lies between the roles below.  Measured in a row, with the staging: 512 tokens times 4096 x 4096,
+// 128 tiles of 32 blocks, 25.2 us (680 TFLOP/s), 1000 tokens on pairs 39.5 (850), 8192 x 4096 x 4096 gradient 308 at the power cap (890; the kernel alone 280).
+// Groups of 32 have four accumulators a block to fold, FP32 three times as many: 512 tokens 44 us, FP32 103, in groups of 128 56.
 // Few columns: by the codes' way from memory to operands; 8192 x 4096 gradient of rank 48 18.7 us (1.8 TB/s), 64 tokens times 4096 x 4096 12.9.
 #pragma once
 #include "tcec_codes.cuh"

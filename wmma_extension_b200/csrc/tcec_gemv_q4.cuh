@@ -17,7 +17,7 @@
 // A CTA takes up to kStrips strips of 16 rows; its warps divide k block by block and add up through shared memory in a fixed order.  One strip after the other, the
 // operands of the columns stay in registers: 16384 x 16384 with 16 tokens 45.6 us, strips side by side 53.8, with one FP32 token (groups of 64) 35 and 42.
 //
-// Measured, from memory: one bf16 token times 4096 x 4096 4.9 us (1.8 TB/s: 32 rows of blocks an SM are over before the copies are up to speed), times
+// Measured, from memory, of calls in a row: one bf16 token times 4096 x 4096 5.3 us (the kernel 4.6, 2.0 TB/s: 32 rows of blocks an SM are over before the copies are up to speed), times
 // 16384 x 16384 29.3 (4.9 TB/s), FP32 in groups of 64 33.8 (4.5 TB/s); 8 tokens 28 us, 16 46, 10 of FP32 94.
 #pragma once
 #include "tcec_gemm_codes.cuh"
