@@ -173,3 +173,42 @@ def test_gradients_have_all_parts_of_fp32(n):
     tol = bound(exact, exact, F32, m, 3)
     assert ((without_last_part(dy).T @ kept - exact).abs() > 1.5 * tol).all()
     check(tcec.wgrad_q8(dy, packed, k), exact, tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("step", [1, 3])
+def test_one_token_and_one_output_as_columns_of_a_matrix(dtype, step):
+    """A row whose elements lie `step` apart or more: x of one token, dY of one output, and results between other columns."""
+    n, k = 150, 333
+    byte, s, z, w = with_codes(n, k, 64, 77)
+    packed = tcec.pack_q4_codes(byte, s, z, k=k, group=64)
+    x = torch.full((k, step), float("nan"), device=DEV, dtype=dtype)
+    x[:, step - 1] = randn(k, seed=78, dtype=dtype)
+    row = x[:, step - 1:].T
+    exact = row.double() @ w.T
+    c = torch.full((n, 5), 7.0, device=DEV)
+    tcec.gemm_q4(row, packed, n, c[:, 2:3].T, group=64)
+    q = torch.stack([byte & 15, byte >> 4], 2).reshape(n, -1)[:, :k].double()
+    each = torch.arange(k, device=DEV) // 64
+    sizes = (q + z.double()[:, each]) * s.double()[:, each]
+    check(c[:, 2:3].T, exact, bound(row.double().abs() @ sizes.T, exact, F32, k, 3 if dtype == F32 else 1))
+    assert (c[:, [0, 1, 3, 4]] == 7.0).all()
+    kept = tcec.pack_q8(randn(k, n, seed=79))
+    values = tcec.unpack_q8(kept, k, n).double()
+    g = torch.full((n, 5), 7.0, device=DEV)
+    tcec.wgrad_q8(x[:, step - 1:], kept, n, g[:, 3:4].T)
+    exact = row.double() @ values
+    check(g[:, 3:4].T, exact, bound(row.double().abs() @ values.abs(), exact, F32, k, 3 if dtype == F32 else 1))
+    assert (g[:, [0, 1, 2, 4]] == 7.0).all()
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (130, 333), (257, 128)])
+def test_codes_between_other_bytes_are_laid_out(n, k):
+    byte, s, z, w = with_codes(n, k, 32, 81, BF16)
+    wide = torch.full((n, byte.shape[1] + 3), 0xFF, dtype=torch.uint8, device=DEV)
+    wide[:, 1:-2] = byte
+    packed = tcec.pack_q4_codes(wide[:, 1:-2], s, z, k=k, group=32)
+    assert torch.equal(packed, tcec.pack_q4_codes(byte, s, z, k=k, group=32))
+    turned = byte.T.contiguous().T  # columns first: copied
+    assert torch.equal(packed, tcec.pack_q4_codes(turned, s, z, k=k, group=32))
+    assert torch.equal(tcec.unpack_q4(packed, n, k, group=32).double(), w)
