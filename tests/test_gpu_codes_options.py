@@ -59,3 +59,26 @@ def test_prompts_leave_sms_to_others():
     finally:
         tcec.set_option("reserve_sms", 0)
     assert len(seen) == 2 and max(seen) <= sms - 20, seen
+
+
+def test_gradients_in_several_launches_are_captured_and_replayed():
+    dy, packed, exact, tol = gradient_case(1000, 16, 16500, BF16, 83, F32)
+    c = torch.zeros(16, 16500, device=dy.device)
+    tcec.wgrad_q8(dy, packed, 16500, c)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    tcec.set_option("reserve_sms", 20)
+    try:
+        tcec.wgrad_q8(dy, packed, 16500, c.zero_())
+        once = c.clone()
+        with torch.cuda.graph(graph):
+            tcec.wgrad_q8(dy, packed, 16500, c)
+            tcec.wgrad_q8(dy, packed, 16500, c, beta=1.0)
+    finally:
+        tcec.set_option("reserve_sms", 0)
+    check(once, exact, tol)
+    for _ in range(3):
+        c.zero_()
+        graph.replay()
+        assert torch.equal(c, once + once)
+    tcec.device_status()
